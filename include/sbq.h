@@ -365,6 +365,94 @@ SBQ_API int sbq_linear_dyn_noalloc(const void* x, int x_dtype, int64_t ldx, int 
                                    const int32_t* rowsum, const float* scale, const float* bias, int64_t m,
                                    int64_t n, int64_t k, float* y, int64_t ldy, void* stream);
 
+/* ---- 4-bit weights with group scales --------------------------------------------------------
+ *
+ * w[n, k] = q[n, k] * s[n, k / group]: q an integer in [-8, 7], s bf16, group 32, 64 or 128 input
+ * features (the last group of a row may be short).  No counterpart in the reference.  A weight is three
+ * device buffers: `packed` (sbq_w4_packed_bytes; 16 x 128 tiles of 1 KiB), `scales` (sbq_w4_scale_bytes;
+ * bf16, tile by tile) and `rowmul` (fp32, n rounded up to 16), both first ones 256-byte aligned. */
+SBQ_API size_t sbq_w4_packed_bytes(int64_t n, int64_t k);
+SBQ_API size_t sbq_w4_scale_bytes(int64_t n, int64_t k, int group);
+
+/* s = bf16(max(max|w|, 1e-8) / 7) per row and group, q = clamp(rint(w / s), -7, 7), packed.  w is [n, k]
+ * with row stride ldw, SBQ_F32, SBQ_F16 or SBQ_BF16. */
+SBQ_API int sbq_w4_quantize_pack(const void* w, int w_dtype, int64_t n, int64_t k, int64_t ldw, int group,
+                                 void* packed, void* scales, float* rowmul, void* stream);
+
+/* Given codes q (int8 [n, k], row stride ldq; values outside [-8, 7] are clamped) and scales (bf16
+ * [n, ceil(k / group)], row stride lds, finite) -> packed. */
+SBQ_API int sbq_w4_pack(const int8_t* q, int64_t ldq, const void* scale, int64_t lds, int64_t n, int64_t k,
+                        int group, void* packed, void* scales, float* rowmul, void* stream);
+
+/* Packed -> q and scale as sbq_w4_pack takes them (either may be NULL). */
+SBQ_API int sbq_w4_unpack(const void* packed, const void* scales, int64_t n, int64_t k, int group, int8_t* q,
+                          int64_t ldq, void* scale, int64_t lds, void* stream);
+
+/* Workspace of sbq_linear_w4 / sbq_mlp_gateup_w4 for x [m, k]: the activation's fp16 parts (fp32 x at
+ * every m, bf16 x above 16 rows), 0 otherwise. */
+SBQ_API size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t k, int x_dtype);
+
+/* y[m, n] = sum_k x[m, k] * q[n, k] * s[n, k / group] (+ bias[n]); x and y SBQ_F32, SBQ_F16 or SBQ_BF16.
+ * q * s enters the product exactly, bf16 x too, fp32 x with 22 bits; sums are fp32.  Up to 16 rows: the
+ * decode product; above: the tensor-memory product.  k a multiple of 16 (zero-fill x past the weight's own
+ * k), x rows 16-byte aligned, workspace 256-byte aligned (NULL when its size is 0). */
+SBQ_API int sbq_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* packed, const void* scales,
+                          const float* rowmul, int group, const float* bias, int64_t m, int64_t n, int64_t k, void* y,
+                          int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
+
+/* h[m, n] = silu(gate) * up, gate and up as sbq_linear_w4 without bias (GatedMLP.forward's first half,
+ * model.py:239-240), in one launch (and the one that makes the activation's parts). */
+SBQ_API int sbq_mlp_gateup_w4(const void* x, int x_dtype, int64_t ldx, const void* packed_gate,
+                              const void* scales_gate, const float* rowmul_gate, const void* packed_up,
+                              const void* scales_up, const float* rowmul_up, int group, int64_t m, int64_t n, int64_t k,
+                              void* h, int h_dtype, int64_t ldh, void* workspace, size_t workspace_bytes, void* stream);
+
+/* ---- the step between two blocks --------------------------------------------------------------
+ *
+ *   h   = branch, or branch * rsqrt(mean(branch^2) + eps) * post_weight     (post_weight set)
+ *   r'  = residual_scale * residual + branch_scale * act(gate) * h          (act(gate) = 1 without a gate)
+ *   out = r' * rsqrt(mean(r'^2) + eps) * pre_weight                         (from r' before it is rounded)
+ *
+ * over rows of d elements (RMSNorm, model.py:30-39; the additions of Block.forward, model.py:388-392).
+ * branch may be NULL (r' = residual_scale * residual), residual_out may be NULL, or the residual itself; out
+ * and pre_weight are both set or both NULL; out may be the branch (same type and stride).  Other overlaps
+ * are not allowed.  branch, residual (and residual_out, of its type), gate and out: SBQ_F32, SBQ_F16 or
+ * SBQ_BF16, any row stride; weights fp32 [d].  gate: [d] (SBQ_GATE_PER_COLUMN), one per row at stride ld_gate
+ * (SBQ_GATE_PER_ROW) or [m, d] (SBQ_GATE_FULL). */
+#define SBQ_GATE_NONE 0
+#define SBQ_GATE_SIGMOID 1
+#define SBQ_GATE_SILU 2
+#define SBQ_GATE_TANH 3
+#define SBQ_GATE_PER_COLUMN 0
+#define SBQ_GATE_PER_ROW 1
+#define SBQ_GATE_FULL 2
+typedef struct sbq_residual_norm_args {
+    const void* branch;
+    int64_t ld_branch;
+    const void* residual;
+    int64_t ld_residual;
+    const void* gate;
+    int64_t ld_gate;
+    const float* post_weight;
+    const float* pre_weight;
+    void* residual_out;
+    int64_t ld_residual_out;
+    void* out;
+    int64_t ld_out;
+    int64_t m;
+    int64_t d;
+    int branch_dtype;
+    int residual_dtype;
+    int gate_dtype;
+    int out_dtype;
+    int gate_mode;
+    int gate_act;
+    float residual_scale;
+    float branch_scale;
+    float eps;
+} sbq_residual_norm_args;
+SBQ_API int sbq_residual_norm(const sbq_residual_norm_args* args, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -42,6 +42,22 @@ class PeerGroup(ctypes.Structure):
                 ("wait_state", ctypes.c_void_p), ("wait_expected", ctypes.c_uint), ("wait_limit_ns", ctypes.c_ulonglong)]
 
 
+class ResidualNormArgs(ctypes.Structure):
+    """struct sbq_residual_norm_args of include/sbq.h."""
+
+    _fields_ = [("branch", ctypes.c_void_p), ("ld_branch", ctypes.c_int64), ("residual", ctypes.c_void_p),
+                ("ld_residual", ctypes.c_int64), ("gate", ctypes.c_void_p), ("ld_gate", ctypes.c_int64),
+                ("post_weight", ctypes.c_void_p), ("pre_weight", ctypes.c_void_p), ("residual_out", ctypes.c_void_p),
+                ("ld_residual_out", ctypes.c_int64), ("out", ctypes.c_void_p), ("ld_out", ctypes.c_int64),
+                ("m", ctypes.c_int64), ("d", ctypes.c_int64), ("branch_dtype", ctypes.c_int),
+                ("residual_dtype", ctypes.c_int), ("gate_dtype", ctypes.c_int), ("out_dtype", ctypes.c_int),
+                ("gate_mode", ctypes.c_int), ("gate_act", ctypes.c_int), ("residual_scale", ctypes.c_float),
+                ("branch_scale", ctypes.c_float), ("eps", ctypes.c_float)]
+
+
+GATE_ACTS = {"none": 0, "sigmoid": 1, "silu": 2, "tanh": 3}
+GATE_PER_COLUMN, GATE_PER_ROW, GATE_FULL = range(3)
+
 # name -> (restype, argtypes); kept in the order of include/sbq.h
 SIGNATURES = {
     "sbq_version": (_c_int, []),
@@ -95,6 +111,17 @@ SIGNATURES = {
                                 _vp, _sz, _vp]),
     "sbq_linear_dyn_noalloc": (_c_int, [_vp, _c_int, _c_i64, _c_int, _vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp,
                                         _c_i64, _vp]),
+    "sbq_w4_packed_bytes": (_sz, [_c_i64, _c_i64]),
+    "sbq_w4_scale_bytes": (_sz, [_c_i64, _c_i64, _c_int]),
+    "sbq_w4_quantize_pack": (_c_int, [_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_int, _vp, _vp, _vp, _vp]),
+    "sbq_w4_pack": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_int, _vp, _vp, _vp, _vp]),
+    "sbq_w4_unpack": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_int, _vp, _c_i64, _vp, _c_i64, _vp]),
+    "sbq_linear_w4_workspace_bytes": (_sz, [_c_i64, _c_i64, _c_int]),
+    "sbq_linear_w4": (_c_int, [_vp, _c_int, _c_i64, _vp, _vp, _vp, _c_int, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_int,
+                               _c_i64, _vp, _sz, _vp]),
+    "sbq_mlp_gateup_w4": (_c_int, [_vp, _c_int, _c_i64, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _vp,
+                                   _c_int, _c_i64, _vp, _sz, _vp]),
+    "sbq_residual_norm": (_c_int, [ctypes.POINTER(ResidualNormArgs), _vp]),
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -1,0 +1,205 @@
+// Entry points of the 4-bit format: argument checks, the activation's 16-bit parts, and the choice of
+// kernel (decode product up to 16 rows).
+#include <atomic>
+
+#include "w4_host.cuh"
+
+namespace sbq {
+
+// SMs of the current device, cached per device.
+int w4_sm_count() {
+    static std::atomic<int> count[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 148;
+    int c = count[dev].load(std::memory_order_relaxed);
+    if (c == 0) {
+        cudaDeviceGetAttribute(&c, cudaDevAttrMultiProcessorCount, dev);
+        c = c > 0 ? c : 148;
+        count[dev].store(c, std::memory_order_relaxed);
+    }
+    return c;
+}
+
+// ---- activation parts ------------------------------------------------------------------------------
+// Row r of x times 2^(14 - e), 2^e <= max |x[r]| < 2^(e + 1) over its finite values, as fp16 (bf16 x:
+// exact unless an element is below 2^-31 of the row's largest) or as two fp16 parts hi + lo (fp32 x: 22
+// bits, the difference x - hi is exact).  Infinities and NaN stay what they are.  inv[r] = 2^(e - 14).
+constexpr int kActThreads = 256;
+
+struct ActParams {
+    const void* x;
+    int64_t ldx;
+    __half* hi;
+    __half* lo;  // null for bf16 x
+    float* inv;
+    int k;       // a multiple of 16
+};
+
+template <bool F32>
+__device__ __forceinline__ void act_load8(const void* x, int64_t i, float (&v)[8]) {
+    if (F32) {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(x) + i);
+        const float4 a = q[0], b = q[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+    } else {
+        const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(x) + i);
+        const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            v[2 * j] = __uint_as_float(u[j] << 16);
+            v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
+        }
+    }
+}
+
+template <bool F32>
+__global__ void __launch_bounds__(kActThreads) w4_acts_kernel(const ActParams p) {
+    __shared__ float part[kActThreads / 32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int64_t row = blockIdx.x, x0 = row * p.ldx, o0 = row * p.k;
+    float big = 0.0f;
+    for (int c = threadIdx.x * 8; c < p.k; c += kActThreads * 8) {
+        float v[8];
+        act_load8<F32>(p.x, x0 + c, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (isfinite(v[i])) big = fmaxf(big, fabsf(v[i]));
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = big;
+    __syncthreads();
+    big = part[0];
+#pragma unroll
+    for (int i = 1; i < kActThreads / 32; ++i) big = fmaxf(big, part[i]);
+    // exponents clamped so that both the factor and its inverse are normal numbers
+    int e = big > 0.0f ? 14 - ilogbf(big) : 0;
+    e = e > 126 ? 126 : e < -126 ? -126 : e;
+    const float mul = scalbnf(1.0f, e);
+    if (threadIdx.x == 0) p.inv[row] = scalbnf(1.0f, -e);
+    for (int c = threadIdx.x * 8; c < p.k; c += kActThreads * 8) {
+        float v[8];
+        act_load8<F32>(p.x, x0 + c, v);
+        uint32_t h[4], l[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const float a = v[2 * j] * mul, b = v[2 * j + 1] * mul;
+            const __half2 hh = __floats2half2_rn(a, b);
+            h[j] = *reinterpret_cast<const uint32_t*>(&hh);
+            if (F32) {
+                const float2 hf = __half22float2(hh);
+                // an infinity has no low part (inf - inf)
+                const __half2 ll = __floats2half2_rn(isinf(a) ? 0.0f : a - hf.x, isinf(b) ? 0.0f : b - hf.y);
+                l[j] = *reinterpret_cast<const uint32_t*>(&ll);
+            }
+        }
+        *reinterpret_cast<uint4*>(p.hi + o0 + c) = make_uint4(h[0], h[1], h[2], h[3]);
+        if (F32) *reinterpret_cast<uint4*>(p.lo + o0 + c) = make_uint4(l[0], l[1], l[2], l[3]);
+    }
+}
+
+constexpr int64_t kW4GemvRows = 16;  // up to this many rows: the decode product
+
+static size_t align256(size_t v) { return (v + 255) & ~size_t(255); }
+
+static bool w4_needs_parts(int64_t m, int x_dtype) {
+    return x_dtype == SBQ_F32 || (x_dtype == SBQ_BF16 && m > kW4GemvRows);
+}
+
+static int check_w4_call(const void* x, int x_dtype, int64_t ldx, const W4Call& c, int group, int nmat) {
+    if (!x || !c.y) return set_error(SBQ_ERR_INVALID_ARGUMENT, "null pointer");
+    for (int i = 0; i < nmat; ++i) {
+        if (!c.w[i].packed || !c.w[i].scales || !c.w[i].rowmul) return set_error(SBQ_ERR_INVALID_ARGUMENT, "null pointer");
+        if (reinterpret_cast<uintptr_t>(c.w[i].packed) % 256 || reinterpret_cast<uintptr_t>(c.w[i].scales) % 256)
+            return set_error(SBQ_ERR_ALIGNMENT, "packed weight and scales must be 256-byte aligned");
+    }
+    if (c.m <= 0 || c.n <= 0 || c.k <= 0)
+        return set_error(SBQ_ERR_INVALID_ARGUMENT, "m, n, k must be positive (m=%lld n=%lld k=%lld)", (long long)c.m,
+                         (long long)c.n, (long long)c.k);
+    if (!c.gpt) return set_error(SBQ_ERR_UNSUPPORTED, "group size %d (32, 64, 128)", group);
+    if (x_dtype != SBQ_F32 && x_dtype != SBQ_F16 && x_dtype != SBQ_BF16)
+        return set_error(SBQ_ERR_UNSUPPORTED, "activation dtype %d (f16, bf16, f32)", x_dtype);
+    if (c.y_dtype != SBQ_F32 && c.y_dtype != SBQ_F16 && c.y_dtype != SBQ_BF16)
+        return set_error(SBQ_ERR_UNSUPPORTED, "output dtype %d (f32, f16, bf16)", c.y_dtype);
+    if (ldx < c.k || c.ldy < c.n) return set_error(SBQ_ERR_INVALID_ARGUMENT, "row stride smaller than the row");
+    if (c.k % 16) return set_error(SBQ_ERR_UNSUPPORTED, "k must be a multiple of 16 (k=%lld)", (long long)c.k);
+    if (reinterpret_cast<uintptr_t>(x) % 16 || (ldx * w4_elem(x_dtype)) % 16)
+        return set_error(SBQ_ERR_ALIGNMENT, "activation rows must be 16-byte aligned");
+    if (reinterpret_cast<uintptr_t>(c.y) % w4_elem(c.y_dtype))
+        return set_error(SBQ_ERR_ALIGNMENT, "output must be aligned to its element size");
+    if (c.n > (int64_t(1) << 31) - 256 || c.k >= (int64_t(1) << 30) || c.m > (int64_t(1) << 31) - 256)
+        return set_error(SBQ_ERR_UNSUPPORTED, "shape too large");
+    return SBQ_OK;
+}
+
+static int w4_run(const void* x, int x_dtype, int64_t ldx, const W4Call& c, int group, int nmat, void* workspace,
+                  size_t workspace_bytes) {
+    int st = check_w4_call(x, x_dtype, ldx, c, group, nmat);
+    if (st) return st;
+    W4Acts a{};
+    a.bf16 = x_dtype == SBQ_BF16;
+    a.part[0] = x;
+    a.ld = ldx;
+    if (w4_needs_parts(c.m, x_dtype)) {
+        const size_t need = sbq_linear_w4_workspace_bytes(c.m, c.k, x_dtype);
+        if (!workspace) return set_error(SBQ_ERR_INVALID_ARGUMENT, "this activation type needs a workspace of %zu bytes", need);
+        if (reinterpret_cast<uintptr_t>(workspace) % 256)
+            return set_error(SBQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
+        if (workspace_bytes < need) return set_error(SBQ_ERR_WORKSPACE, "workspace needs %zu bytes", need);
+        const size_t one = align256((size_t)c.m * c.k * 2);
+        uint8_t* ws = static_cast<uint8_t*>(workspace);
+        ActParams p{};
+        p.x = x;
+        p.ldx = ldx;
+        p.hi = reinterpret_cast<__half*>(ws);
+        p.lo = x_dtype == SBQ_F32 ? reinterpret_cast<__half*>(ws + one) : nullptr;
+        p.inv = reinterpret_cast<float*>(ws + (x_dtype == SBQ_F32 ? 2 : 1) * one);
+        p.k = (int)c.k;
+        const cudaError_t e = x_dtype == SBQ_F32 ? w4_launch(w4_acts_kernel<true>, (unsigned)c.m, kActThreads, 0, c.stream, p)
+                                                 : w4_launch(w4_acts_kernel<false>, (unsigned)c.m, kActThreads, 0, c.stream, p);
+        if (e != cudaSuccess) return set_error(SBQ_ERR_CUDA, "w4 activation parts launch: %s", cudaGetErrorString(e));
+        a.part[0] = p.hi;
+        a.part[1] = p.lo;
+        a.ld = c.k;
+        a.inv = p.inv;
+        a.bf16 = false;
+    }
+    return gemv_w4_run(c, a);
+}
+
+}  // namespace sbq
+
+using namespace sbq;
+
+extern "C" size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t k, int x_dtype) {
+    if (m <= 0 || k <= 0 || !w4_needs_parts(m, x_dtype)) return 0;
+    return (x_dtype == SBQ_F32 ? 2 : 1) * align256((size_t)m * k * 2) + align256((size_t)m * 4);
+}
+
+extern "C" int sbq_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* packed, const void* scales,
+                             const float* rowmul, int group, const float* bias, int64_t m, int64_t n, int64_t k, void* y,
+                             int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {
+    W4Call c{};
+    c.w[0] = {static_cast<const uint8_t*>(packed), static_cast<const __nv_bfloat16*>(scales), rowmul};
+    c.gpt = w4_groups_per_tile(group);
+    c.bias = bias;
+    c.m = m, c.n = n, c.k = k;
+    c.y = y, c.y_dtype = y_dtype, c.ldy = ldy;
+    c.stream = static_cast<cudaStream_t>(stream);
+    return w4_run(x, x_dtype, ldx, c, group, 1, workspace, workspace_bytes);
+}
+
+extern "C" int sbq_mlp_gateup_w4(const void* x, int x_dtype, int64_t ldx, const void* packed_gate,
+                                 const void* scales_gate, const float* rowmul_gate, const void* packed_up,
+                                 const void* scales_up, const float* rowmul_up, int group, int64_t m, int64_t n, int64_t k,
+                                 void* h, int h_dtype, int64_t ldh, void* workspace, size_t workspace_bytes, void* stream) {
+    W4Call c{};
+    c.w[0] = {static_cast<const uint8_t*>(packed_gate), static_cast<const __nv_bfloat16*>(scales_gate), rowmul_gate};
+    c.w[1] = {static_cast<const uint8_t*>(packed_up), static_cast<const __nv_bfloat16*>(scales_up), rowmul_up};
+    c.gpt = w4_groups_per_tile(group);
+    c.m = m, c.n = n, c.k = k;
+    c.y = h, c.y_dtype = h_dtype, c.ldy = ldh;
+    c.stream = static_cast<cudaStream_t>(stream);
+    return w4_run(x, x_dtype, ldx, c, group, 2, workspace, workspace_bytes);
+}

@@ -1,0 +1,64 @@
+// What the 4-bit entry points and kernels share on the host, and the device helpers of their epilogues.
+#pragma once
+
+#include "w4.cuh"
+
+namespace sbq {
+
+// One checked call of sbq_linear_w4 (w[1] null) or sbq_mlp_gateup_w4.
+struct W4Call {
+    W4Weight w[2];
+    int gpt;  // groups per 128-column tile
+    const float* bias;
+    int64_t m, n, k;
+    void* y;
+    int y_dtype;
+    int64_t ldy;
+    cudaStream_t stream;
+};
+
+// The activation as the kernels read it: 16-bit parts [m, k] with row stride ld.  fp16 and bf16 inputs
+// are read in place; the parts of an fp32 input (and of a bf16 input above 16 rows) are fp16 made by
+// w4_prepare_acts, each row multiplied by a power of two whose inverse is inv[row].
+struct W4Acts {
+    const void* part[2];
+    int64_t ld;
+    const float* inv;
+    bool bf16;
+};
+
+int gemv_w4_run(const W4Call& c, const W4Acts& x);
+int w4_sm_count();
+
+inline int w4_elem(int dtype) { return dtype == SBQ_F32 ? 4 : 2; }
+
+// A launch as a programmatic dependent of the previous kernel on the stream.  Each kernel launched
+// this way reads nothing but packed weights before its griddepcontrol.wait and lets its own dependents
+// begin only after that wait.
+template <class K, class P>
+cudaError_t w4_launch(K kernel, dim3 grid, unsigned block, size_t smem, cudaStream_t s, const P& p) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(block);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+__device__ __forceinline__ float w4_silu(float v) { return v / (1.0f + expf(-v)); }
+
+__device__ __forceinline__ void w4_store(void* y, int dtype, int64_t i, float v) {
+    if (dtype == SBQ_F32)
+        static_cast<float*>(y)[i] = v;
+    else if (dtype == SBQ_F16)
+        static_cast<__half*>(y)[i] = __float2half_rn(v);
+    else
+        static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
+}
+
+}  // namespace sbq

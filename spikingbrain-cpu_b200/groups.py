@@ -11,7 +11,8 @@ whole group, the others return their slice of that result, so the reference's mo
 unchanged.  A result is handed out once per computation; a member called again (or with another
 x) recomputes.  Members' outputs are column views of the group's [m, padded N] result.
 
-Both int8 formats are supported (all members of one group share the format).  int8-dyn members
+The int8 formats and the int4 ones are supported (all members of one group share the format, and the
+group size of an int4 one).  int8-dyn members
 give bit-identical results to separate calls: the per-tensor activation quantisation depends on x
 only, and each output channel's integer dot product does not depend on its neighbours.
 """
@@ -22,7 +23,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .quant import DynamicInt8Linear, Int8Linear, _DTYPE_CODE, _prepare_x, _ptr, _stream, _workspace
+from .quant import DynamicInt8Linear, Int4Linear, Int8Linear, _DTYPE_CODE, _prepare_x, _ptr, _stream, _workspace
 
 
 class SharedInputGroup(nn.Module):
@@ -31,14 +32,16 @@ class SharedInputGroup(nn.Module):
         if not members:
             raise ValueError("a group needs at least one projection")
         kind = type(members[0])
-        if kind not in (Int8Linear, DynamicInt8Linear) or any(type(m) is not kind for m in members):
-            raise ValueError("group members must all be Int8Linear or all DynamicInt8Linear")
+        if kind not in (Int8Linear, DynamicInt8Linear, Int4Linear) or any(type(m) is not kind for m in members):
+            raise ValueError("group members must all be Int8Linear, all DynamicInt8Linear or all Int4Linear")
         k = members[0].in_features
         if any(m.in_features != k for m in members):
             raise ValueError("group members must read the same input width")
         if kind is DynamicInt8Linear and len({m.mode for m in members}) != 1:
             raise ValueError("group members must share the activation quantisation mode")
-        dev = members[0].scale.device
+        if kind is Int4Linear and len({m.group for m in members}) != 1:
+            raise ValueError("int4 group members must share the group size")
+        dev = members[0].packed.device
         self.kind, self.in_features = kind, k
         self.sizes = [m.out_features for m in members]
         self.offsets, off = [], 0
@@ -46,6 +49,14 @@ class SharedInputGroup(nn.Module):
             self.offsets.append(off)
             off += (n + 15) // 16 * 16
         self.n_pad = off
+        self.mode = getattr(members[0], "mode", None)
+        self.out_dtype = torch.float32
+        self._result = None
+        self._key = None
+        self._handed = set()
+        if kind is Int4Linear:
+            self._join_int4(members)
+            return
         kt = (k + 63) // 64
         packed = torch.zeros(L.packed_bytes(self.n_pad, k), dtype=torch.int8, device=dev)
         scale = torch.zeros(self.n_pad, dtype=torch.float32, device=dev)
@@ -64,15 +75,25 @@ class SharedInputGroup(nn.Module):
         self.register_buffer("scale", scale, persistent=False)
         self.register_buffer("bias", bias, persistent=False)
         self.register_buffer("rowsum", rowsum, persistent=False)
-        self.mode = getattr(members[0], "mode", None)
-        self.out_dtype = torch.float32
-        self._result = None
-        self._key = None
-        self._handed = set()
+
+    def _join_int4(self, members: list[nn.Module]) -> None:
+        """One Int4Linear over the members' packed rows, which follow one another in every buffer."""
+        bias = None
+        if any(m.bias is not None for m in members):
+            bias = torch.zeros(self.n_pad, device=members[0].packed.device)
+            for m, o, n in zip(members, self.offsets, self.sizes):
+                if m.bias is not None:
+                    bias[o:o + n].copy_(m.bias)
+        self.linear = Int4Linear.from_packed(*(torch.cat([getattr(m, b) for m in members]) for b in ("packed", "scales", "rowmul")),
+                                             self.n_pad, self.in_features, bias, members[0].group)
 
     def forward_all(self, x: torch.Tensor) -> list[torch.Tensor]:
         """Every member's output for x [..., k] (one launch sequence); a list of column views."""
         shape = x.shape
+        if self.kind is Int4Linear:
+            self.linear.out_dtype = self.out_dtype
+            out = self.linear(x)
+            return [out[..., o:o + n] for o, n in zip(self.offsets, self.sizes)]
         dev = self.scale.device
         x2, k16, on_host = _prepare_x(x, self.in_features, dev)
         m = x2.shape[0]

@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .quant import _DTYPE_CODE, DynamicInt8Linear, Int8Linear, _device, _ptr
+from .quant import _DTYPE_CODE, INT4_FORMATS, DynamicInt8Linear, Int8Linear, _device, _ptr
 from .quant import make_linear as _make_linear_eager
 
 
@@ -104,9 +104,10 @@ class StreamingPacker:
         return ev
 
     def make_linear(self, fmt: str, weight: torch.Tensor, bias: torch.Tensor | None = None) -> nn.Module:
-        """quant.make_linear's signature and results (quant.py:100-111); int8 formats streamed."""
+        """quant.make_linear's signature and results (quant.py:100-111); int8 formats streamed
+        (the others, int4 among them, are made on the current stream)."""
         if fmt not in ("int8", "int8-dyn"):
-            if fmt in ("float32", "bfloat16", "float16"):
+            if fmt in ("float32", "bfloat16", "float16") + INT4_FORMATS:
                 return _make_linear_eager(fmt, weight, bias)
             raise ValueError("unknown weight format " + fmt)
         dyn = fmt == "int8-dyn"

@@ -1,4 +1,4 @@
-"""Fused SwiGLU MLP over int8 projections (GatedMLP.forward, spikingbrain_cpu/model.py:239-240).
+"""Fused SwiGLU MLP over int8 or int4 projections (GatedMLP.forward, spikingbrain_cpu/model.py:239-240).
 
 The reference runs ``down(silu(gate(x)) * up(x))`` as three Int8Linear calls plus two
 elementwise ops.  For decode-sized inputs ``FusedGatedMLP`` streams the gate and up weights in one
@@ -13,7 +13,8 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .quant import _DTYPE_CODE, Int8Linear, _prepare_x, _ptr, _stream, _workspace
+from .quant import (_DTYPE_CODE, Int4Linear, Int8Linear, _current, _int4_workspace, _prepare_x, _ptr, _rows16, _stream,
+                    _workspace)
 
 
 class FusedGatedMLP(nn.Module):
@@ -22,8 +23,11 @@ class FusedGatedMLP(nn.Module):
         """``shards`` > 1: gate/up hold one output-channel shard each and down consumes the gathered
         activation of all ``shards`` of them (the sharded stack); ``forward`` is then unavailable."""
         super().__init__()
-        if not all(isinstance(mod, Int8Linear) for mod in (gate, up, down)):
-            raise ValueError("FusedGatedMLP needs int8 gate, up and down projections")
+        if not all(isinstance(mod, (Int8Linear, Int4Linear)) for mod in (gate, up, down)) or type(gate) is not type(up):
+            raise ValueError("FusedGatedMLP needs int8 gate, up and down projections (or gate and up both int4)")
+        self.int4 = isinstance(gate, Int4Linear)
+        if self.int4 and gate.group != up.group:
+            raise ValueError("int4 gate and up projections must have the same group size")
         if gate.bias is not None or up.bias is not None:
             raise ValueError("the fused gate/up epilogue has no bias term")
         if gate.out_features != up.out_features or gate.in_features != up.in_features:
@@ -31,8 +35,8 @@ class FusedGatedMLP(nn.Module):
         if down.in_features != gate.out_features * shards:
             raise ValueError("down projection input must match the gate/up output")
         self.shards = shards
-        if h_dtype not in (torch.float16, torch.float32):
-            raise ValueError("hidden activation dtype must be float16 or float32")
+        if h_dtype not in (torch.float16, torch.float32) and not (self.int4 and h_dtype == torch.bfloat16):
+            raise ValueError("hidden activation dtype must be float16 or float32 (or bfloat16 with int4 weights)")
         self.gate_proj, self.up_proj, self.down_proj = gate, up, down
         self.h_dtype = h_dtype
 
@@ -40,15 +44,27 @@ class FusedGatedMLP(nn.Module):
         if self.shards != 1:
             raise RuntimeError("a sharded FusedGatedMLP needs the gather between gate/up and down; use the stack")
         shape = x.shape
-        dev = self.gate_proj.scale.device
+        dev = self.gate_proj.packed.device
         x2, k16, on_host = _prepare_x(x, self.gate_proj.in_features, dev)
         m, n = x2.shape[0], self.gate_proj.out_features
         h = self.gateup_into(x2, torch.empty(m, n, dtype=self.h_dtype, device=dev))
         y = self.down_proj(h).reshape(*shape[:-1], self.down_proj.out_features)
         return y.to("cpu") if on_host else y
 
+    def gateup(self, x: torch.Tensor) -> torch.Tensor:
+        """The hidden activation alone: silu(gate(x)) * up(x) in ``h_dtype``, x as ``forward`` takes it."""
+        dev = self.gate_proj.packed.device
+        x2, _, on_host = _rows16(x, self.gate_proj.in_features, dev)
+        n = self.gate_proj.out_features
+        h = self.gateup_into(x2, torch.empty(x2.shape[0], n, dtype=self.h_dtype, device=dev))
+        if x.dim() != 2:
+            h = h.view(*x.shape[:-1], n)
+        return h.to("cpu") if on_host else h
+
     def gateup_job(self, x2: torch.Tensor, h: torch.Tensor) -> L.GemvJob:
-        """silu(gate(x2)) * up(x2) into ``h`` as one job of a grouped decode launch."""
+        """silu(gate(x2)) * up(x2) into ``h`` as one job of a grouped decode launch (int8 weights)."""
+        if self.int4:
+            raise ValueError("grouped decode launches take int8 weights")
         g, u = self.gate_proj, self.up_proj
         return L.GemvJob(x2.data_ptr(), x2.stride(0), g.packed.data_ptr(), g.scale.data_ptr(), u.packed.data_ptr(),
                          u.scale.data_ptr(), None, g.out_features, x2.shape[1], h.data_ptr(),
@@ -63,6 +79,8 @@ class FusedGatedMLP(nn.Module):
         parts in a workspace that both GEMMs read).
         """
         m, n = x2.shape[0], self.gate_proj.out_features
+        if self.int4:
+            return self._gateup_int4(x2, h)
         if m > 0:
             ws, ws_bytes = _workspace(m, x2.shape[1], x2.dtype, h.device)
             L.call("sbq_mlp_gateup_w8_ws", _ptr(x2), _DTYPE_CODE[x2.dtype], x2.stride(0),
@@ -72,8 +90,28 @@ class FusedGatedMLP(nn.Module):
         return h
 
 
+    def _gateup_int4(self, x2: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
+        m, n, k = x2.shape[0], self.gate_proj.out_features, (self.gate_proj.in_features + 15) // 16 * 16
+        g, u = self.gate_proj._buffers, self.up_proj._buffers
+        dev = g["packed"].device
+        if h.shape != (m, n) or (n > 1 and h.stride(1) != 1) or h.dtype not in _DTYPE_CODE or h.device != dev:
+            raise ValueError("hidden activation must be an fp32/fp16/bf16 [%d, %d] view with unit column stride" % (m, n))
+        if x2.shape[1] != k or x2.stride(1) != 1 or x2.dtype not in _DTYPE_CODE or x2.device != dev:
+            raise ValueError("input must be an fp32/fp16/bf16 [m, %d] view with unit column stride" % k)
+        if m > 0:
+            code = _DTYPE_CODE[x2.dtype]
+            with _current(dev):
+                ws, ws_bytes = _int4_workspace(m, k, code, dev)
+                L.call("sbq_mlp_gateup_w4", x2.data_ptr(), code, x2.stride(0) if m > 1 else k, g["packed"].data_ptr(),
+                       g["scales"].data_ptr(), g["rowmul"].data_ptr(), u["packed"].data_ptr(), u["scales"].data_ptr(),
+                       u["rowmul"].data_ptr(), self.gate_proj.group, m, n, k, h.data_ptr(), _DTYPE_CODE[h.dtype],
+                       h.stride(0) if m > 1 else n, None if ws is None else ws.data_ptr(), ws_bytes,
+                       torch.cuda.current_stream(dev).cuda_stream)
+        return h
+
+
 def fuse_gated_mlp(model: nn.Module, h_dtype: torch.dtype = torch.float16) -> int:
-    """Replace every submodule holding int8 ``gate_proj``/``up_proj``/``down_proj`` by FusedGatedMLP.
+    """Replace every submodule holding int8 or int4 ``gate_proj``/``up_proj``/``down_proj`` by FusedGatedMLP.
 
     Returns how many were replaced.
     """
@@ -82,13 +120,14 @@ def fuse_gated_mlp(model: nn.Module, h_dtype: torch.dtype = torch.float16) -> in
         if isinstance(mod, FusedGatedMLP):
             continue
         parts = [getattr(mod, a, None) for a in ("gate_proj", "up_proj", "down_proj")]
-        if all(isinstance(p, Int8Linear) for p in parts) and parts[0].bias is None and parts[1].bias is None:
+        same = any(all(isinstance(p, kind) for p in parts) for kind in (Int8Linear, Int4Linear))
+        if same and getattr(parts[0], "group", None) == getattr(parts[1], "group", None) and parts[0].bias is None \
+                and parts[1].bias is None:
             parent_name, _, child = name.rpartition(".")
-            parent = model.get_submodule(parent_name) if parent_name else None
-            fused = FusedGatedMLP(*parts, h_dtype=h_dtype)
-            if parent is None:
+            if not name:
                 raise ValueError("cannot replace the root module in place")
-            setattr(parent, child, fused)
+            parent = model.get_submodule(parent_name) if parent_name else model
+            setattr(parent, child, FusedGatedMLP(*parts, h_dtype=h_dtype))
             count += 1
     return count
 

@@ -23,6 +23,10 @@ import torch.nn.functional as F
 from . import _lib as L
 
 FORMATS = ("float32", "bfloat16", "float16", "int8", "int8-dyn")
+# 4-bit weights with one bf16 scale per group of 32, 64 or 128 input features (no reference counterpart):
+# accepted by make_linear beside the reference's formats
+INT4_FORMATS = ("int4-g32", "int4-g64", "int4-g128")
+INT4_GROUPS = (32, 64, 128)
 
 _DTYPE_CODE = {torch.float32: L.F32, torch.float16: L.F16, torch.bfloat16: L.BF16}
 _ELEM = {torch.float32: 4, torch.float16: 2, torch.bfloat16: 2}
@@ -317,6 +321,251 @@ class DynamicInt8Linear(_PackedLinear):
         return y, xq[:, :self.in_features], s, zp, acc
 
 
+# ---- format int4: 4-bit weights with group scales ------------------------------------------------
+
+_Y_CODE = _DTYPE_CODE  # the 4-bit kernels write fp32, fp16 or bf16
+
+
+def _check_group(group: int) -> int:
+    if group not in INT4_GROUPS:
+        raise ValueError("group size must be one of %s, got %s" % (INT4_GROUPS, group))
+    return int(group)
+
+
+def _int4_buffers(n: int, k: int, group: int, dev: torch.device):
+    lib = L.load()
+    return (torch.empty(int(lib.sbq_w4_packed_bytes(n, k)), dtype=torch.uint8, device=dev),
+            torch.empty(int(lib.sbq_w4_scale_bytes(n, k, group)), dtype=torch.uint8, device=dev),
+            torch.empty((n + 15) // 16 * 16, dtype=torch.float32, device=dev))
+
+
+def pack_weight_int4(weight: torch.Tensor, group: int = 128, device=None):
+    """Quantise an [n, k] float weight per output channel and group of ``group`` inputs on the device, packed.
+
+    ``s = bf16(max(max|w|, 1e-8) / 7)``, ``q = clamp(rint(w / s), -7, 7)``.  Returns ``(packed, scales,
+    rowmul)``, the three device buffers the 4-bit kernels read.
+    """
+    dev = _device(device)
+    group = _check_group(group)
+    if weight.dim() != 2 or weight.numel() == 0:
+        raise ValueError("weight must be 2-D [out_features, in_features], got shape %s" % (tuple(weight.shape),))
+    w = weight.detach()
+    if w.dtype not in _DTYPE_CODE:
+        w = w.float()
+    w = w.to(dev)
+    if w.stride(1) != 1 or w.stride(0) < w.shape[1]:
+        w = w.contiguous()
+    n, k = w.shape
+    bufs = _int4_buffers(n, k, group, dev)
+    with torch.cuda.device(dev):
+        L.call("sbq_w4_quantize_pack", _ptr(w), _DTYPE_CODE[w.dtype], n, k, w.stride(0), group, *map(_ptr, bufs), _stream(dev))
+    return bufs
+
+
+def pack_int4(q: torch.Tensor, scale: torch.Tensor, group: int = 128, device=None):
+    """Pack given codes (int8 [n, k], values in [-8, 7]) and bf16 scales [n, ceil(k / group)].
+
+    The scales are taken as they are: they must be finite bf16 (round others yourself, so that the codes
+    fit the scales that are stored).  Returns the buffers of ``pack_weight_int4``.
+    """
+    dev = _device(device)
+    group = _check_group(group)
+    if q.dim() != 2 or q.dtype != torch.int8 or q.numel() == 0:
+        raise ValueError("codes must be a 2-D int8 tensor")
+    n, k = q.shape
+    if scale.dtype != torch.bfloat16 or tuple(scale.shape) != (n, -(-k // group)):
+        raise ValueError("scales must be bf16 [%d, %d], got %s %s" % (n, -(-k // group), scale.dtype, tuple(scale.shape)))
+    q, scale = q.to(dev).contiguous(), scale.to(dev).contiguous()
+    lo, hi = (int(v) for v in torch.aminmax(q))
+    if lo < -8 or hi > 7:
+        raise ValueError("codes must lie in [-8, 7], got [%d, %d]" % (lo, hi))
+    if not bool(torch.isfinite(scale).all()):
+        raise ValueError("scales must be finite")
+    bufs = _int4_buffers(n, k, group, dev)
+    with torch.cuda.device(dev):
+        L.call("sbq_w4_pack", _ptr(q), k, _ptr(scale), scale.shape[1], n, k, group, *map(_ptr, bufs), _stream(dev))
+    return bufs
+
+
+def unpack_int4(packed: torch.Tensor, scales: torch.Tensor, n: int, k: int, group: int):
+    """Packed buffers -> ``(q int8 [n, k], scale bf16 [n, ceil(k / group)])`` on the same device."""
+    dev = packed.device
+    q = torch.empty(n, k, dtype=torch.int8, device=dev)
+    scale = torch.empty(n, -(-k // group), dtype=torch.bfloat16, device=dev)
+    with torch.cuda.device(dev):
+        L.call("sbq_w4_unpack", _ptr(packed), _ptr(scales), n, k, group, _ptr(q), k, _ptr(scale), scale.shape[1], _stream(dev))
+    return q, scale
+
+
+def quantize_per_group(weight: torch.Tensor, group: int = 128, device=None) -> tuple[torch.Tensor, torch.Tensor]:
+    """``(q int8 [n, k], scale bf16 [n, ceil(k / group)])`` of the ``int4`` formats, computed on the device."""
+    packed, scales, _ = pack_weight_int4(weight, group, device)
+    return unpack_int4(packed, scales, *weight.shape, group)
+
+
+def _rows16(x: torch.Tensor, k: int, device: torch.device):
+    """``_prepare_x`` with a shortcut for what a decode loop passes: ``(x2, k16, on_host)``."""
+    if x.device == device and k % 16 == 0 and x.shape[-1] == k and x.dtype in _DTYPE_CODE and x.is_contiguous() \
+            and x.data_ptr() % 16 == 0:
+        return x.view(-1, k), k, False
+    return _prepare_x(x, k, device)
+
+
+class Int4Linear(nn.Module):
+    """Formats ``int4-g32`` / ``int4-g64`` / ``int4-g128``: 4-bit weight, one bf16 scale per output channel and
+    group of input features; y = x (q * s)^T + b.
+
+    x may be fp32, fp16 or bf16 (fp32 enters the product with 22 bits, the others exactly), products are
+    summed in fp32, and ``out_dtype`` (fp32 as in the other formats, or fp16 / bf16) is the type of the
+    result.  Frozen like every format here: no gradient flows through it.  State dicts hold ``qweight``
+    (int8 codes [n, k]) and ``scale`` (bf16 [n, ceil(k / group)]); both are copies of the packed weight, so
+    writing into them does not change it (load a state dict, or pack anew).
+    """
+
+    def __init__(self, weight: torch.Tensor, bias: torch.Tensor | None, group: int = 128, device=None):
+        super().__init__()
+        self._adopt(pack_weight_int4(weight, group, device), weight.shape, bias, group)
+
+    def _adopt(self, bufs, shape, bias, group: int) -> None:
+        packed, scales, rowmul = bufs
+        self.out_features, self.in_features, self.group = int(shape[0]), int(shape[1]), int(group)
+        if bias is not None and tuple(bias.shape) != (self.out_features,):
+            raise ValueError("bias must have shape (%d,), got %s" % (self.out_features, tuple(bias.shape)))
+        self.register_buffer("packed", packed, persistent=False)
+        self.register_buffer("scales", scales, persistent=False)
+        self.register_buffer("rowmul", rowmul, persistent=False)
+        self.bias = None if bias is None else nn.Parameter(bias.detach().float().to(packed.device).contiguous(), requires_grad=False)
+        self.out_dtype = torch.float32
+
+    @classmethod
+    def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, rowmul: torch.Tensor, out_features: int,
+                    in_features: int, bias: torch.Tensor | None = None, group: int = 128):
+        """A module around buffers of ``pack_weight_int4`` / ``pack_int4``; they are adopted, not copied."""
+        lib = L.load()
+        group = _check_group(group)
+        if packed.numel() != int(lib.sbq_w4_packed_bytes(out_features, in_features)) or \
+                scales.numel() != int(lib.sbq_w4_scale_bytes(out_features, in_features, group)) or \
+                rowmul.numel() != (out_features + 15) // 16 * 16:
+            raise ValueError("packed buffers do not match a [%d, %d] weight in groups of %d" % (out_features, in_features, group))
+        mod = cls.__new__(cls)
+        nn.Module.__init__(mod)
+        mod._adopt((packed, scales, rowmul), (out_features, in_features), bias, group)
+        return mod
+
+    @classmethod
+    def from_quantized(cls, q: torch.Tensor, scale: torch.Tensor, bias: torch.Tensor | None = None, group: int = 128,
+                       device=None):
+        """A module of given codes (int8 [n, k] in [-8, 7]) and bf16 scales [n, ceil(k / group)]."""
+        return cls.from_packed(*pack_int4(q, scale, group, device), q.shape[0], q.shape[1], bias, group)
+
+    @property
+    def qweight(self) -> torch.Tensor:
+        """The codes, int8 [out, in] (a copy)."""
+        return unpack_int4(self.packed, self.scales, self.out_features, self.in_features, self.group)[0]
+
+    @property
+    def scale(self) -> torch.Tensor:
+        """The group scales, bf16 [out, ceil(in / group)] (a copy)."""
+        return unpack_int4(self.packed, self.scales, self.out_features, self.in_features, self.group)[1]
+
+    def _save_to_state_dict(self, destination, prefix, keep_vars):
+        super()._save_to_state_dict(destination, prefix, keep_vars)
+        destination[prefix + "qweight"], destination[prefix + "scale"] = unpack_int4(
+            self.packed, self.scales, self.out_features, self.in_features, self.group)
+
+    def _load_from_state_dict(self, state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                              error_msgs):
+        keys = (prefix + "qweight", prefix + "scale")
+        q, scale = (state_dict.get(key) for key in keys)
+        super()._load_from_state_dict(state_dict, prefix, local_metadata, strict, missing_keys, unexpected_keys,
+                                      error_msgs)
+        for key in keys:
+            if key in unexpected_keys:
+                unexpected_keys.remove(key)
+        if q is None or scale is None:
+            if strict:
+                missing_keys.extend(key for key, v in zip(keys, (q, scale)) if v is None)
+            return
+        want = ((self.out_features, self.in_features), (self.out_features, -(-self.in_features // self.group)))
+        if (tuple(q.shape), tuple(scale.shape)) != want:
+            error_msgs.append("size mismatch for %s: %s, %s != %s, %s" % (prefix + "qweight / scale", tuple(q.shape),
+                                                                          tuple(scale.shape), *want))
+            return
+        try:
+            bufs = pack_int4(q, scale, self.group, self.packed.device)
+        except ValueError as e:
+            error_msgs.append("%s: %s" % (prefix + "qweight / scale", e))
+            return
+        for dst, src in zip((self.packed, self.scales, self.rowmul), bufs):
+            dst.copy_(src)
+
+    def forward_into(self, x2: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
+        """Low-level device call: x2 [m, k'] (k' = in_features rounded up to 16, 16-byte aligned rows)
+        into ``out`` [m, out_features] (fp32, fp16 or bf16, unit column stride, any row stride)."""
+        m, n = x2.shape[0], self.out_features
+        if out.shape != (m, n) or (out.stride(1) != 1 and n > 1) or out.dtype not in _Y_CODE:
+            raise ValueError("output must be an fp32/fp16/bf16 [%d, %d] view with unit column stride" % (m, n))
+        k16 = (self.in_features + 15) // 16 * 16
+        if x2.shape[1] != k16 or x2.stride(1) != 1 or x2.dtype not in _DTYPE_CODE:
+            raise ValueError("input must be an fp32/fp16/bf16 [m, %d] view with unit column stride" % k16)
+        b = self._buffers
+        dev = b["packed"].device
+        if x2.device != dev or out.device != dev:
+            raise ValueError("input and output must be on the weight's device %s" % dev)
+        if m > 0:
+            with _current(dev):
+                self._call(x2, k16, m, n, out, b, dev)
+        return out
+
+    def _call(self, x2, k, m, n, out, b, dev) -> None:
+        x_code = _DTYPE_CODE[x2.dtype]
+        ws, ws_bytes = _int4_workspace(m, k, x_code, dev)
+        bias = self._parameters.get("bias")
+        L.call("sbq_linear_w4", x2.data_ptr(), x_code, x2.stride(0) if m > 1 else k, b["packed"].data_ptr(),
+               b["scales"].data_ptr(), b["rowmul"].data_ptr(), self.group, None if bias is None else bias.data_ptr(), m, n,
+               k, out.data_ptr(), _Y_CODE[out.dtype], out.stride(0) if m > 1 else n, None if ws is None else ws.data_ptr(), ws_bytes,
+               torch.cuda.current_stream(dev).cuda_stream)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        dev = self._buffers["packed"].device
+        x2, k16, on_host = _rows16(x, self.in_features, dev)
+        out = torch.empty(x2.shape[0], self.out_features, dtype=self.out_dtype, device=dev)
+        self.forward_into(x2, out)
+        if x.dim() != 2:
+            out = out.view(*x.shape[:-1], self.out_features)
+        return out.to("cpu") if on_host else out
+
+    def extra_repr(self) -> str:
+        return "in_features=%d, out_features=%d, bias=%s, group=%d" % (self.in_features, self.out_features,
+                                                                       self.bias is not None, self.group)
+
+
+class _Here:
+    """A context that changes nothing."""
+
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return None
+
+
+_HERE = _Here()
+
+
+def _current(device: torch.device):
+    """Makes ``device`` the current one for a library call (the library launches on the current device)."""
+    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
+
+
+def _int4_workspace(m: int, k: int, x_code: int, device: torch.device):
+    """(tensor or None, bytes) for the activation's fp16 parts, from torch's caching allocator."""
+    if x_code == L.F16:
+        return None, 0
+    nbytes = int(L.load().sbq_linear_w4_workspace_bytes(m, k, x_code))
+    return (torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes) if nbytes else (None, 0)
+
+
 # ---- float formats (outside the int8 hot path; cuBLAS through torch, fp32 results) ----------
 
 class FP16Linear(nn.Module):
@@ -368,7 +617,8 @@ class FloatLinear(nn.Module):
 
 
 def make_linear(fmt: str, weight: torch.Tensor, bias: torch.Tensor | None = None) -> nn.Module:
-    """quant.py:100-111: format string -> module; ``ValueError`` for an unknown format."""
+    """quant.py:100-111: format string -> module; ``ValueError`` for an unknown format.  Beside the
+    reference's formats it takes ``INT4_FORMATS``."""
     if fmt == "float32":
         return FloatLinear(weight, bias)
     if fmt == "bfloat16":
@@ -379,4 +629,6 @@ def make_linear(fmt: str, weight: torch.Tensor, bias: torch.Tensor | None = None
         return Int8Linear(weight, bias)
     if fmt == "int8-dyn":
         return DynamicInt8Linear(weight, bias)
+    if fmt in INT4_FORMATS:
+        return Int4Linear(weight, bias, group=int(fmt[6:]))
     raise ValueError("unknown weight format " + fmt)

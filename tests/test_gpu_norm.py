@@ -1,0 +1,265 @@
+"""The step between two blocks (residual_norm) against its formula in 64 bits.
+
+Tolerances.  Sums of squares run over fp32 values in a tree of depth log2(d) above a chain of at most 64
+additions per thread, so a statistic is off by at most (64 + 16) * 2^-24 relative; the square root halves
+that, rsqrt, the divisions, exp and tanh add a few units in the last place.  C = 64 * 2^-24 covers a factor of
+one norm.  r' adds a sum of two terms (2^-23 of their magnitudes); its own norm divides by a statistic of r',
+whose relative error is that of r' in the mean.  The results are rounded once to their type.
+"""
+
+import itertools
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+C = 64 * 2.0 ** -24
+ACTS = {"none": lambda g: g, "sigmoid": torch.sigmoid, "silu": lambda g: g * torch.sigmoid(g), "tanh": torch.tanh}
+
+
+def rand(*shape, seed, dtype=F32, scale=1.0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return (torch.randn(*shape, generator=g, device="cuda") * scale).to(dtype)
+
+
+def reference(branch, residual, pre, post, gate, act, a, b, eps):
+    """(r', x, bound on the error of r', of x) in 64 bits."""
+    r = a * residual.double()
+    err = r.abs() * 2.0 ** -23
+    if branch is not None:
+        h = branch.double()
+        if post is not None:
+            h = h / (h.square().mean(-1, keepdim=True) + eps).sqrt() * post.double()
+        if gate is not None:
+            h = h * ACTS[act](gate.double())
+        h = b * h
+        err = err + h.abs() * C
+        r = r + h
+    x = err_x = None
+    if pre is not None:
+        norm = (r.square().mean(-1, keepdim=True) + eps).sqrt()
+        x = r / norm * pre.double()
+        mean_err = (err.square().mean(-1, keepdim=True)).sqrt() / norm
+        err_x = err / norm * pre.double().abs() + x.abs() * (mean_err + C)
+    return r, x, err, err_x
+
+
+def check(got, want, err):
+    tol = err + want.abs() * torch.finfo(got.dtype).eps / 2 + (2.0 ** -25 if got.dtype == F16 else 0.0)
+    bad = ((got.double() - want).abs() - tol).max().item()
+    assert bad <= 0, "off by %g over the tolerance" % bad
+
+
+def run(sbq, branch, residual, pre, post=None, gate=None, act="none", a=1.0, b=1.0, eps=1e-6, out=F16, **kw):
+    r, x = sbq.residual_norm(branch, residual, pre, post_weight=post, gate=gate, gate_act=act, residual_scale=a,
+                             branch_scale=b, eps=eps, out_dtype=out, **kw)
+    wr, wx, er, ex = reference(branch, residual, pre, post, gate, act, a, b, eps)
+    assert r.dtype == residual.dtype and r.shape == residual.shape
+    check(r, wr, er)
+    if pre is None:
+        assert x is None
+    else:
+        assert x.dtype == out and x.shape == residual.shape
+        check(x, wx, ex)
+    return r, x
+
+
+SIZES = [1, 2, 7, 8, 31, 64, 100, 128, 255, 256, 257, 512, 513, 1000, 1024, 2048, 2559, 2560, 4096, 4100, 8192, 8200, 12288,
+         16384, 20000, 33001]
+
+
+@pytest.mark.parametrize("d", SIZES)
+@pytest.mark.parametrize("m", [1, 3, 200])
+def test_sizes(sbq, m, d):
+    i = d + m
+    post = 1 + rand(d, seed=1, scale=0.1) if i % 2 else None
+    gate = rand(m, d, seed=2) if i % 3 == 0 else None
+    run(sbq, rand(m, d, seed=3), rand(m, d, seed=4, scale=4.0), 1 + rand(d, seed=5, scale=0.1), post, gate,
+        "sigmoid" if gate is not None else "none", 0.75, 1.25, out=(F16, BF16, F32)[i % 3])
+
+
+@pytest.mark.parametrize("y,r,x", list(itertools.product([F32, F16, BF16], repeat=3)))
+@pytest.mark.parametrize("d", [640, 333])
+def test_types(sbq, y, r, x, d):
+    run(sbq, rand(17, d, seed=6, dtype=y), rand(17, d, seed=7, dtype=r), 1 + rand(d, seed=8, scale=0.1),
+        rand(d, seed=9), rand(17, d, seed=10, dtype=y), "silu", out=x)
+
+
+@pytest.mark.parametrize("act", ["none", "sigmoid", "silu", "tanh"])
+@pytest.mark.parametrize("mode", ["vector", "token", "full"])
+@pytest.mark.parametrize("post", [False, True])
+def test_gates(sbq, act, mode, post):
+    for m, d, dt in ((5, 96, F32), (150, 1030, BF16), (2, 18000, F16)):
+        shape = {"vector": (d,), "token": (m, 1), "full": (m, d)}[mode]
+        run(sbq, rand(m, d, seed=11, dtype=dt), rand(m, d, seed=12), 1 + rand(d, seed=13, scale=0.1),
+            rand(d, seed=14) if post else None, rand(*shape, seed=15, dtype=dt, scale=3.0), act, -0.5, 2.0, out=BF16)
+
+
+def test_parts_left_out(sbq):
+    d = 520
+    y, r, w = rand(9, d, seed=16), rand(9, d, seed=17), rand(d, seed=18)
+    run(sbq, y, r, None)
+    run(sbq, y, r, None, post=w)
+    kept, x = run(sbq, None, r, w)
+    assert kept is r
+    run(sbq, None, r, w, a=0.5)
+    big = rand(3, 17000, seed=19)
+    run(sbq, big, big * 2, None, post=rand(17000, seed=20))
+    run(sbq, None, big, rand(17000, seed=20))
+
+
+@pytest.mark.parametrize("d", [64, 1000, 4096, 17001])
+def test_in_place_and_strides(sbq, d):
+    for m, dt in ((1, F32), (40, F32), (40, BF16)):
+        y, r, w = rand(m, d, seed=21), rand(m, d, seed=22, dtype=dt), 1 + rand(d, seed=23, scale=0.1)
+        want_r, want_x = run(sbq, y, r, w, post=w)
+        mine = r.clone()
+        got_r, got_x = sbq.residual_norm(y, mine, w, post_weight=w, residual_out=mine)
+        assert got_r is mine and torch.equal(mine, want_r) and torch.equal(got_x, want_x)
+        # strided rows, the surroundings of the output left alone
+        wide = torch.full((m + 2, d + 24), 3.0, dtype=dt, device="cuda")
+        rows = rand(m, d + 16, seed=24)
+        yv = rows[:, 8:8 + d]
+        wide[1:m + 1, 8:8 + d] = r
+        got_r, got_x = sbq.residual_norm(yv, wide[1:m + 1, 8:8 + d], w, residual_out=wide[1:m + 1, 8:8 + d])
+        want_r, want_x = sbq.residual_norm(yv.contiguous(), r, w)
+        assert torch.equal(got_r, want_r) and torch.equal(got_x, want_x)
+        wide[1:m + 1, 8:8 + d] = 3.0
+        assert (wide == 3.0).all()
+        # addresses off by one element take the narrow accesses
+        flat = rand(m * d + 1, seed=25)
+        y1 = flat[1:].view(m, d)
+        run(sbq, y1, r, w)
+        run(sbq, rand(d, m, seed=26).t(), r, w)           # columns: copied
+        run(sbq, rand(1, d, seed=27).expand(m, d), r, w)  # one row for all
+
+
+def test_leading_shapes_and_empty(sbq):
+    y, r, w = rand(2, 3, 80, seed=28), rand(2, 3, 80, seed=29), rand(80, seed=30)
+    got = sbq.residual_norm(y, r, w, gate=rand(2, 3, 1, seed=31), gate_act="tanh")
+    flat = sbq.residual_norm(y.view(6, 80), r.view(6, 80), w, gate=rand(2, 3, 1, seed=31).view(6, 1), gate_act="tanh")
+    assert torch.equal(got[0].view(6, 80), flat[0]) and torch.equal(got[1].view(6, 80), flat[1])
+    one = sbq.residual_norm(y[0, 0], r[0, 0], w)
+    assert one[0].shape == (80,) and torch.equal(one[1], sbq.residual_norm(y[0, :1], r[0, :1], w)[1][0])
+    e = sbq.residual_norm(y[:0], r[:0], w)
+    assert e[0].shape == (0, 3, 80) and e[1].shape == (0, 3, 80)
+
+
+def test_zeros_and_special_values(sbq):
+    d = 300
+    y, r, w = rand(6, d, seed=32), rand(6, d, seed=33), rand(d, seed=34)
+    y[0], r[0] = 0.0, 0.0
+    y[2, 5], r[3, 7] = float("nan"), float("inf")
+    got_r, got_x = sbq.residual_norm(y, r, w, post_weight=w, out_dtype=F32)
+    assert (got_x[0] == 0).all() and (got_r[0] == 0).all()
+    assert torch.isnan(got_r[2]).all() and torch.isnan(got_x[2]).all()
+    assert torch.isinf(got_r[3, 7]) and torch.isfinite(got_r[3, :7]).all()
+    rest = [1, 4, 5]
+    wr, wx, er, ex = reference(y[rest], r[rest], w, w, None, "none", 1.0, 1.0, 1e-6)
+    check(got_r[rest], wr, er)
+    check(got_x[rest], wx, ex)
+    # far gates saturate and do not overflow
+    g = torch.tensor([[-300.0], [300.0], [-90.0], [90.0], [0.0], [1.0]], device="cuda")
+    for act in ("sigmoid", "silu", "tanh"):
+        run(sbq, rand(6, d, seed=35), rand(6, d, seed=36), w, None, g, act, out=F32)
+
+
+def test_refusals(sbq):
+    y, r, w = rand(4, 32, seed=37), rand(4, 32, seed=38), rand(32, seed=39)
+    for kw, match in (({"gate": rand(4, 16, seed=1)}, "gate must have"), ({"gate": rand(32, seed=1), "gate_act": "gelu"}, "activation"),
+                      ({"eps": -1.0}, "eps"), ({"eps": float("nan")}, "eps"), ({"out_dtype": torch.int8}, "output dtype"),
+                      ({"post_weight": rand(31, seed=1)}, "post_weight"), ({"residual_out": r.half()}, "residual_out"),
+                      ({"residual_out": torch.empty(32, 4, device="cuda").t()}, "residual_out")):
+        with pytest.raises(ValueError, match=match):
+            sbq.residual_norm(y, r, w, **kw)
+    with pytest.raises(ValueError, match="same shape"):
+        sbq.residual_norm(y[:, :16], r, w)
+    with pytest.raises(ValueError, match="needs a branch"):
+        sbq.residual_norm(None, r, w, post_weight=w)
+    with pytest.raises(ValueError, match="CUDA"):
+        sbq.residual_norm(y, r.cpu(), w)
+    with pytest.raises(ValueError, match="device"):
+        sbq.residual_norm(y.cpu(), r, w)
+    with pytest.raises(ValueError, match="fp32, fp16 or bf16"):
+        sbq.residual_norm(y.double(), r, w)
+    with pytest.raises(ValueError, match="pre_weight"):
+        sbq.residual_norm(y, r, w[:16])
+    with pytest.raises(ValueError, match="no gradient"):
+        sbq.residual_norm(y, r.requires_grad_(), w)
+    with torch.no_grad():
+        sbq.residual_norm(y, r, w)
+
+
+@pytest.mark.parametrize("m", [1, 300])
+def test_streams_and_graphs(sbq, m):
+    step = sbq.ResidualNorm(rand(768, seed=40), rand(768, seed=41), "sigmoid", 0.5, 2.0).cuda()
+    y, r, g = rand(m, 768, seed=42), rand(m, 768, seed=43), rand(m, 768, seed=44)
+    want = step(y, r, g)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = step(y, r, g)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    buf = torch.zeros_like(y)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step(buf, r, g)
+    buf.copy_(y)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(out, want))
+
+
+@pytest.mark.parametrize("fmt", ["int4-g64", "int8"])
+@pytest.mark.parametrize("m", [1, 13, 70])
+def test_blocks_joined_by_norms(sbq, fmt, m):
+    """Two gated MLP blocks with norms before and after each, as a decode step and as a prompt, eager and
+    captured, against the same network in 64 bits on the weights the modules hold."""
+    hidden, inter = 128, 320
+
+    def block(seed):
+        ws = [rand(*s, seed=seed + i, scale=0.05) for i, s in enumerate(((inter, hidden), (inter, hidden), (hidden, inter)))]
+        return sbq.FusedGatedMLP(*(sbq.make_linear(fmt, w) for w in ws))
+
+    def weights(lin):
+        q, s = lin.qweight.double(), lin.scale.double()
+        return q * (s[:, None] if s.dim() == 1 else s.repeat_interleave(lin.group, 1)[:, :q.shape[1]])
+
+    blocks = [block(50), block(60)]
+    norms = [sbq.ResidualNorm(1 + rand(hidden, seed=70, scale=0.1), 1 + rand(hidden, seed=71, scale=0.1), "tanh", 1.0, 0.5).cuda()
+             for _ in range(2)]
+    gates = [rand(hidden, seed=72), rand(hidden, seed=73)]
+    first = 1 + rand(hidden, seed=74, scale=0.1)
+
+    def net(e):
+        r, x = sbq.residual_norm(None, e, first)
+        for blk, norm, gate in zip(blocks, norms, gates):
+            r, x = norm(blk(x), r, gate)
+        return r, x
+
+    def rms(v, w):
+        return v / (v.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+
+    e = rand(m, hidden, seed=75)
+    r = e.double()
+    x = rms(r, first)
+    for blk, norm, gate in zip(blocks, norms, gates):
+        wg, wu, wd = (weights(p) for p in (blk.gate_proj, blk.up_proj, blk.down_proj))
+        g = x @ wg.t()
+        y = (g * g.sigmoid() * (x @ wu.t())) @ wd.t()
+        r = r + 0.5 * torch.tanh(gate.double()) * rms(y, norm.post_weight)
+        x = rms(r, norm.pre_weight)
+    got = net(e)
+    # each block takes x and h rounded to fp16 (2^-11 of each value); a block's output is normalised, so its relative
+    # error (a few of those in the mean) is that of the term added to r
+    for a, b in zip(got, (r, x)):
+        assert (a.double() - b).norm() <= 8 * 2.0 ** -11 * b.norm()
+    buf = torch.zeros_like(e)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = net(buf)
+    buf.copy_(e)
+    graph.replay()
+    assert all(torch.equal(a, b) for a, b in zip(out, got))
