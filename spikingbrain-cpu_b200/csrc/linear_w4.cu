@@ -1,5 +1,5 @@
 // Entry points of the 4-bit format: argument checks, the activation's 16-bit parts, and the choice of
-// kernel (decode product up to 16 rows).
+// kernel (decode product up to 16 rows, the tensor-memory product above).
 #include <atomic>
 
 #include "w4_host.cuh"
@@ -165,7 +165,7 @@ static int w4_run(const void* x, int x_dtype, int64_t ldx, const W4Call& c, int 
         a.inv = p.inv;
         a.bf16 = false;
     }
-    return gemv_w4_run(c, a);
+    return c.m <= kW4GemvRows ? gemv_w4_run(c, a) : gemm_w4_run(c, a);
 }
 
 }  // namespace sbq

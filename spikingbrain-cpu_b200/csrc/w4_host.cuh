@@ -27,7 +27,8 @@ struct W4Acts {
     bool bf16;
 };
 
-int gemv_w4_run(const W4Call& c, const W4Acts& x);
+int gemv_w4_run(const W4Call& c, const W4Acts& x);  // up to 16 rows
+int gemm_w4_run(const W4Call& c, const W4Acts& x);  // fp16 parts only
 int w4_sm_count();
 
 inline int w4_elem(int dtype) { return dtype == SBQ_F32 ? 4 : 2; }
