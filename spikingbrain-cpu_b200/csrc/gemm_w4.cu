@@ -50,17 +50,19 @@ struct GemmW4Params {
     int y_dtype;
 };
 
-// Sizes of one kernel.  XROWS: tokens of x this CTA loads per stage; N: the MMA's tokens.
-template <int XROWS, int N, int PARTS, bool SEG, int TMEM, int RING>
+// Sizes of one kernel.  XROWS: tokens of x this CTA loads per block of 128 k; N: the MMA's tokens; CODES: code
+// matrices per block; ND: accumulators per matrix.
+template <int XROWS, int N, int PARTS, int CODES, int ND, int TMEM, int RING>
 struct W4Shape {
     static constexpr int kXSub = XROWS * 128;               // 64 columns of k: a 128-byte row per token
     static constexpr int kXBytes = 2 * PARTS * kXSub;       // [64-column half][part]
-    static constexpr int kCodes = kW4Rows * 64;
-    static constexpr int kStage = kXBytes + kCodes + 1024;  // scales: at most 1 KiB
+    static constexpr int kCodes = kW4Rows * 64;             // one matrix
+    static constexpr int kScales = 1024;                    // one matrix (at most)
+    static constexpr int kStage = kXBytes + CODES * (kCodes + kScales);
     static constexpr int kStages = RING / kStage < 8 ? RING / kStage : 8;
-    static constexpr int kACol = SEG ? 2 * N : N;            // accumulator(s) first
-    static constexpr int kABufs0 = (TMEM - kACol) / 64;
-    static constexpr int kABufs = kABufs0 < kStages ? kABufs0 : kStages;  // 64 columns per 128 k
+    static constexpr int kACol = CODES * ND * N;            // accumulators first
+    static constexpr int kABufs0 = (TMEM - kACol) / (64 * CODES);
+    static constexpr int kABufs = kABufs0 < kStages ? kABufs0 : kStages;  // 64 columns per 128 k and matrix
     static constexpr int kSegBlocks = kSegSteps / (8 * PARTS);
     static constexpr int kBarOff = kStages * kStage;
     static constexpr int kBytes = kBarOff + 512 + kW4Rows * 8 + 1024;
@@ -69,39 +71,52 @@ struct W4Shape {
     static_assert(kBytes <= 227 * 1024, "shared memory");
 };
 
-// One channel's 128 codes (64 bytes of row `row`, 64-byte swizzle) -> words 16 w + 4 t + i = columns
-// 32 w + 8 t + 2 i, + 1 of the scaled fp16 weight.  `half` 0 / 1: the words of columns 0..63 / 64..127.
+// fp16 scale pairs (s, s) and (-24 s, -24 s) of one channel's groups in a tile.
 template <int GPT>
-__device__ __forceinline__ void w4_convert_half(const uint4 (&raw)[4], const uint32_t (&s2)[GPT], const uint32_t (&c2)[GPT],
-                                                int half, uint32_t (&h)[32]) {
+__device__ __forceinline__ void w4_scales(const uint8_t* scales, int row, float rowmul, int g0, uint32_t* s2, uint32_t* c2,
+                                          int count) {
 #pragma unroll
-    for (int w2 = 0; w2 < 2; ++w2)
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            const uint32_t v = half ? (w2 ? raw[t].w : raw[t].z) : (w2 ? raw[t].y : raw[t].x);
-            const int gi = (2 * half + w2) * GPT / 4;
-            uint32_t* o = h + 16 * w2 + 4 * t;
-            o[0] = hfma2(lop3_and_or(v << 6, 0x03C003C0u, 0x4C004C00u), s2[gi], c2[gi]);
-            o[1] = hfma2(lop3_and_or(v << 2, 0x03C003C0u, 0x4C004C00u), s2[gi], c2[gi]);
-            o[2] = hfma2(lop3_and_or(v >> 2, 0x03C003C0u, 0x4C004C00u), s2[gi], c2[gi]);
-            o[3] = hfma2(lop3_and_or(v >> 6, 0x03C003C0u, 0x4C004C00u), s2[gi], c2[gi]);
-        }
+    for (int i = 0; i < count; ++i) {
+        const uint16_t u = *reinterpret_cast<const uint16_t*>(
+            scales + (((row >> 4) * 8 + (row & 7)) * GPT + g0 + i) * 4 + ((row >> 3) & 1) * 2);
+        const __half2 s = __float2half2_rn(__uint_as_float((uint32_t)u << 16) * rowmul);
+        s2[i] = *reinterpret_cast<const uint32_t*>(&s);
+        const __half2 c = __hmul2(s, __float2half2_rn(-24.0f));
+        c2[i] = *reinterpret_cast<const uint32_t*>(&c);
+    }
 }
 
-// A converter thread's stage: codes and scales of channel `row` -> 64 tensor-memory columns.
+// Eight codes -> four words of scaled fp16 weights.
+__device__ __forceinline__ void w4_convert_word(uint32_t v, uint32_t s, uint32_t c, uint32_t* o) {
+    o[0] = hfma2(lop3_and_or(v << 6, 0x03C003C0u, 0x4C004C00u), s, c);
+    o[1] = hfma2(lop3_and_or(v << 2, 0x03C003C0u, 0x4C004C00u), s, c);
+    o[2] = hfma2(lop3_and_or(v >> 2, 0x03C003C0u, 0x4C004C00u), s, c);
+    o[3] = hfma2(lop3_and_or(v >> 6, 0x03C003C0u, 0x4C004C00u), s, c);
+}
+
+// Columns 64 half .. 64 half + 63 of channel `row` of one tile (64 bytes of codes, 64-byte swizzle) -> 32
+// tensor-memory columns.
 template <int GPT>
-__device__ __forceinline__ void w4_convert_stage(const uint8_t* codes, const uint8_t* scales, int row, float rowmul,
-                                                 uint32_t tmem_dst) {
-    uint32_t s2[GPT], c2[GPT];
+__device__ __forceinline__ void w4_convert_half(const uint8_t* codes, const uint8_t* scales, int row, float rowmul, int half,
+                                                uint32_t tmem_dst) {
+    constexpr int NG = GPT == 4 ? 2 : 1;  // groups in 64 columns
+    uint32_t s2[NG], c2[NG], h[32];
+    w4_scales<GPT>(scales, row, rowmul, half * GPT / 2, s2, c2, NG);
 #pragma unroll
-    for (int gi = 0; gi < GPT; ++gi) {
-        const uint16_t u = *reinterpret_cast<const uint16_t*>(
-            scales + (((row >> 4) * 8 + (row & 7)) * GPT + gi) * 4 + ((row >> 3) & 1) * 2);
-        const __half2 s = __float2half2_rn(__uint_as_float((uint32_t)u << 16) * rowmul);
-        s2[gi] = *reinterpret_cast<const uint32_t*>(&s);
-        const __half2 c = __hmul2(s, __float2half2_rn(-24.0f));
-        c2[gi] = *reinterpret_cast<const uint32_t*>(&c);
+    for (int t = 0; t < 4; ++t) {
+        const uint2 v = *reinterpret_cast<const uint2*>(codes + row * 64 + ((t ^ ((row >> 1) & 3)) << 4) + half * 8);
+        w4_convert_word(v.x, s2[0], c2[0], h + 4 * t);
+        w4_convert_word(v.y, s2[NG - 1], c2[NG - 1], h + 16 + 4 * t);
     }
+    tc::tmem_st_32x32b_x32(tmem_dst, h);
+}
+
+// All 128 columns of channel `row` -> 64 tensor-memory columns.
+template <int GPT>
+__device__ __forceinline__ void w4_convert_tile(const uint8_t* codes, const uint8_t* scales, int row, float rowmul,
+                                                uint32_t tmem_dst) {
+    uint32_t s2[GPT], c2[GPT];
+    w4_scales<GPT>(scales, row, rowmul, 0, s2, c2, GPT);
     uint4 raw[4];
 #pragma unroll
     for (int t = 0; t < 4; ++t)
@@ -109,7 +124,12 @@ __device__ __forceinline__ void w4_convert_stage(const uint8_t* codes, const uin
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
         uint32_t h[32];
-        w4_convert_half<GPT>(raw, s2, c2, half, h);
+        const int ga = half * GPT / 2, gb = (2 * half + 1) * GPT / 4;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            w4_convert_word(half ? raw[t].z : raw[t].x, s2[ga], c2[ga], h + 4 * t);
+            w4_convert_word(half ? raw[t].w : raw[t].y, s2[gb], c2[gb], h + 16 + 4 * t);
+        }
         tc::tmem_st_32x32b_x32(tmem_dst + half * 32, h);
     }
 }
@@ -163,50 +183,104 @@ __device__ __forceinline__ void w4_finish(const GemmW4Params& p, const float (&v
 }
 
 // ---------------------------------------------------------------------------------------------
-// More than 128 rows: CTA pairs (cta_group::2), 256 channels x TOK tokens per pair.  Each CTA converts its own
-// 128 channels and loads half of the tokens.  SEG (TOK 128): segmented sums.
+// More than 128 rows: CTA pairs (cta_group::2), persistent.  A pair computes tiles of 256 channels x TOK tokens (with
+// two matrices: of both) one after the other; blocks of 128 k run through the rings without a break between
+// tiles.  Each CTA converts its own 128 channels and loads half of the tokens; both converter warpgroups work
+// on every block, on one half of its columns each (two matrices: on one matrix each).
+//
+// Results are taken out of tensor memory NA blocks behind the conversion, when their MMAs are known to be
+// done: the operand buffers of the next tile are then full, so the tensor cores wait only for the accumulator
+// to be read, and the stores run under the next tile's MMAs.  Without segments (16-bit results) there is one
+// accumulator of TOK * NMAT = 256 columns; with segments two of 128.
 // ---------------------------------------------------------------------------------------------
-template <int TOK, int PARTS>
-using W4Pair = W4Shape<TOK / 2, TOK, PARTS, TOK == 128, 512, 224 * 1024>;
+template <int PARTS, int NMAT, bool SEG>
+struct W4PairShape {
+    static constexpr int TOK = (SEG ? 128 : 256) / NMAT;
+    using S = W4Shape<TOK / 2, TOK, PARTS, NMAT, SEG ? 2 : 1, 512, 224 * 1024>;
+};
 
-template <int TOK, int PARTS, int NMAT, int GPT>
+template <class T>
+__device__ __forceinline__ T w4_round(float v);
+template <>
+__device__ __forceinline__ float w4_round<float>(float v) { return v; }
+template <>
+__device__ __forceinline__ __half w4_round<__half>(float v) { return __float2half_rn(v); }
+template <>
+__device__ __forceinline__ __nv_bfloat16 w4_round<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// One channel's results of CNT tokens from t0 on: consecutive lanes hold consecutive channels.
+template <class T, int CNT, class F>
+__device__ __forceinline__ void w4_put_as(const GemmW4Params& p, int t0, int n, F value) {
+    T* y = static_cast<T*>(p.y) + (int64_t)t0 * p.ldy + n;
+    if (t0 + CNT <= p.m) {
+#pragma unroll
+        for (int j = 0; j < CNT; ++j, y += p.ldy) *y = w4_round<T>(value(j));
+    } else {
+#pragma unroll
+        for (int j = 0; j < CNT; ++j, y += p.ldy)
+            if (t0 + j < p.m) *y = w4_round<T>(value(j));
+    }
+}
+
+template <int CNT, class F>
+__device__ __forceinline__ void w4_put(const GemmW4Params& p, int t0, int n, F value) {
+    if (n >= p.n) return;
+    if (p.y_dtype == SBQ_F32)
+        w4_put_as<float, CNT>(p, t0, n, value);
+    else if (p.y_dtype == SBQ_F16)
+        w4_put_as<__half, CNT>(p, t0, n, value);
+    else
+        w4_put_as<__nv_bfloat16, CNT>(p, t0, n, value);
+}
+
+// 32 tokens' factors (the array is padded to a multiple of 64 values).
+__device__ __forceinline__ void w4_times_xinv(const float* xinv, int t0, float* v) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const float4 f = __ldg(reinterpret_cast<const float4*>(xinv + t0) + j);
+        v[4 * j] *= f.x, v[4 * j + 1] *= f.y, v[4 * j + 2] *= f.z, v[4 * j + 3] *= f.w;
+    }
+}
+
+template <int PARTS, int NMAT, bool SEG, int GPT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
     gemm_w4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_lo,
                         const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2,
                         const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_s2,
                         const __grid_constant__ GemmW4Params p) {
-    using S = W4Pair<TOK, PARTS>;
-    constexpr bool SEG = TOK == 128;
-    constexpr int NS = S::kStages, NA = S::kABufs, COLS = TOK / 2;
+    using Shape = W4PairShape<PARTS, NMAT, SEG>;
+    using S = typename Shape::S;
+    constexpr int TOK = Shape::TOK, COLS = TOK / 2;  // tokens of a tile, tokens per converter warpgroup in the epilogue
+    constexpr int NS = S::kStages, NA = S::kABufs, ND = SEG ? 2 : 1;
+    constexpr int kMat = S::kCodes + S::kScales;     // one matrix of a stage
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* wfull = reinterpret_cast<uint64_t*>(smem + S::kBarOff);  // this CTA's codes and scales landed
     uint64_t* ready = wfull + NS;      // leader: both CTAs' x landed and both CTAs' converters wrote
     uint64_t* conv_done = ready + NS;  // this CTA's converters have read the codes
     uint64_t* mma_done = conv_done + NS;
-    uint64_t* done = mma_done + NS;    // per accumulator: its segment's (without segments: all) MMAs completed
-    uint64_t* taken = done + 2;        // leader, per accumulator: both CTAs' converters have added it up
+    uint64_t* done = mma_done + NS;    // per accumulator: the MMAs of its segment (tile) completed
+    uint64_t* taken = done + 2;        // leader, per accumulator: both CTAs' converters have read it
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 2);
-    float* s_mul = reinterpret_cast<float*>(smem + S::kBarOff + 512);
-    float* s_bias = s_mul + kW4Rows;
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_ctarank();
     const bool leader = rank == 0;
-    constexpr int kCh = kW4Rows / NMAT;
-    const int n0 = (int)blockIdx.x * kCh, t0 = blockIdx.y * TOK;
+    // tiles of this pair: pair, pair + npairs, ... (channels fastest)
+    const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
+    const int cols = (p.n + 2 * kW4Rows - 1) / (2 * kW4Rows), tiles = cols * ((p.m + TOK - 1) / TOK), kt = p.kt;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
             tc::mbar_init(&wfull[s], 1);
-            tc::mbar_init(&ready[s], 1 + 8);
-            tc::mbar_init(&conv_done[s], 4);
+            tc::mbar_init(&ready[s], 1 + 16);
+            tc::mbar_init(&conv_done[s], 8);
             tc::mbar_init(&mma_done[s], 1);
         }
-        tc::mbar_init(&done[0], 1);
-        tc::mbar_init(&done[1], 1);
-        tc::mbar_init(&taken[0], 16);
-        tc::mbar_init(&taken[1], 16);
+        for (int d = 0; d < 2; ++d) {
+            tc::mbar_init(&done[d], 1);
+            tc::mbar_init(&taken[d], 16);
+        }
         tc::fence_mbar_init();
         tc::prefetch_tmap(&map_x);
         tc::prefetch_tmap(&map_w);
@@ -216,11 +290,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
         tc::tmem_alloc_pair(tmem_slot, 512);
         tc::tmem_relinquish_pair();
     }
-    for (int i = threadIdx.x; i < kW4Rows; i += blockDim.x) {
-        const int n = w4_channel<NMAT>(n0, i);
-        s_mul[i] = n < p.n ? p.rowmul[NMAT == 2 ? i >> 6 : 0][n] : 1.0f;
-        s_bias[i] = p.bias && n < p.n ? p.bias[n] : 0.0f;
-    }
     tc::fence_before_sync();
     tc::cluster_sync();
     tc::fence_after_sync();
@@ -228,21 +297,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
 
     if (warp == 0) {
         if (lane == 0) {
-            const int tr = t0 + (int)rank * (TOK / 2);
-            auto load_w = [&](int kb) {
-                const int s = kb % NS;
+            // block g of the pair: its tile and k-block
+            auto load_w = [&](int s, int tile, int kb) {
                 uint8_t* ws = smem + s * S::kStage + S::kXBytes;
-                tc::mbar_arrive_expect_tx(&wfull[s], S::kCodes + 256 * GPT);
-                tc::tma_load_4d(ws, &map_w, &wfull[s], 0, 0, kb, n0 / 16);
-                tma_load_3d(ws + S::kCodes, &map_s, &wfull[s], 0, kb, n0 / 16);
+                const int nt = (tile % cols) * (2 * kW4Rows / 16) + (int)rank * (kW4Rows / 16);
+                tc::mbar_arrive_expect_tx(&wfull[s], NMAT * (S::kCodes + 256 * GPT));
+                tc::tma_load_4d(ws, &map_w, &wfull[s], 0, 0, kb, nt);
+                tma_load_3d(ws + S::kCodes, &map_s, &wfull[s], 0, kb, nt);
                 if (NMAT == 2) {
-                    tc::tma_load_4d(ws + S::kCodes / 2, &map_w2, &wfull[s], 0, 0, kb, n0 / 16);
-                    tma_load_3d(ws + S::kCodes + 128 * GPT, &map_s2, &wfull[s], 0, kb, n0 / 16);
+                    tc::tma_load_4d(ws + kMat, &map_w2, &wfull[s], 0, 0, kb, nt);
+                    tma_load_3d(ws + kMat + S::kCodes, &map_s2, &wfull[s], 0, kb, nt);
                 }
             };
-            auto load_x = [&](int kb) {
-                const int s = kb % NS;
+            auto load_x = [&](int s, int tile, int kb) {
                 uint8_t* xs = smem + s * S::kStage;
+                const int tr = (tile / cols) * TOK + (int)rank * (TOK / 2);
                 const uint32_t xb = tc::cluster_addr(&ready[s], 0);
                 if (leader) tc::mbar_arrive_expect_tx(&ready[s], 2 * S::kXBytes);
 #pragma unroll
@@ -251,121 +320,236 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
                     if (PARTS == 2) tc::tma_load_2d_pair(xs + (h * PARTS + 1) * S::kXSub, &map_lo, xb, kb * 128 + h * 64, tr);
                 }
             };
-            const int pre = p.kt < NS ? p.kt : NS;
-            for (int kb = 0; kb < pre; ++kb) load_w(kb);
+            // codes of the first stages before the wait for the previous kernel, x after it
+            int g = 0;
+            for (int tile = pair, kb = 0; tile < tiles && g < NS; ++g) {
+                load_w(g, tile, kb);
+                if (++kb == kt) kb = 0, tile += npairs;
+            }
+            const int pre = g;
             asm volatile("griddepcontrol.wait;" ::: "memory");
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            for (int kb = 0; kb < pre; ++kb) load_x(kb);
-            for (int kb = pre; kb < p.kt; ++kb) {
-                const int s = kb % NS;
-                const uint32_t ph = (kb / NS) & 1;
-                if (!tc::mbar_wait(&conv_done[s], ph ^ 1)) break;
-                if (!tc::mbar_wait(&mma_done[s], ph ^ 1)) break;
-                load_w(kb);
-                load_x(kb);
-            }
+            g = 0;
+            bool ok = true;
+            for (int tile = pair; tile < tiles && ok; tile += npairs)
+                for (int kb = 0; kb < kt; ++kb, ++g) {
+                    const int s = g % NS;
+                    if (g >= pre) {
+                        const uint32_t ph = ((g / NS) & 1) ^ 1;
+                        if (!tc::mbar_wait(&conv_done[s], ph) || !tc::mbar_wait(&mma_done[s], ph)) {
+                            ok = false;
+                            break;
+                        }
+                        load_w(s, tile, kb);
+                    }
+                    load_x(s, tile, kb);
+                }
         }
     } else if (warp == 1) {
         if (lane == 0 && leader) {
             constexpr uint32_t idesc = tc::idesc_f16(2 * kW4Rows, TOK, false);
-            for (int kb = 0; kb < p.kt; ++kb) {
-                const int s = kb % NS, seg = SEG ? kb / S::kSegBlocks : 0;
-                const bool fresh = SEG ? kb % S::kSegBlocks == 0 : kb == 0;
-                if (SEG && fresh && seg >= 2 && !tc::mbar_wait_cluster(&taken[seg & 1], ((seg >> 1) - 1) & 1)) break;
-                if (!tc::mbar_wait_cluster(&ready[s], (kb / NS) & 1)) break;
-                tc::fence_after_sync();
-                const uint8_t* xs = smem + s * S::kStage;
-                const uint32_t d = tmem + (seg & 1) * TOK, a = tmem + S::kACol + (kb % NA) * 64;
-#pragma unroll
-                for (int j = 0; j < 8; ++j)
-#pragma unroll
-                    for (int q = 0; q < PARTS; ++q) {
-                        const uint64_t bd = tc::smem_desc(xs + ((j >> 2) * PARTS + q) * S::kXSub + (j & 3) * 32, tc::kSwizzle128B, 1024);
-                        tc::mma_f16_ts_pair(d, a + j * 8, bd, idesc, !(fresh && j == 0 && q == 0));
+            int g = 0, seg = -1;
+            bool ok = true;
+            for (int tile = pair; tile < tiles && ok; tile += npairs)
+                for (int kb = 0; kb < kt; ++kb, ++g) {
+                    const int s = g % NS;
+                    const bool fresh = SEG ? kb % S::kSegBlocks == 0 : kb == 0;
+                    if (fresh && ++seg >= ND && !tc::mbar_wait_cluster(&taken[seg % ND], ((seg / ND) - 1) & 1)) {
+                        ok = false;
+                        break;
                     }
-                tc::mma_commit_pair(tc::cluster_addr(&mma_done[s], 0));
-                tc::mma_commit_pair(tc::cluster_addr(&mma_done[s], 1));
-                if (kb + 1 == p.kt || (SEG && (kb + 1) % S::kSegBlocks == 0)) {
-                    tc::mma_commit_pair(tc::cluster_addr(&done[seg & 1], 0));
-                    tc::mma_commit_pair(tc::cluster_addr(&done[seg & 1], 1));
+                    if (!tc::mbar_wait_cluster(&ready[s], (g / NS) & 1)) {
+                        ok = false;
+                        break;
+                    }
+                    tc::fence_after_sync();
+                    const uint8_t* xs = smem + s * S::kStage;
+#pragma unroll
+                    for (int a = 0; a < NMAT; ++a) {
+                        const uint32_t d = tmem + ((seg % ND) * NMAT + a) * TOK;
+                        const uint32_t op = tmem + S::kACol + ((g % NA) * NMAT + a) * 64;
+#pragma unroll
+                        for (int j = 0; j < 8; ++j)
+#pragma unroll
+                            for (int q = 0; q < PARTS; ++q) {
+                                const uint64_t bd =
+                                    tc::smem_desc(xs + ((j >> 2) * PARTS + q) * S::kXSub + (j & 3) * 32, tc::kSwizzle128B, 1024);
+                                tc::mma_f16_ts_pair(d, op + j * 8, bd, idesc, !(fresh && j == 0 && q == 0));
+                            }
+                    }
+                    tc::mma_commit_pair(tc::cluster_addr(&mma_done[s], 0));
+                    tc::mma_commit_pair(tc::cluster_addr(&mma_done[s], 1));
+                    if (kb + 1 == kt || (SEG && (kb + 1) % S::kSegBlocks == 0)) {
+                        tc::mma_commit_pair(tc::cluster_addr(&done[seg % ND], 0));
+                        tc::mma_commit_pair(tc::cluster_addr(&done[seg % ND], 1));
+                    }
                 }
-            }
         }
     } else if (warp >= 4) {
         const int grp = (warp - 4) >> 2, wq = (warp - 4) & 3, row = wq * 32 + lane;
         const uint32_t lane_tmem = tmem + ((uint32_t)(wq * 32) << 16);
-        const float mul = s_mul[row];
-        float sum[SEG ? COLS : 32];
-        int taken_segs = 0;
-        // the next segment: waits for its MMAs.  A segment's accumulator is filled again only after it was
-        // taken, so its barrier is never more than one phase ahead.
+        const int cn = (int)rank * kW4Rows + row;  // this thread's channel within a tile's 256
+        auto mul_of = [&](int mat, int tile) {
+            const int n = (tile % cols) * (2 * kW4Rows) + cn;
+            return tile < tiles && n < p.n ? __ldg(p.rowmul[mat] + n) : 1.0f;
+        };
+        float sum[SEG ? NMAT * COLS : 1];
+        // the next segment to be taken, the global number of its last block, its tile and that one's last block
+        int seg = 0, tk_tile = pair, tk_end = kt - 1;
+        int tk_last = SEG && S::kSegBlocks < kt ? S::kSegBlocks - 1 : kt - 1;
+        bool tk_first = true;
         auto take = [&]() -> bool {
-            if constexpr (SEG) {
-                if (!__all_sync(0xffffffffu, tc::mbar_wait(&done[taken_segs & 1], (taken_segs >> 1) & 1))) return false;
-                tc::fence_after_sync();
-                w4_take_segment<COLS>(lane_tmem + (taken_segs & 1) * TOK + grp * COLS, sum, taken_segs == 0);
+            const int d = seg % ND;
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(&done[d], (seg / ND) & 1))) return false;
+            tc::fence_after_sync();
+            const uint32_t src = lane_tmem + d * NMAT * TOK + grp * COLS;
+            const bool last = tk_last == tk_end;
+            const int n = (tk_tile % cols) * (2 * kW4Rows) + cn, t0 = (tk_tile / cols) * TOK + grp * COLS;
+            auto release = [&]() {
                 tc::fence_before_sync();
                 __syncwarp();
-                if (lane == 0) tc::mbar_arrive_cluster(tc::cluster_addr(&taken[taken_segs & 1], 0));
-                ++taken_segs;
+                if (lane == 0) tc::mbar_arrive_cluster(tc::cluster_addr(&taken[d], 0));
+            };
+            float inv[NMAT], bias = 0.0f;
+            if (last) {
+#pragma unroll
+                for (int a = 0; a < NMAT; ++a) inv[a] = 1.0f / mul_of(a, tk_tile);
+                if (NMAT == 1 && p.bias && n < p.n) bias = __ldg(p.bias + n);
+            }
+            if constexpr (SEG) {
+#pragma unroll
+                for (int a = 0; a < NMAT; ++a)
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+                        uint32_t r[32];
+                        tc::tmem_ld_32x32b_x32(src + a * TOK + c * 32, r);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 32; ++j) {
+                            const float v = __uint_as_float(r[j]);
+                            float& o = sum[a * COLS + c * 32 + j];
+                            o = tk_first ? v : o + v;
+                        }
+                    }
+                release();
+                if (last) {
+#pragma unroll
+                    for (int c = 0; c < COLS / 32; ++c) {
+#pragma unroll
+                        for (int a = 0; a < NMAT; ++a) {
+                            float* v = sum + a * COLS + c * 32;
+#pragma unroll
+                            for (int j = 0; j < 32; ++j) v[j] *= inv[a];
+                            if (p.xinv) w4_times_xinv(p.xinv, t0 + c * 32, v);
+                        }
+                        w4_put<32>(p, t0 + c * 32, n, [&](int j) {
+                            const float v = sum[c * 32 + j];
+                            return NMAT == 2 ? w4_silu(v) * sum[(NMAT - 1) * COLS + c * 32 + j] : v + bias;
+                        });
+                    }
+                }
+            } else if constexpr (NMAT == 1) {
+                // 128 tokens, rounded here: half the registers until they are stored
+                uint32_t h[COLS / 2];
+                const bool f16 = p.y_dtype == SBQ_F16;
+#pragma unroll
+                for (int c = 0; c < COLS / 32; ++c) {
+                    uint32_t r[32];
+                    tc::tmem_ld_32x32b_x32(src + c * 32, r);
+                    tc::tmem_wait_ld();
+                    float v[32];
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * inv[0];
+                    if (p.xinv) w4_times_xinv(p.xinv, t0 + c * 32, v);
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) {
+                        const __half2 a = __floats2half2_rn(v[2 * j] + bias, v[2 * j + 1] + bias);
+                        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j] + bias, v[2 * j + 1] + bias);
+                        h[c * 16 + j] = f16 ? *reinterpret_cast<const uint32_t*>(&a) : *reinterpret_cast<const uint32_t*>(&b);
+                    }
+                }
+                release();
+                if (n < p.n) {
+                    uint16_t* y = static_cast<uint16_t*>(p.y) + (int64_t)t0 * p.ldy + n;
+#pragma unroll
+                    for (int j = 0; j < COLS; ++j, y += p.ldy)
+                        if (t0 + j < p.m) *y = (uint16_t)(j & 1 ? h[j >> 1] >> 16 : h[j >> 1] & 0xFFFFu);
+                }
+            } else {
+                float gv[COLS], uv[COLS];
+#pragma unroll
+                for (int c = 0; c < COLS / 32; ++c) {
+                    tc::tmem_ld_32x32b_x32(src + c * 32, *reinterpret_cast<uint32_t(*)[32]>(gv + c * 32));
+                    tc::tmem_ld_32x32b_x32(src + TOK + c * 32, *reinterpret_cast<uint32_t(*)[32]>(uv + c * 32));
+                }
+                tc::tmem_wait_ld();
+                release();
+#pragma unroll
+                for (int c = 0; c < COLS / 32; ++c) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) gv[c * 32 + j] *= inv[0], uv[c * 32 + j] *= inv[NMAT - 1];
+                    if (p.xinv) {
+                        w4_times_xinv(p.xinv, t0 + c * 32, gv + c * 32);
+                        w4_times_xinv(p.xinv, t0 + c * 32, uv + c * 32);
+                    }
+                    // a 16-bit result: the approximate exponential and division (a few 2^-22) are far below its rounding
+                    w4_put<32>(p, t0 + c * 32, n, [&](int j) {
+                        const float v = gv[c * 32 + j];
+                        return __fdividef(v, 1.0f + __expf(-v)) * uv[c * 32 + j];
+                    });
+                }
+            }
+            ++seg;
+            tk_first = last;
+            if (last) {
+                tk_tile += npairs;
+                tk_end += kt;
+                tk_last = SEG && S::kSegBlocks < kt ? tk_last + S::kSegBlocks : tk_end;
+            } else {
+                tk_last = tk_last + S::kSegBlocks < tk_end ? tk_last + S::kSegBlocks : tk_end;
             }
             return true;
         };
-        bool ok = true;
-        for (int kb = grp; kb < p.kt; kb += 2) {
-            const int s = kb % NS;
-            // the operand buffer was last read by k-block kb - NA; waiting for its MMAs also puts every
-            // earlier phase of this stage's barriers behind us (NA <= NS), so a parity names one phase
-            if (kb >= NA) {
-                const int prev = kb - NA;
-                if (!__all_sync(0xffffffffu, tc::mbar_wait(&mma_done[prev % NS], (prev / NS) & 1))) { ok = false; break; }
+        int g = 0;
+        bool ok = true, waited = false;
+        const int mat = NMAT == 2 ? grp : 0;
+        float mul = mul_of(mat, pair);
+        for (int tile = pair; tile < tiles && ok; tile += npairs) {
+            const float next_mul = mul_of(mat, tile + npairs);
+            for (int kb = 0; kb < kt; ++kb, ++g) {
+                const int s = g % NS;
+                if (g >= NA) {
+                    // the operand buffer was last read by block g - NA.  Every warp takes every block, and
+                    // NA <= NS, so each barrier is at most one phase from the one awaited
+                    const int prev = g - NA;
+                    if (!__all_sync(0xffffffffu, tc::mbar_wait(&mma_done[prev % NS], (prev / NS) & 1))) { ok = false; break; }
+                    if (tk_last <= prev && !waited) {
+                        asm volatile("griddepcontrol.wait;" ::: "memory");  // before y is written, and xinv read
+                        waited = true;
+                    }
+                    while (ok && tk_last <= prev) ok = take();
+                    if (!ok) break;
+                }
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&wfull[s], (g / NS) & 1))) { ok = false; break; }
+                tc::fence_after_sync();
+                const uint8_t* codes = smem + s * S::kStage + S::kXBytes + mat * kMat;
+                const uint32_t dst = lane_tmem + S::kACol + (g % NA) * NMAT * 64;
+                if (NMAT == 2)
+                    w4_convert_tile<GPT>(codes, codes + S::kCodes, row, mul, dst + mat * 64);
+                else
+                    w4_convert_half<GPT>(codes, codes + S::kCodes, row, mul, grp, dst + grp * 32);
+                tc::tmem_wait_st();
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) {
+                    tc::mbar_arrive_cluster(tc::cluster_addr(&ready[s], 0));
+                    tc::mbar_arrive(&conv_done[s]);
+                }
             }
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(&wfull[s], (kb / NS) & 1))) { ok = false; break; }
-            tc::fence_after_sync();
-            const uint8_t* codes = smem + s * S::kStage + S::kXBytes;
-            w4_convert_stage<GPT>(codes, codes + S::kCodes, row, mul, lane_tmem + S::kACol + (kb % NA) * 64);
-            tc::tmem_wait_st();
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) {
-                tc::mbar_arrive_cluster(tc::cluster_addr(&ready[s], 0));
-                tc::mbar_arrive(&conv_done[s]);
-            }
-            // a segment is taken NA blocks after its last one: its MMAs are done by then (the wait above), and
-            // the MMAs of the segment after the next, which need its accumulator, are not due yet
-            if (SEG && kb - NA + 1 >= (taken_segs + 1) * S::kSegBlocks && !(ok = take())) break;
+            mul = next_mul;
         }
-        if constexpr (SEG) {
-            while (ok && taken_segs * S::kSegBlocks < p.kt) ok = take();
-        } else {
-            ok = __all_sync(0xffffffffu, ok && tc::mbar_wait(&done[0], 0));
-            tc::fence_after_sync();
-        }
-        asm volatile("griddepcontrol.wait;" ::: "memory");  // before y is written, and xinv read
-        const int n = w4_channel<NMAT>(n0, row);
-        const float inv = 1.0f / mul, bias = s_bias[row];
-        float* xch = reinterpret_cast<float*>(smem) + grp * 32 * 64;
-        // every MMA of the pair is done, so the ring is free for the exchange
-#pragma unroll
-        for (int c = 0; c < COLS / 32; ++c) {
-            const int tb = t0 + grp * COLS + c * 32;
-            float v[32];
-            if constexpr (SEG) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = sum[32 * c + j] * inv;
-            } else {
-                uint32_t r[32];
-                tc::tmem_ld_32x32b_x32(lane_tmem + grp * COLS + c * 32, r);
-                tc::tmem_wait_ld();
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * inv;
-            }
-            if (p.xinv) {
-#pragma unroll
-                for (int j = 0; j < 32; ++j) v[j] *= tb + j < p.m ? p.xinv[tb + j] : 0.0f;
-            }
-            w4_finish<NMAT>(p, v, tb, n, row, grp, bias, xch, ok);
-        }
+        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
+        while (ok && tk_tile < tiles) ok = take();
     }
     tc::fence_before_sync();
     tc::cluster_sync();
@@ -382,7 +566,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
 // ---------------------------------------------------------------------------------------------
 constexpr int kSTok4 = 64;
 template <int PARTS>
-using W4Small = W4Shape<kSTok4, kSTok4, PARTS, true, 256, 108 * 1024>;
+using W4Small = W4Shape<kSTok4, kSTok4, PARTS, 1, 2, 256, 108 * 1024>;
 
 template <int PARTS, int NMAT, int GPT>
 __global__ void __launch_bounds__(kW4Threads, 2)
@@ -530,7 +714,7 @@ __global__ void __launch_bounds__(kW4Threads, 2)
             if (!__all_sync(0xffffffffu, tc::mbar_wait(&wfull[s], (i / NS) & 1))) { ok = false; break; }
             tc::fence_after_sync();
             const uint8_t* codes = smem + s * S::kStage + S::kXBytes;
-            w4_convert_stage<GPT>(codes, codes + S::kCodes, row, mul, lane_tmem + S::kACol + (i % NA) * 64);
+            w4_convert_tile<GPT>(codes, codes + S::kCodes, row, mul, lane_tmem + S::kACol + (i % NA) * 64);
             tc::tmem_wait_st();
             tc::fence_before_sync();
             __syncwarp();
@@ -598,7 +782,8 @@ struct W4Maps {
     CUtensorMap x, lo, w[2], s[2];
 };
 
-static int make_maps(W4Maps& m, const W4Call& c, const W4Acts& x, int x_rows) {
+// x in boxes of `x_rows` tokens, codes and scales in boxes of `w_rows` channels.
+static int make_maps(W4Maps& m, const W4Call& c, const W4Acts& x, int x_rows, int w_rows) {
     const uint64_t xd[2] = {(uint64_t)c.k, (uint64_t)c.m}, xs[1] = {(uint64_t)x.ld * 2};
     const uint32_t xb[2] = {64, (uint32_t)x_rows};
     int st = encode_tmap(&m.x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x.part[0], xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B);
@@ -606,13 +791,12 @@ static int make_maps(W4Maps& m, const W4Call& c, const W4Acts& x, int x_rows) {
     if (!st && x.part[1]) st = encode_tmap(&m.lo, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, x.part[1], xd, xs, xb, CU_TENSOR_MAP_SWIZZLE_128B);
     const int nmat = c.w[1].packed ? 2 : 1;
     const uint64_t kt = (uint64_t)w4_tiles_k(c.k), nt = (uint64_t)ceil_div(c.n, kTileRows), sb = 32 * (uint64_t)c.gpt;
-    const uint32_t rows = kW4Rows / 16 / nmat;
     for (int i = 0; i < nmat && !st; ++i) {
         const uint64_t wd[4] = {64, 16, kt, nt}, ws[3] = {64, 1024, kt * 1024};
-        const uint32_t wb[4] = {64, 16, 1, rows};
+        const uint32_t wb[4] = {64, 16, 1, (uint32_t)w_rows / 16};
         st = encode_tmap(&m.w[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 4, c.w[i].packed, wd, ws, wb, CU_TENSOR_MAP_SWIZZLE_64B);
         const uint64_t sd[3] = {sb, kt, nt}, ss[2] = {sb, kt * sb};
-        const uint32_t bb[3] = {(uint32_t)sb, 1, rows};
+        const uint32_t bb[3] = {(uint32_t)sb, 1, (uint32_t)w_rows / 16};
         if (!st) st = encode_tmap(&m.s[i], CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, c.w[i].scales, sd, ss, bb, CU_TENSOR_MAP_SWIZZLE_NONE);
     }
     if (nmat == 1) m.w[1] = m.w[0], m.s[1] = m.s[0];
@@ -640,19 +824,21 @@ static cudaError_t launch_maps(K kernel, dim3 grid, int smem, int parts, cudaStr
     return cudaLaunchKernelEx(&cfg, kernel, m.x, m.lo, m.w[0], m.w[1], m.s[0], m.s[1], p);
 }
 
+template <int PARTS, int NMAT, bool SEG, int GPT>
+static cudaError_t launch_pair_w4(const W4Maps& m, const GemmW4Params& p, cudaStream_t s) {
+    using Shape = W4PairShape<PARTS, NMAT, SEG>;
+    const int64_t tiles = ceil_div(p.n, 2 * kW4Rows) * ceil_div(p.m, Shape::TOK), pairs = w4_sm_count() / 2;
+    return launch_maps(gemm_w4_pair_kernel<PARTS, NMAT, SEG, GPT>, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))),
+                       Shape::S::kBytes, 0, s, m, p);
+}
+
 template <int PARTS, int NMAT, int GPT>
 static cudaError_t launch_gemm_w4(int tok, const W4Maps& m, const GemmW4Params& p, cudaStream_t s) {
-    constexpr int kCh = kW4Rows / NMAT;
     if (tok == kSTok4)
         return launch_maps(gemm_w4_small_kernel<PARTS, NMAT, GPT>,
-                           dim3((unsigned)ceil_div(p.n, kCh), (unsigned)ceil_div(p.m, kSTok4), (unsigned)p.parts),
+                           dim3((unsigned)ceil_div(p.n, kW4Rows / NMAT), (unsigned)ceil_div(p.m, kSTok4), (unsigned)p.parts),
                            W4Small<PARTS>::kBytes, p.parts, s, m, p);
-    const unsigned gx = 2 * (unsigned)ceil_div(p.n, 2 * kCh);
-    if (tok == 128)
-        return launch_maps(gemm_w4_pair_kernel<128, PARTS, NMAT, GPT>, dim3(gx, (unsigned)ceil_div(p.m, 128)),
-                           W4Pair<128, PARTS>::kBytes, 0, s, m, p);
-    return launch_maps(gemm_w4_pair_kernel<256, PARTS, NMAT, GPT>, dim3(gx, (unsigned)ceil_div(p.m, 256)),
-                       W4Pair<256, PARTS>::kBytes, 0, s, m, p);
+    return tok == 128 ? launch_pair_w4<PARTS, NMAT, true, GPT>(m, p, s) : launch_pair_w4<PARTS, NMAT, false, GPT>(m, p, s);
 }
 
 template <int PARTS, int NMAT>
@@ -686,12 +872,12 @@ int gemm_w4_run(const W4Call& c, const W4Acts& x) {
         const int64_t tiles = ceil_div(c.n, ch) * ceil_div(c.m, kSTok4);
         while (p.parts < 8 && tiles * (2 * p.parts) * 8 <= (int64_t)2 * sms * 7 && p.kt / (2 * p.parts) >= 2) p.parts *= 2;
     } else {
-        // 256-token tiles for 16-bit results (see the top), unless they leave SMs without work
-        const int64_t cols = ceil_div(c.n, 2 * ch), pairs = cols * ceil_div(c.m, 256);
-        tok = c.y_dtype == SBQ_F32 || pairs * 10 < (int64_t)(sms / 2) * 9 ? 128 : 256;
+        // one accumulator per tile for 16-bit results (see the top), unless that leaves pairs without a tile
+        const int64_t cols = ceil_div(c.n, 2 * kW4Rows), wide = cols * ceil_div(c.m, 256 / nmat);
+        tok = c.y_dtype == SBQ_F32 || wide * 10 < (int64_t)(sms / 2) * 9 ? 128 : 256;
     }
     W4Maps maps;
-    const int st = make_maps(maps, c, x, tok == kSTok4 ? kSTok4 : tok / 2);
+    const int st = tok == kSTok4 ? make_maps(maps, c, x, kSTok4, ch) : make_maps(maps, c, x, tok / nmat / 2, kW4Rows);
     if (st) return st;
     const cudaError_t e = x.part[1] ? (nmat == 2 ? launch_gemm_w4_g<2, 2>(c.gpt, tok, maps, p, c.stream)
                                                  : launch_gemm_w4_g<2, 1>(c.gpt, tok, maps, p, c.stream))

@@ -174,7 +174,8 @@ using namespace sbq;
 
 extern "C" size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t k, int x_dtype) {
     if (m <= 0 || k <= 0 || !w4_needs_parts(m, x_dtype)) return 0;
-    return (x_dtype == SBQ_F32 ? 2 : 1) * align256((size_t)m * k * 2) + align256((size_t)m * 4);
+    // the factors are read 32 at a time: rounded up to the largest token tile
+    return (x_dtype == SBQ_F32 ? 2 : 1) * align256((size_t)m * k * 2) + (size_t)ceil_div(m, 256) * 1024;
 }
 
 extern "C" int sbq_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* packed, const void* scales,

@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .quant import (_DTYPE_CODE, Int4Linear, Int8Linear, _current, _int4_workspace, _prepare_x, _ptr, _rows16, _stream,
+from .quant import (_DTYPE_CODE, Int4Linear, Int8Linear, _in_place, _int4_workspace, _prepare_x, _ptr, _raw_stream, _stream,
                     _workspace)
 
 
@@ -53,12 +53,14 @@ class FusedGatedMLP(nn.Module):
 
     def gateup(self, x: torch.Tensor) -> torch.Tensor:
         """The hidden activation alone: silu(gate(x)) * up(x) in ``h_dtype``, x as ``forward`` takes it."""
-        dev = self.gate_proj.packed.device
-        x2, _, on_host = _rows16(x, self.gate_proj.in_features, dev)
-        n = self.gate_proj.out_features
-        h = self.gateup_into(x2, torch.empty(x2.shape[0], n, dtype=self.h_dtype, device=dev))
-        if x.dim() != 2:
-            h = h.view(*x.shape[:-1], n)
+        gate = self.gate_proj
+        k, n, dev = gate.in_features, gate.out_features, gate.packed.device
+        if self.int4 and _in_place(x, k, dev):
+            h = torch.empty((*x.shape[:-1], n), dtype=self.h_dtype, device=dev)
+            self._run_int4(x, x.numel() // k, k, k, h, n, dev)
+            return h
+        x2, _, on_host = _prepare_x(x, k, dev)
+        h = self.gateup_into(x2, torch.empty(x2.shape[0], n, dtype=self.h_dtype, device=dev)).view(*x.shape[:-1], n)
         return h.to("cpu") if on_host else h
 
     def gateup_job(self, x2: torch.Tensor, h: torch.Tensor) -> L.GemvJob:
@@ -92,22 +94,29 @@ class FusedGatedMLP(nn.Module):
 
     def _gateup_int4(self, x2: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
         m, n, k = x2.shape[0], self.gate_proj.out_features, (self.gate_proj.in_features + 15) // 16 * 16
-        g, u = self.gate_proj._buffers, self.up_proj._buffers
-        dev = g["packed"].device
+        dev = self.gate_proj.packed.device
         if h.shape != (m, n) or (n > 1 and h.stride(1) != 1) or h.dtype not in _DTYPE_CODE or h.device != dev:
             raise ValueError("hidden activation must be an fp32/fp16/bf16 [%d, %d] view with unit column stride" % (m, n))
         if x2.shape[1] != k or x2.stride(1) != 1 or x2.dtype not in _DTYPE_CODE or x2.device != dev:
             raise ValueError("input must be an fp32/fp16/bf16 [m, %d] view with unit column stride" % k)
-        if m > 0:
-            code = _DTYPE_CODE[x2.dtype]
-            with _current(dev):
-                ws, ws_bytes = _int4_workspace(m, k, code, dev)
-                L.call("sbq_mlp_gateup_w4", x2.data_ptr(), code, x2.stride(0) if m > 1 else k, g["packed"].data_ptr(),
-                       g["scales"].data_ptr(), g["rowmul"].data_ptr(), u["packed"].data_ptr(), u["scales"].data_ptr(),
-                       u["rowmul"].data_ptr(), self.gate_proj.group, m, n, k, h.data_ptr(), _DTYPE_CODE[h.dtype],
-                       h.stride(0) if m > 1 else n, None if ws is None else ws.data_ptr(), ws_bytes,
-                       torch.cuda.current_stream(dev).cuda_stream)
+        self._run_int4(x2, m, k, x2.stride(0) if m > 1 else k, h, h.stride(0) if m > 1 else n, dev)
         return h
+
+    def _run_int4(self, x: torch.Tensor, m: int, k: int, ldx: int, h: torch.Tensor, ldh: int, dev: torch.device) -> None:
+        if m == 0:
+            return
+        if dev.index != torch._C._cuda_getDevice():  # the library launches on the current device
+            with torch.cuda.device(dev):
+                return self._run_int4(x, m, k, ldx, h, ldh, dev)
+        gate, code = self.gate_proj, _DTYPE_CODE[x.dtype]
+        g, u = gate._buffers, self.up_proj._buffers
+        ws, ws_bytes = _int4_workspace(m, k, code, dev)
+        status = L.load().sbq_mlp_gateup_w4(
+            x.data_ptr(), code, ldx, g["packed"].data_ptr(), g["scales"].data_ptr(), g["rowmul"].data_ptr(),
+            u["packed"].data_ptr(), u["scales"].data_ptr(), u["rowmul"].data_ptr(), gate.group, m, gate.out_features, k,
+            h.data_ptr(), _DTYPE_CODE[h.dtype], ldh, None if ws is None else ws.data_ptr(), ws_bytes, _raw_stream(dev))
+        if status:
+            L.check(status, "sbq_mlp_gateup_w4")
 
 
 def fuse_gated_mlp(model: nn.Module, h_dtype: torch.dtype = torch.float16) -> int:

@@ -16,26 +16,31 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .quant import _DTYPE_CODE, _current
+from .quant import _DTYPE_CODE, _raw_stream
 
 
-def _rows(t: torch.Tensor, d: int, what: str, dev: torch.device) -> torch.Tensor:
-    """t as [m, d] with unit column stride on ``dev`` (a copy only if its rows are not evenly strided)."""
+def _rows(t: torch.Tensor, d: int, what: str, dev: torch.device) -> tuple[torch.Tensor, int]:
+    """(t, row stride) of t as [m, d] with unit column stride (t is a copy only if its rows are not evenly strided)."""
     if t.device != dev:
         raise ValueError("%s must be on the residual's device %s, got %s" % (what, dev, t.device))
     if t.dtype not in _DTYPE_CODE:
         raise ValueError("%s must be fp32, fp16 or bf16, got %s" % (what, t.dtype))
+    if t.is_contiguous():
+        return t, d
     t = t if t.dim() == 2 else t.reshape(-1, d)
-    return t if (t.stride(1) == 1 or d == 1) and (t.shape[0] <= 1 or t.stride(0) >= d) else t.contiguous()
+    if (t.stride(1) == 1 or d == 1) and (t.shape[0] <= 1 or t.stride(0) >= d):
+        return t, t.stride(0) if t.shape[0] > 1 else d
+    return t.contiguous(), d
 
 
 def _weight(w: torch.Tensor, d: int, what: str, dev: torch.device) -> torch.Tensor:
-    if tuple(w.shape) != (d,):
+    if w.shape != (d,):
         raise ValueError("%s must have shape (%d,), got %s" % (what, d, tuple(w.shape)))
     if w.device != dev:
         raise ValueError("%s must be on the residual's device %s, got %s" % (what, dev, w.device))
-    w = w if w.dtype == torch.float32 else w.float()
-    return w if d == 1 or w.stride(0) == 1 else w.contiguous()
+    if w.dtype != torch.float32:
+        w = w.float()
+    return w if w.is_contiguous() else w.contiguous()
 
 
 def residual_norm(branch: torch.Tensor | None, residual: torch.Tensor, pre_weight: torch.Tensor | None = None, *,
@@ -55,71 +60,81 @@ def residual_norm(branch: torch.Tensor | None, residual: torch.Tensor, pre_weigh
     the residual's type; it may be the residual itself); with no branch, a residual_scale of 1 and no
     ``residual_out`` the residual is returned as it is.
     """
-    if not residual.is_cuda:
-        raise ValueError("residual_norm runs on a CUDA device, got " + str(residual.device))
-    if residual.dim() == 0 or residual.shape[-1] == 0:
-        raise ValueError("residual must have a last dimension to normalise over, got shape %s" % (tuple(residual.shape),))
-    dev, shape, d = residual.device, residual.shape, residual.shape[-1]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (branch, residual, gate)):
+    dev, shape = residual.device, residual.shape
+    if dev.type != "cuda":
+        raise ValueError("residual_norm runs on a CUDA device, got " + str(dev))
+    if not shape or shape[-1] == 0:
+        raise ValueError("residual must have a last dimension to normalise over, got shape %s" % (tuple(shape),))
+    if dev.index != torch._C._cuda_getDevice():  # the library launches on the current device
+        with torch.cuda.device(dev):
+            return residual_norm(branch, residual, pre_weight, post_weight=post_weight, gate=gate, gate_act=gate_act,
+                                 residual_scale=residual_scale, branch_scale=branch_scale, eps=eps, out_dtype=out_dtype,
+                                 residual_out=residual_out)
+    if torch.is_grad_enabled() and (residual.requires_grad or (branch is not None and branch.requires_grad) or
+                                    (gate is not None and gate.requires_grad)):
         raise ValueError("residual_norm has no gradient: call it under torch.no_grad() or detach its inputs")
-    if gate_act not in L.GATE_ACTS:
+    act = L.GATE_ACTS.get(gate_act)
+    if act is None:
         raise ValueError("unknown gate activation %s (one of %s)" % (gate_act, ", ".join(L.GATE_ACTS)))
-    if out_dtype not in _DTYPE_CODE:
+    out_code = _DTYPE_CODE.get(out_dtype)
+    if out_code is None:
         raise ValueError("output dtype must be fp32, fp16 or bf16, got %s" % out_dtype)
     if not eps >= 0.0:
         raise ValueError("eps must not be negative")
-    if branch is None and (gate is not None or post_weight is not None):
-        raise ValueError("a gate or post_weight needs a branch")
-    if branch is not None and branch.shape != shape:
-        raise ValueError("branch %s and residual %s must have the same shape" % (tuple(branch.shape), tuple(shape)))
-    r = _rows(residual, d, "residual", dev)
-    m = r.shape[0]
-    a = L.ResidualNormArgs(residual=r.data_ptr(), ld_residual=r.stride(0), residual_dtype=_DTYPE_CODE[r.dtype], m=m, d=d,
-                           gate_act=L.GATE_ACTS[gate_act], residual_scale=residual_scale, branch_scale=branch_scale,
-                           eps=eps, out_dtype=_DTYPE_CODE[out_dtype])
-    keep = [r]  # operands that may be copies live until the launch is queued
+    d = shape[-1]
+    a = L.ResidualNormArgs()
+    # every operand (`r`, `y`, `g` and the weights) may be a copy: it stays referenced until the launch is queued
+    r, a.ld_residual = _rows(residual, d, "residual", dev)
+    a.residual, a.residual_dtype = r.data_ptr(), _DTYPE_CODE[r.dtype]
+    m = residual.numel() // d
+    a.m, a.d = m, d
+    a.gate_act, a.residual_scale, a.branch_scale, a.eps, a.out_dtype = act, residual_scale, branch_scale, eps, out_code
     if branch is not None:
-        y = _rows(branch, d, "branch", dev)
-        keep.append(y)
-        a.branch, a.ld_branch, a.branch_dtype = y.data_ptr(), y.stride(0), _DTYPE_CODE[y.dtype]
+        if branch.shape != shape:
+            raise ValueError("branch %s and residual %s must have the same shape" % (tuple(branch.shape), tuple(shape)))
+        y, a.ld_branch = _rows(branch, d, "branch", dev)
+        a.branch, a.branch_dtype = y.data_ptr(), _DTYPE_CODE[y.dtype]
+    elif gate is not None or post_weight is not None:
+        raise ValueError("a gate or post_weight needs a branch")
     if gate is not None:
-        if tuple(gate.shape) == (d,) and gate.dim() == 1:
-            g = _rows(gate.view(1, d) if gate.stride(0) == 1 or d == 1 else gate.reshape(1, d), d, "gate", dev)
+        if gate.dim() == 1 and gate.shape[0] == d:
+            g, a.ld_gate = _rows(gate.view(1, d), d, "gate", dev)
             a.gate_mode = L.GATE_PER_COLUMN
         elif gate.shape == shape:
-            g = _rows(gate, d, "gate", dev)
+            g, a.ld_gate = _rows(gate, d, "gate", dev)
             a.gate_mode = L.GATE_FULL
         elif gate.shape == (*shape[:-1], 1):
-            g = _rows(gate, 1, "gate", dev)
+            g, a.ld_gate = _rows(gate, 1, "gate", dev)
             a.gate_mode = L.GATE_PER_ROW
         else:
             raise ValueError("gate must have shape (%d,), %s or %s, got %s" % (d, (*shape[:-1], 1), tuple(shape), tuple(gate.shape)))
-        keep.append(g)
-        a.gate, a.ld_gate, a.gate_dtype = g.data_ptr(), g.stride(0), _DTYPE_CODE[g.dtype]
+        a.gate, a.gate_dtype = g.data_ptr(), _DTYPE_CODE[g.dtype]
     if post_weight is not None:
-        w = _weight(post_weight, d, "post_weight", dev)
-        keep.append(w)
-        a.post_weight = w.data_ptr()
+        wp = _weight(post_weight, d, "post_weight", dev)
+        a.post_weight = wp.data_ptr()
     x = None
     if pre_weight is not None:
         w = _weight(pre_weight, d, "pre_weight", dev)
-        keep.append(w)
         x = torch.empty(shape, dtype=out_dtype, device=dev)
         a.pre_weight, a.out, a.ld_out = w.data_ptr(), x.data_ptr(), d
-    if residual_out is None and branch is None and residual_scale == 1.0:
-        new = residual
-    else:
-        new = torch.empty(shape, dtype=residual.dtype, device=dev) if residual_out is None else residual_out
-        if new.shape != shape or new.dtype != residual.dtype or new.device != dev:
+    if residual_out is not None:
+        if residual_out.shape != shape or residual_out.dtype != residual.dtype or residual_out.device != dev:
             raise ValueError("residual_out must be a %s tensor of shape %s on %s" % (residual.dtype, tuple(shape), dev))
+        new = residual_out
         if m > 0:
             o = new if new.dim() == 2 else new.reshape(-1, d)
             if o.data_ptr() != new.data_ptr() or (d > 1 and o.stride(1) != 1) or (m > 1 and o.stride(0) < d):
                 raise ValueError("residual_out must be rows of unit stride at an even distance")
-            a.residual_out, a.ld_residual_out = o.data_ptr(), o.stride(0)
-    if m > 0 and (a.out or a.residual_out):
-        with _current(dev):
-            L.call("sbq_residual_norm", ctypes.byref(a), torch.cuda.current_stream(dev).cuda_stream)
+            a.residual_out, a.ld_residual_out = new.data_ptr(), o.stride(0) if m > 1 else d
+    elif branch is None and residual_scale == 1.0:
+        new = residual
+    else:
+        new = torch.empty(shape, dtype=residual.dtype, device=dev)
+        a.residual_out, a.ld_residual_out = new.data_ptr(), d
+    if m > 0 and (x is not None or new is not residual or residual_out is not None):
+        status = L.load().sbq_residual_norm(ctypes.byref(a), _raw_stream(dev))
+        if status:
+            L.check(status, "sbq_residual_norm")
     return new, x
 
 

@@ -323,9 +323,6 @@ class DynamicInt8Linear(_PackedLinear):
 
 # ---- format int4: 4-bit weights with group scales ------------------------------------------------
 
-_Y_CODE = _DTYPE_CODE  # the 4-bit kernels write fp32, fp16 or bf16
-
-
 def _check_group(group: int) -> int:
     if group not in INT4_GROUPS:
         raise ValueError("group size must be one of %s, got %s" % (INT4_GROUPS, group))
@@ -403,12 +400,15 @@ def quantize_per_group(weight: torch.Tensor, group: int = 128, device=None) -> t
     return unpack_int4(packed, scales, *weight.shape, group)
 
 
-def _rows16(x: torch.Tensor, k: int, device: torch.device):
-    """``_prepare_x`` with a shortcut for what a decode loop passes: ``(x2, k16, on_host)``."""
-    if x.device == device and k % 16 == 0 and x.shape[-1] == k and x.dtype in _DTYPE_CODE and x.is_contiguous() \
-            and x.data_ptr() % 16 == 0:
-        return x.view(-1, k), k, False
-    return _prepare_x(x, k, device)
+def _raw_stream(device: torch.device) -> int:
+    """The current stream's handle (torch.cuda.current_stream builds an object for it: 2 us of a 9 us call)."""
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _in_place(x: torch.Tensor, k: int, device: torch.device) -> bool:
+    """Whether the kernels can read x [..., k] where it is, as a decode loop passes it: no copy, no padding."""
+    return x.dtype in _DTYPE_CODE and x.shape[-1] == k and k % 16 == 0 and x.device == device and x.is_contiguous() \
+        and x.data_ptr() % 16 == 0
 
 
 class Int4Linear(nn.Module):
@@ -503,59 +503,47 @@ class Int4Linear(nn.Module):
         """Low-level device call: x2 [m, k'] (k' = in_features rounded up to 16, 16-byte aligned rows)
         into ``out`` [m, out_features] (fp32, fp16 or bf16, unit column stride, any row stride)."""
         m, n = x2.shape[0], self.out_features
-        if out.shape != (m, n) or (out.stride(1) != 1 and n > 1) or out.dtype not in _Y_CODE:
+        if out.shape != (m, n) or (out.stride(1) != 1 and n > 1) or out.dtype not in _DTYPE_CODE:
             raise ValueError("output must be an fp32/fp16/bf16 [%d, %d] view with unit column stride" % (m, n))
         k16 = (self.in_features + 15) // 16 * 16
         if x2.shape[1] != k16 or x2.stride(1) != 1 or x2.dtype not in _DTYPE_CODE:
             raise ValueError("input must be an fp32/fp16/bf16 [m, %d] view with unit column stride" % k16)
-        b = self._buffers
-        dev = b["packed"].device
+        dev = self._buffers["packed"].device
         if x2.device != dev or out.device != dev:
             raise ValueError("input and output must be on the weight's device %s" % dev)
-        if m > 0:
-            with _current(dev):
-                self._call(x2, k16, m, n, out, b, dev)
+        self._run(x2, m, k16, x2.stride(0) if m > 1 else k16, out, out.stride(0) if m > 1 else n, dev)
         return out
 
-    def _call(self, x2, k, m, n, out, b, dev) -> None:
-        x_code = _DTYPE_CODE[x2.dtype]
-        ws, ws_bytes = _int4_workspace(m, k, x_code, dev)
-        bias = self._parameters.get("bias")
-        L.call("sbq_linear_w4", x2.data_ptr(), x_code, x2.stride(0) if m > 1 else k, b["packed"].data_ptr(),
-               b["scales"].data_ptr(), b["rowmul"].data_ptr(), self.group, None if bias is None else bias.data_ptr(), m, n,
-               k, out.data_ptr(), _Y_CODE[out.dtype], out.stride(0) if m > 1 else n, None if ws is None else ws.data_ptr(), ws_bytes,
-               torch.cuda.current_stream(dev).cuda_stream)
+    def _run(self, x: torch.Tensor, m: int, k: int, ldx: int, out: torch.Tensor, ldy: int, dev: torch.device) -> None:
+        if m == 0:
+            return
+        if dev.index != torch._C._cuda_getDevice():  # the library launches on the current device
+            with torch.cuda.device(dev):
+                return self._run(x, m, k, ldx, out, ldy, dev)
+        b, code, bias = self._buffers, _DTYPE_CODE[x.dtype], self._parameters.get("bias")
+        ws, ws_bytes = _int4_workspace(m, k, code, dev)
+        status = L.load().sbq_linear_w4(
+            x.data_ptr(), code, ldx, b["packed"].data_ptr(), b["scales"].data_ptr(), b["rowmul"].data_ptr(), self.group,
+            None if bias is None else bias.data_ptr(), m, self.out_features, k, out.data_ptr(), _DTYPE_CODE[out.dtype], ldy,
+            None if ws is None else ws.data_ptr(), ws_bytes, _raw_stream(dev))
+        if status:
+            L.check(status, "sbq_linear_w4")
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        dev = self._buffers["packed"].device
-        x2, k16, on_host = _rows16(x, self.in_features, dev)
-        out = torch.empty(x2.shape[0], self.out_features, dtype=self.out_dtype, device=dev)
+        k, n, dev = self.in_features, self.out_features, self._buffers["packed"].device
+        if _in_place(x, k, dev):
+            out = torch.empty((*x.shape[:-1], n), dtype=self.out_dtype, device=dev)
+            self._run(x, x.numel() // k, k, k, out, n, dev)
+            return out
+        x2, k16, on_host = _prepare_x(x, k, dev)
+        out = torch.empty(x2.shape[0], n, dtype=self.out_dtype, device=dev)
         self.forward_into(x2, out)
-        if x.dim() != 2:
-            out = out.view(*x.shape[:-1], self.out_features)
+        out = out.view(*x.shape[:-1], n)
         return out.to("cpu") if on_host else out
 
     def extra_repr(self) -> str:
         return "in_features=%d, out_features=%d, bias=%s, group=%d" % (self.in_features, self.out_features,
                                                                        self.bias is not None, self.group)
-
-
-class _Here:
-    """A context that changes nothing."""
-
-    def __enter__(self):
-        return None
-
-    def __exit__(self, *exc):
-        return None
-
-
-_HERE = _Here()
-
-
-def _current(device: torch.device):
-    """Makes ``device`` the current one for a library call (the library launches on the current device)."""
-    return _HERE if torch.cuda.current_device() == device.index else torch.cuda.device(device)
 
 
 def _int4_workspace(m: int, k: int, x_code: int, device: torch.device):
