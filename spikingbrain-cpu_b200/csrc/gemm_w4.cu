@@ -347,48 +347,60 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
         }
     } else if (warp == 1) {
         if (lane == 0 && leader) {
+            // One thread issues everything, so its instructions per block are kept few: a descriptor is the first
+            // stage's plus a multiple of 16 bytes, ring positions are counted along.
             constexpr uint32_t idesc = tc::idesc_f16(2 * kW4Rows, TOK, false);
-            int g = 0, seg = -1;
+            const uint64_t desc0 = tc::smem_desc(smem, tc::kSwizzle128B, 1024);
+            const uint32_t bar_done0 = tc::cluster_addr(mma_done, 0), bar_done1 = tc::cluster_addr(mma_done, 1);
+            const uint32_t bar_seg0 = tc::cluster_addr(done, 0), bar_seg1 = tc::cluster_addr(done, 1);
+            int s = 0, ab = 0, seg = 0;  // stage, operand buffer, segment
+            uint32_t ph = 0;
             bool ok = true;
-            for (int tile = pair; tile < tiles && ok; tile += npairs)
-                for (int kb = 0; kb < kt; ++kb, ++g) {
-                    const int s = g % NS;
-                    const bool fresh = SEG ? kb % S::kSegBlocks == 0 : kb == 0;
-                    if (fresh && ++seg >= ND && !tc::mbar_wait_cluster(&taken[seg % ND], ((seg / ND) - 1) & 1)) {
-                        ok = false;
-                        break;
+            for (int tile = pair; tile < tiles && ok; tile += npairs) {
+                int left = 0;  // blocks left in the segment
+                for (int kb = 0; kb < kt; ++kb) {
+                    const bool fresh = left == 0;
+                    if (fresh) {
+                        left = SEG && S::kSegBlocks < kt - kb ? S::kSegBlocks : kt - kb;
+                        if (seg >= ND && !tc::mbar_wait(&taken[seg % ND], ((seg / ND) - 1) & 1)) {
+                            ok = false;
+                            break;
+                        }
                     }
-                    if (!tc::mbar_wait_cluster(&ready[s], (g / NS) & 1)) {
+                    if (!tc::mbar_wait(&ready[s], ph)) {
                         ok = false;
                         break;
                     }
                     tc::fence_after_sync();
-                    const uint8_t* xs = smem + s * S::kStage;
+                    const uint64_t xd = desc0 + (uint64_t)(s * (S::kStage / 16));
 #pragma unroll
                     for (int a = 0; a < NMAT; ++a) {
                         const uint32_t d = tmem + ((seg % ND) * NMAT + a) * TOK;
-                        const uint32_t op = tmem + S::kACol + ((g % NA) * NMAT + a) * 64;
+                        const uint32_t op = tmem + S::kACol + (ab * NMAT + a) * 64;
 #pragma unroll
                         for (int j = 0; j < 8; ++j)
 #pragma unroll
-                            for (int q = 0; q < PARTS; ++q) {
-                                const uint64_t bd =
-                                    tc::smem_desc(xs + ((j >> 2) * PARTS + q) * S::kXSub + (j & 3) * 32, tc::kSwizzle128B, 1024);
-                                tc::mma_f16_ts_pair(d, op + j * 8, bd, idesc, !(fresh && j == 0 && q == 0));
-                            }
+                            for (int q = 0; q < PARTS; ++q)
+                                tc::mma_f16_ts_pair(d, op + j * 8, xd + (((j >> 2) * PARTS + q) * S::kXSub + (j & 3) * 32) / 16,
+                                                    idesc, j == 0 && q == 0 ? !fresh : 1u);
                     }
-                    tc::mma_commit_pair(tc::cluster_addr(&mma_done[s], 0));
-                    tc::mma_commit_pair(tc::cluster_addr(&mma_done[s], 1));
-                    if (kb + 1 == kt || (SEG && (kb + 1) % S::kSegBlocks == 0)) {
-                        tc::mma_commit_pair(tc::cluster_addr(&done[seg % ND], 0));
-                        tc::mma_commit_pair(tc::cluster_addr(&done[seg % ND], 1));
+                    tc::mma_commit_pair(bar_done0 + s * 8);
+                    tc::mma_commit_pair(bar_done1 + s * 8);
+                    if (--left == 0) {
+                        tc::mma_commit_pair(bar_seg0 + (seg % ND) * 8);
+                        tc::mma_commit_pair(bar_seg1 + (seg % ND) * 8);
+                        ++seg;
                     }
+                    if (++s == NS) s = 0, ph ^= 1;
+                    if (++ab == NA) ab = 0;
                 }
+            }
         }
     } else if (warp >= 4) {
         const int grp = (warp - 4) >> 2, wq = (warp - 4) & 3, row = wq * 32 + lane;
         const uint32_t lane_tmem = tmem + ((uint32_t)(wq * 32) << 16);
         const int cn = (int)rank * kW4Rows + row;  // this thread's channel within a tile's 256
+        const uint32_t ready0 = tc::cluster_addr(ready, 0);
         auto mul_of = [&](int mat, int tile) {
             const int n = (tile % cols) * (2 * kW4Rows) + cn;
             return tile < tiles && n < p.n ? __ldg(p.rowmul[mat] + n) : 1.0f;
@@ -510,30 +522,33 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
             }
             return true;
         };
-        int g = 0;
         bool ok = true, waited = false;
         const int mat = NMAT == 2 ? grp : 0;
+        // ring positions are counted along (a division by the ring size per block is not free: the converters'
+        // instructions are what limits 128-token tiles): stage s in its phase ph, operand buffer ab, and the
+        // stage sa of the block that used that buffer before, in its phase pa
+        int g = 0, s = 0, ab = 0, sa = 0;
+        uint32_t ph = 0, pa = 0;
         float mul = mul_of(mat, pair);
         for (int tile = pair; tile < tiles && ok; tile += npairs) {
             const float next_mul = mul_of(mat, tile + npairs);
             for (int kb = 0; kb < kt; ++kb, ++g) {
-                const int s = g % NS;
                 if (g >= NA) {
                     // the operand buffer was last read by block g - NA.  Every warp takes every block, and
                     // NA <= NS, so each barrier is at most one phase from the one awaited
-                    const int prev = g - NA;
-                    if (!__all_sync(0xffffffffu, tc::mbar_wait(&mma_done[prev % NS], (prev / NS) & 1))) { ok = false; break; }
-                    if (tk_last <= prev && !waited) {
-                        asm volatile("griddepcontrol.wait;" ::: "memory");  // before y is written, and xinv read
+                    if (!__all_sync(0xffffffffu, tc::mbar_wait(&mma_done[sa], pa))) { ok = false; break; }
+                    if (++sa == NS) sa = 0, pa ^= 1;
+                    if (tk_last <= g - NA) {
+                        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");  // before y is written, and xinv read
                         waited = true;
+                        while (ok && tk_last <= g - NA) ok = take();
+                        if (!ok) break;
                     }
-                    while (ok && tk_last <= prev) ok = take();
-                    if (!ok) break;
                 }
-                if (!__all_sync(0xffffffffu, tc::mbar_wait(&wfull[s], (g / NS) & 1))) { ok = false; break; }
+                if (!__all_sync(0xffffffffu, tc::mbar_wait(&wfull[s], ph))) { ok = false; break; }
                 tc::fence_after_sync();
                 const uint8_t* codes = smem + s * S::kStage + S::kXBytes + mat * kMat;
-                const uint32_t dst = lane_tmem + S::kACol + (g % NA) * NMAT * 64;
+                const uint32_t dst = lane_tmem + S::kACol + ab * (NMAT * 64);
                 if (NMAT == 2)
                     w4_convert_tile<GPT>(codes, codes + S::kCodes, row, mul, dst + mat * 64);
                 else
@@ -542,9 +557,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
                 tc::fence_before_sync();
                 __syncwarp();
                 if (lane == 0) {
-                    tc::mbar_arrive_cluster(tc::cluster_addr(&ready[s], 0));
+                    tc::mbar_arrive_cluster(ready0 + s * 8);
                     tc::mbar_arrive(&conv_done[s]);
                 }
+                if (++s == NS) s = 0, ph ^= 1;
+                if (++ab == NA) ab = 0;
             }
             mul = next_mul;
         }
