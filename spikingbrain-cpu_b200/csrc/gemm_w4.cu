@@ -9,8 +9,8 @@
 // Channels are the MMA's M, tokens its N.  Per 128 columns of k (one packed tile):
 //   * warp 0 (one thread) loads the tokens' x (TMA, 128-byte swizzle), the codes (64 bytes per channel, 64-byte
 //     swizzle, so that 32 rows read 16 bytes each without bank conflicts) and the scales into a ring of stages;
-//   * warps 4-11, two converter warpgroups taking alternate k-blocks, one channel per thread, turn the codes
-//     into scaled fp16 weights and write them to tensor memory (the MMA's A operand, a ring of its own);
+//   * two converter warpgroups, one channel per thread, turn the codes into scaled fp16 weights and write them to
+//     tensor memory (the MMA's A operand, a ring of its own);
 //   * warp 1 (one thread) issues tcgen05.mma, A from tensor memory, x from shared memory.
 //
 // Conversion: a code moved to bits 6..9 under the fp16 exponent of 16 reads as 16 + u, and
@@ -19,10 +19,8 @@
 //
 // Tensor-core accumulation truncates: measured on B200, the relative error of a sum grows by about 1.3e-8 per
 // k16 step (1.2e-5 at k = 12288).  Where the result is kept in fp32 the sum is therefore cut into segments
-// of 32 steps (kSegSteps) that alternate between two accumulators; the converter warps add each finished
-// segment to fp32 registers (round to nearest) while the other one fills.  128-token tiles have room
-// for that (64 sums per thread), 256-token tiles, which read half the weight per product, do not, and
-// serve 16-bit results, whose own rounding (2^-12 and up) is far above it.
+// of kSegSteps steps, and each finished segment is added to fp32 registers (round to nearest).  16-bit results,
+// whose own rounding (2^-12 and up) is far above it, are summed in one piece.
 #include "tc.cuh"
 #include "w4_host.cuh"
 
@@ -30,7 +28,7 @@ namespace sbq {
 
 constexpr int kW4Threads = 384;   // producer, MMA, tensor-memory, idle warp, two converter warpgroups
 constexpr int kW4Rows = 128;      // channels (tensor-memory lanes) per CTA
-constexpr int kSegSteps = 32;     // MMA steps per accumulation segment
+constexpr int kSegSteps = 64;     // MMA steps per accumulation segment (measured error: 8e-7)
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
     asm volatile(
@@ -42,6 +40,7 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
 
 struct GemmW4Params {
     int m, n, kt, parts;
+    int seg_blocks;  // blocks of 128 k per accumulation segment
     const float* rowmul[2];
     const float* bias;
     const float* xinv;
@@ -50,21 +49,22 @@ struct GemmW4Params {
     int y_dtype;
 };
 
-// Sizes of one kernel.  XROWS: tokens of x this CTA loads per block of 128 k; N: the MMA's tokens; CODES: code
-// matrices per block; ND: accumulators per matrix.
-template <int XROWS, int N, int PARTS, int CODES, int ND, int TMEM, int RING>
+// Sizes of one kernel.  XROWS: tokens of x this CTA loads per block of 128 k; N: the MMA's tokens; ND:
+// accumulators; XCH: bytes for the gate / up exchange.
+template <int XROWS, int N, int PARTS, int ND, int TMEM, int RING, int XCH>
 struct W4Shape {
     static constexpr int kXSub = XROWS * 128;               // 64 columns of k: a 128-byte row per token
     static constexpr int kXBytes = 2 * PARTS * kXSub;       // [64-column half][part]
-    static constexpr int kCodes = kW4Rows * 64;             // one matrix
-    static constexpr int kScales = 1024;                    // one matrix (at most)
-    static constexpr int kStage = kXBytes + CODES * (kCodes + kScales);
-    static constexpr int kStages = RING / kStage < 8 ? RING / kStage : 8;
-    static constexpr int kACol = CODES * ND * N;            // accumulators first
-    static constexpr int kABufs0 = (TMEM - kACol) / (64 * CODES);
-    static constexpr int kABufs = kABufs0 < kStages ? kABufs0 : kStages;  // 64 columns per 128 k and matrix
+    static constexpr int kCodes = kW4Rows * 64;
+    static constexpr int kStage = kXBytes + kCodes + 1024;  // scales: at most 1 KiB
+    static constexpr int kStages = (RING - XCH) / kStage < 8 ? (RING - XCH) / kStage : 8;
+    static constexpr int kACol = ND * N;                    // accumulators first
+    static constexpr int kABufs0 = (TMEM - kACol) / 64;
+    static constexpr int kABufs1 = kABufs0 < 4 ? kABufs0 : 4;
+    static constexpr int kABufs = kABufs1 < kStages ? kABufs1 : kStages;  // 64 columns per 128 k
     static constexpr int kSegBlocks = kSegSteps / (8 * PARTS);
-    static constexpr int kBarOff = kStages * kStage;
+    static constexpr int kXchOff = kStages * kStage;
+    static constexpr int kBarOff = kXchOff + XCH;
     static constexpr int kBytes = kBarOff + 512 + kW4Rows * 8 + 1024;
     static_assert(kStages >= 2 && kABufs >= 2, "pipeline depth");
     static_assert((4 * kStages + 4) * 8 + 4 <= 512, "barriers");
@@ -94,21 +94,41 @@ __device__ __forceinline__ void w4_convert_word(uint32_t v, uint32_t s, uint32_t
     o[3] = hfma2(lop3_and_or(v >> 6, 0x03C003C0u, 0x4C004C00u), s, c);
 }
 
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        : "memory");
+}
+
+// 32 lanes x 16 tensor-memory columns: thread t of the warp gets lane (base lane + t).
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr));
+}
+
 // Columns 64 half .. 64 half + 63 of channel `row` of one tile (64 bytes of codes, 64-byte swizzle) -> 32
 // tensor-memory columns.
 template <int GPT>
 __device__ __forceinline__ void w4_convert_half(const uint8_t* codes, const uint8_t* scales, int row, float rowmul, int half,
                                                 uint32_t tmem_dst) {
     constexpr int NG = GPT == 4 ? 2 : 1;  // groups in 64 columns
-    uint32_t s2[NG], c2[NG], h[32];
+    uint32_t s2[NG], c2[NG], h[16];
     w4_scales<GPT>(scales, row, rowmul, half * GPT / 2, s2, c2, NG);
+    uint2 v[4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-        const uint2 v = *reinterpret_cast<const uint2*>(codes + row * 64 + ((t ^ ((row >> 1) & 3)) << 4) + half * 8);
-        w4_convert_word(v.x, s2[0], c2[0], h + 4 * t);
-        w4_convert_word(v.y, s2[NG - 1], c2[NG - 1], h + 16 + 4 * t);
-    }
-    tc::tmem_st_32x32b_x32(tmem_dst, h);
+    for (int t = 0; t < 4; ++t)
+        v[t] = *reinterpret_cast<const uint2*>(codes + row * 64 + ((t ^ ((row >> 1) & 3)) << 4) + half * 8);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) w4_convert_word(v[t].x, s2[0], c2[0], h + 4 * t);
+    tmem_st_x16(tmem_dst, h);
+#pragma unroll
+    for (int t = 0; t < 4; ++t) w4_convert_word(v[t].y, s2[NG - 1], c2[NG - 1], h + 4 * t);
+    tmem_st_x16(tmem_dst + 16, h);
 }
 
 // All 128 columns of channel `row` -> 64 tensor-memory columns.
@@ -183,21 +203,31 @@ __device__ __forceinline__ void w4_finish(const GemmW4Params& p, const float (&v
 }
 
 // ---------------------------------------------------------------------------------------------
-// More than 128 rows: CTA pairs (cta_group::2), persistent.  A pair computes tiles of 256 channels x TOK tokens (with
-// two matrices: of both) one after the other; blocks of 128 k run through the rings without a break between
-// tiles.  Each CTA converts its own 128 channels and loads half of the tokens; both converter warpgroups work
-// on every block, on one half of its columns each (two matrices: on one matrix each).
+// More than 128 rows: CTA pairs (cta_group::2), persistent.  A pair computes tiles of 256 channels x TOK tokens one
+// after the other; blocks of 128 k run through the rings without a break between tiles.  Each CTA converts its
+// own 128 channels and loads half of the tokens.  With two matrices a CTA's lanes 0..63 are gate channels and
+// lanes 64..127 the same channels of the up projection (128 channels per pair).
 //
-// Results are taken out of tensor memory NA blocks behind the conversion, when their MMAs are known to be
-// done: the operand buffers of the next tile are then full, so the tensor cores wait only for the accumulator
-// to be read, and the stores run under the next tile's MMAs.  Without segments (16-bit results) there is one
-// accumulator of TOK * NMAT = 256 columns; with segments two of 128.
+// Roles: warp 0 producer, warp 1 MMA (leader), warp 2 tensor memory; warps 4-11 converters, each on one half of the
+// columns of every block; warps 12-19 takers: they read a finished segment (tile) out of the accumulator, let the
+// MMAs go on, and scale and store a finished tile under the next one's MMAs.  Registers are dealt to the roles
+// by setmaxnreg: a taker holds up to 128 fp32 sums.
+//
+// TOK = 256 (the accumulator and four operand buffers fill tensor memory).  An MMA of 128 tokens whose A operand
+// comes from tensor memory takes about 100 cycles, not half of the 256-token one's 128-150, so 128-token tiles
+// serve only products that have too few 256-token tiles for the GPU.
 // ---------------------------------------------------------------------------------------------
-template <int PARTS, int NMAT, bool SEG>
-struct W4PairShape {
-    static constexpr int TOK = (SEG ? 128 : 256) / NMAT;
-    using S = W4Shape<TOK / 2, TOK, PARTS, NMAT, SEG ? 2 : 1, 512, 224 * 1024>;
-};
+constexpr int kPairThreads = 640;
+constexpr int kRegsIssue = 40, kRegsConvert = 56, kRegsTake = 160;
+static_assert(kRegsIssue + 2 * kRegsConvert + 2 * kRegsTake <= 5 * 96, "the launch's registers: 96 x 640 threads");
+
+template <int N>
+__device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N>
+__device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
+
+template <int PARTS, int NMAT, int TOK>
+using W4Pair = W4Shape<TOK / 2, TOK, PARTS, 1, 512, 224 * 1024, NMAT == 2 ? 32 * 1024 : 0>;
 
 template <class T>
 __device__ __forceinline__ T w4_round(float v);
@@ -233,42 +263,41 @@ __device__ __forceinline__ void w4_put(const GemmW4Params& p, int t0, int n, F v
         w4_put_as<__nv_bfloat16, CNT>(p, t0, n, value);
 }
 
-// 32 tokens' factors (the array is padded to a multiple of 64 values).
+// CNT tokens' factors (the array is padded to a multiple of 256 values).
+template <int CNT>
 __device__ __forceinline__ void w4_times_xinv(const float* xinv, int t0, float* v) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
+    for (int j = 0; j < CNT / 4; ++j) {
         const float4 f = __ldg(reinterpret_cast<const float4*>(xinv + t0) + j);
         v[4 * j] *= f.x, v[4 * j + 1] *= f.y, v[4 * j + 2] *= f.z, v[4 * j + 3] *= f.w;
     }
 }
 
-template <int PARTS, int NMAT, bool SEG, int GPT>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
+template <int PARTS, int NMAT, int TOK, int GPT>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     gemm_w4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_lo,
                         const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2,
                         const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_s2,
                         const __grid_constant__ GemmW4Params p) {
-    using Shape = W4PairShape<PARTS, NMAT, SEG>;
-    using S = typename Shape::S;
-    constexpr int TOK = Shape::TOK, COLS = TOK / 2;  // tokens of a tile, tokens per converter warpgroup in the epilogue
-    constexpr int NS = S::kStages, NA = S::kABufs, ND = SEG ? 2 : 1;
-    constexpr int kMat = S::kCodes + S::kScales;     // one matrix of a stage
+    using S = W4Pair<PARTS, NMAT, TOK>;
+    constexpr int NS = S::kStages, NA = S::kABufs, COLS = TOK / 2;  // COLS: tokens per taker warpgroup
+    constexpr int kCh = kW4Rows / NMAT;                             // channels of this CTA's tile
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* wfull = reinterpret_cast<uint64_t*>(smem + S::kBarOff);  // this CTA's codes and scales landed
     uint64_t* ready = wfull + NS;      // leader: both CTAs' x landed and both CTAs' converters wrote
     uint64_t* conv_done = ready + NS;  // this CTA's converters have read the codes
     uint64_t* mma_done = conv_done + NS;
-    uint64_t* done = mma_done + NS;    // per accumulator: the MMAs of its segment (tile) completed
-    uint64_t* taken = done + 2;        // leader, per accumulator: both CTAs' converters have read it
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 2);
+    uint64_t* done = mma_done + NS;    // a segment's MMAs completed
+    uint64_t* taken = done + 1;        // leader: both CTAs' takers have read the accumulator
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 1);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_ctarank();
     const bool leader = rank == 0;
-    // tiles of this pair: pair, pair + npairs, ... (channels fastest)
-    const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
-    const int cols = (p.n + 2 * kW4Rows - 1) / (2 * kW4Rows), tiles = cols * ((p.m + TOK - 1) / TOK), kt = p.kt;
+    // tiles of this pair: pair, pair + npairs, ... (channels fastest); segments of seg_blocks blocks in each
+    const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1), kt = p.kt, seg_blocks = p.seg_blocks;
+    const int cols = (p.n + 2 * kCh - 1) / (2 * kCh), tiles = cols * ((p.m + TOK - 1) / TOK);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
@@ -277,10 +306,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
             tc::mbar_init(&conv_done[s], 8);
             tc::mbar_init(&mma_done[s], 1);
         }
-        for (int d = 0; d < 2; ++d) {
-            tc::mbar_init(&done[d], 1);
-            tc::mbar_init(&taken[d], 16);
-        }
+        tc::mbar_init(done, 1);
+        tc::mbar_init(taken, 16);
         tc::fence_mbar_init();
         tc::prefetch_tmap(&map_x);
         tc::prefetch_tmap(&map_w);
@@ -295,18 +322,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
     tc::fence_after_sync();
     const uint32_t tmem = *tmem_slot;
 
-    if (warp == 0) {
-        if (lane == 0) {
-            // block g of the pair: its tile and k-block
+    if (warp < 4) {
+        regs_less<kRegsIssue>();
+        if (warp == 0 && lane == 0) {
             auto load_w = [&](int s, int tile, int kb) {
                 uint8_t* ws = smem + s * S::kStage + S::kXBytes;
-                const int nt = (tile % cols) * (2 * kW4Rows / 16) + (int)rank * (kW4Rows / 16);
-                tc::mbar_arrive_expect_tx(&wfull[s], NMAT * (S::kCodes + 256 * GPT));
+                const int nt = (tile % cols) * (2 * kCh / 16) + (int)rank * (kCh / 16);
+                tc::mbar_arrive_expect_tx(&wfull[s], S::kCodes + 256 * GPT);
                 tc::tma_load_4d(ws, &map_w, &wfull[s], 0, 0, kb, nt);
                 tma_load_3d(ws + S::kCodes, &map_s, &wfull[s], 0, kb, nt);
                 if (NMAT == 2) {
-                    tc::tma_load_4d(ws + kMat, &map_w2, &wfull[s], 0, 0, kb, nt);
-                    tma_load_3d(ws + kMat + S::kCodes, &map_s2, &wfull[s], 0, kb, nt);
+                    tc::tma_load_4d(ws + S::kCodes / 2, &map_w2, &wfull[s], 0, 0, kb, nt);
+                    tma_load_3d(ws + S::kCodes + 128 * GPT, &map_s2, &wfull[s], 0, kb, nt);
                 }
             };
             auto load_x = [&](int s, int tile, int kb) {
@@ -321,21 +348,19 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
                 }
             };
             // codes of the first stages before the wait for the previous kernel, x after it
-            int g = 0;
-            for (int tile = pair, kb = 0; tile < tiles && g < NS; ++g) {
-                load_w(g, tile, kb);
+            int pre = 0;
+            for (int tile = pair, kb = 0; tile < tiles && pre < NS; ++pre) {
+                load_w(pre, tile, kb);
                 if (++kb == kt) kb = 0, tile += npairs;
             }
-            const int pre = g;
             asm volatile("griddepcontrol.wait;" ::: "memory");
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            g = 0;
+            int s = 0, g = 0;
+            uint32_t ph = 1;  // of the blocks that used the stages before
             bool ok = true;
             for (int tile = pair; tile < tiles && ok; tile += npairs)
                 for (int kb = 0; kb < kt; ++kb, ++g) {
-                    const int s = g % NS;
                     if (g >= pre) {
-                        const uint32_t ph = ((g / NS) & 1) ^ 1;
                         if (!tc::mbar_wait(&conv_done[s], ph) || !tc::mbar_wait(&mma_done[s], ph)) {
                             ok = false;
                             break;
@@ -343,10 +368,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
                         load_w(s, tile, kb);
                     }
                     load_x(s, tile, kb);
+                    if (++s == NS) s = 0, ph ^= 1;
                 }
-        }
-    } else if (warp == 1) {
-        if (lane == 0 && leader) {
+        } else if (warp == 1 && lane == 0 && leader) {
             // One thread issues everything, so its instructions per block are kept few: a descriptor is the first
             // stage's plus a multiple of 16 bytes, ring positions are counted along.
             constexpr uint32_t idesc = tc::idesc_f16(2 * kW4Rows, TOK, false);
@@ -361,8 +385,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
                 for (int kb = 0; kb < kt; ++kb) {
                     const bool fresh = left == 0;
                     if (fresh) {
-                        left = SEG && S::kSegBlocks < kt - kb ? S::kSegBlocks : kt - kb;
-                        if (seg >= ND && !tc::mbar_wait(&taken[seg % ND], ((seg / ND) - 1) & 1)) {
+                        left = seg_blocks < kt - kb ? seg_blocks : kt - kb;
+                        if (seg > 0 && !tc::mbar_wait(taken, (seg - 1) & 1)) {
                             ok = false;
                             break;
                         }
@@ -373,22 +397,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
                     }
                     tc::fence_after_sync();
                     const uint64_t xd = desc0 + (uint64_t)(s * (S::kStage / 16));
+                    const uint32_t op = tmem + S::kACol + ab * 64;
 #pragma unroll
-                    for (int a = 0; a < NMAT; ++a) {
-                        const uint32_t d = tmem + ((seg % ND) * NMAT + a) * TOK;
-                        const uint32_t op = tmem + S::kACol + (ab * NMAT + a) * 64;
+                    for (int j = 0; j < 8; ++j)
 #pragma unroll
-                        for (int j = 0; j < 8; ++j)
-#pragma unroll
-                            for (int q = 0; q < PARTS; ++q)
-                                tc::mma_f16_ts_pair(d, op + j * 8, xd + (((j >> 2) * PARTS + q) * S::kXSub + (j & 3) * 32) / 16,
-                                                    idesc, j == 0 && q == 0 ? !fresh : 1u);
-                    }
+                        for (int q = 0; q < PARTS; ++q)
+                            tc::mma_f16_ts_pair(tmem, op + j * 8, xd + (((j >> 2) * PARTS + q) * S::kXSub + (j & 3) * 32) / 16,
+                                                idesc, j == 0 && q == 0 ? !fresh : 1u);
                     tc::mma_commit_pair(bar_done0 + s * 8);
                     tc::mma_commit_pair(bar_done1 + s * 8);
                     if (--left == 0) {
-                        tc::mma_commit_pair(bar_seg0 + (seg % ND) * 8);
-                        tc::mma_commit_pair(bar_seg1 + (seg % ND) * 8);
+                        tc::mma_commit_pair(bar_seg0);
+                        tc::mma_commit_pair(bar_seg1);
                         ++seg;
                     }
                     if (++s == NS) s = 0, ph ^= 1;
@@ -396,163 +416,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
                 }
             }
         }
-    } else if (warp >= 4) {
-        const int grp = (warp - 4) >> 2, wq = (warp - 4) & 3, row = wq * 32 + lane;
-        const uint32_t lane_tmem = tmem + ((uint32_t)(wq * 32) << 16);
-        const int cn = (int)rank * kW4Rows + row;  // this thread's channel within a tile's 256
+    } else if (warp < 12) {
+        regs_less<kRegsConvert>();
+        const int half = (warp - 4) >> 2, wq = warp & 3, row = wq * 32 + lane;
+        const uint32_t dst0 = tmem + ((uint32_t)(wq * 32) << 16) + S::kACol + half * 32;
         const uint32_t ready0 = tc::cluster_addr(ready, 0);
-        auto mul_of = [&](int mat, int tile) {
-            const int n = (tile % cols) * (2 * kW4Rows) + cn;
-            return tile < tiles && n < p.n ? __ldg(p.rowmul[mat] + n) : 1.0f;
+        const float* rowmul = p.rowmul[NMAT == 2 ? row >> 6 : 0];
+        const int cn = (int)rank * kCh + (NMAT == 2 ? row & 63 : row);
+        auto mul_of = [&](int tile) {
+            const int n = (tile % cols) * (2 * kCh) + cn;
+            return tile < tiles && n < p.n ? __ldg(rowmul + n) : 1.0f;
         };
-        float sum[SEG ? NMAT * COLS : 1];
-        // the next segment to be taken, the global number of its last block, its tile and that one's last block
-        int seg = 0, tk_tile = pair, tk_end = kt - 1;
-        int tk_last = SEG && S::kSegBlocks < kt ? S::kSegBlocks - 1 : kt - 1;
-        bool tk_first = true;
-        auto take = [&]() -> bool {
-            const int d = seg % ND;
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(&done[d], (seg / ND) & 1))) return false;
-            tc::fence_after_sync();
-            const uint32_t src = lane_tmem + d * NMAT * TOK + grp * COLS;
-            const bool last = tk_last == tk_end;
-            const int n = (tk_tile % cols) * (2 * kW4Rows) + cn, t0 = (tk_tile / cols) * TOK + grp * COLS;
-            auto release = [&]() {
-                tc::fence_before_sync();
-                __syncwarp();
-                if (lane == 0) tc::mbar_arrive_cluster(tc::cluster_addr(&taken[d], 0));
-            };
-            float inv[NMAT], bias = 0.0f;
-            if (last) {
-#pragma unroll
-                for (int a = 0; a < NMAT; ++a) inv[a] = 1.0f / mul_of(a, tk_tile);
-                if (NMAT == 1 && p.bias && n < p.n) bias = __ldg(p.bias + n);
-            }
-            if constexpr (SEG) {
-#pragma unroll
-                for (int a = 0; a < NMAT; ++a)
-#pragma unroll
-                    for (int c = 0; c < COLS / 32; ++c) {
-                        uint32_t r[32];
-                        tc::tmem_ld_32x32b_x32(src + a * TOK + c * 32, r);
-                        tc::tmem_wait_ld();
-#pragma unroll
-                        for (int j = 0; j < 32; ++j) {
-                            const float v = __uint_as_float(r[j]);
-                            float& o = sum[a * COLS + c * 32 + j];
-                            o = tk_first ? v : o + v;
-                        }
-                    }
-                release();
-                if (last) {
-#pragma unroll
-                    for (int c = 0; c < COLS / 32; ++c) {
-#pragma unroll
-                        for (int a = 0; a < NMAT; ++a) {
-                            float* v = sum + a * COLS + c * 32;
-#pragma unroll
-                            for (int j = 0; j < 32; ++j) v[j] *= inv[a];
-                            if (p.xinv) w4_times_xinv(p.xinv, t0 + c * 32, v);
-                        }
-                        w4_put<32>(p, t0 + c * 32, n, [&](int j) {
-                            const float v = sum[c * 32 + j];
-                            return NMAT == 2 ? w4_silu(v) * sum[(NMAT - 1) * COLS + c * 32 + j] : v + bias;
-                        });
-                    }
-                }
-            } else if constexpr (NMAT == 1) {
-                // 128 tokens, rounded here: half the registers until they are stored
-                uint32_t h[COLS / 2];
-                const bool f16 = p.y_dtype == SBQ_F16;
-#pragma unroll
-                for (int c = 0; c < COLS / 32; ++c) {
-                    uint32_t r[32];
-                    tc::tmem_ld_32x32b_x32(src + c * 32, r);
-                    tc::tmem_wait_ld();
-                    float v[32];
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]) * inv[0];
-                    if (p.xinv) w4_times_xinv(p.xinv, t0 + c * 32, v);
-#pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const __half2 a = __floats2half2_rn(v[2 * j] + bias, v[2 * j + 1] + bias);
-                        const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * j] + bias, v[2 * j + 1] + bias);
-                        h[c * 16 + j] = f16 ? *reinterpret_cast<const uint32_t*>(&a) : *reinterpret_cast<const uint32_t*>(&b);
-                    }
-                }
-                release();
-                if (n < p.n) {
-                    uint16_t* y = static_cast<uint16_t*>(p.y) + (int64_t)t0 * p.ldy + n;
-#pragma unroll
-                    for (int j = 0; j < COLS; ++j, y += p.ldy)
-                        if (t0 + j < p.m) *y = (uint16_t)(j & 1 ? h[j >> 1] >> 16 : h[j >> 1] & 0xFFFFu);
-                }
-            } else {
-                float gv[COLS], uv[COLS];
-#pragma unroll
-                for (int c = 0; c < COLS / 32; ++c) {
-                    tc::tmem_ld_32x32b_x32(src + c * 32, *reinterpret_cast<uint32_t(*)[32]>(gv + c * 32));
-                    tc::tmem_ld_32x32b_x32(src + TOK + c * 32, *reinterpret_cast<uint32_t(*)[32]>(uv + c * 32));
-                }
-                tc::tmem_wait_ld();
-                release();
-#pragma unroll
-                for (int c = 0; c < COLS / 32; ++c) {
-#pragma unroll
-                    for (int j = 0; j < 32; ++j) gv[c * 32 + j] *= inv[0], uv[c * 32 + j] *= inv[NMAT - 1];
-                    if (p.xinv) {
-                        w4_times_xinv(p.xinv, t0 + c * 32, gv + c * 32);
-                        w4_times_xinv(p.xinv, t0 + c * 32, uv + c * 32);
-                    }
-                    // a 16-bit result: the approximate exponential and division (a few 2^-22) are far below its rounding
-                    w4_put<32>(p, t0 + c * 32, n, [&](int j) {
-                        const float v = gv[c * 32 + j];
-                        return __fdividef(v, 1.0f + __expf(-v)) * uv[c * 32 + j];
-                    });
-                }
-            }
-            ++seg;
-            tk_first = last;
-            if (last) {
-                tk_tile += npairs;
-                tk_end += kt;
-                tk_last = SEG && S::kSegBlocks < kt ? tk_last + S::kSegBlocks : tk_end;
-            } else {
-                tk_last = tk_last + S::kSegBlocks < tk_end ? tk_last + S::kSegBlocks : tk_end;
-            }
-            return true;
-        };
-        bool ok = true, waited = false;
-        const int mat = NMAT == 2 ? grp : 0;
-        // ring positions are counted along (a division by the ring size per block is not free: the converters'
-        // instructions are what limits 128-token tiles): stage s in its phase ph, operand buffer ab, and the
-        // stage sa of the block that used that buffer before, in its phase pa
+        // ring positions are counted along: stage s in its phase ph, operand buffer ab, and the stage sa of the
+        // block that used that buffer before, in its phase pa
         int g = 0, s = 0, ab = 0, sa = 0;
         uint32_t ph = 0, pa = 0;
-        float mul = mul_of(mat, pair);
+        bool ok = true;
+        float mul = mul_of(pair);
         for (int tile = pair; tile < tiles && ok; tile += npairs) {
-            const float next_mul = mul_of(mat, tile + npairs);
+            const float next_mul = mul_of(tile + npairs);
             for (int kb = 0; kb < kt; ++kb, ++g) {
                 if (g >= NA) {
                     // the operand buffer was last read by block g - NA.  Every warp takes every block, and
                     // NA <= NS, so each barrier is at most one phase from the one awaited
                     if (!__all_sync(0xffffffffu, tc::mbar_wait(&mma_done[sa], pa))) { ok = false; break; }
                     if (++sa == NS) sa = 0, pa ^= 1;
-                    if (tk_last <= g - NA) {
-                        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");  // before y is written, and xinv read
-                        waited = true;
-                        while (ok && tk_last <= g - NA) ok = take();
-                        if (!ok) break;
-                    }
                 }
                 if (!__all_sync(0xffffffffu, tc::mbar_wait(&wfull[s], ph))) { ok = false; break; }
                 tc::fence_after_sync();
-                const uint8_t* codes = smem + s * S::kStage + S::kXBytes + mat * kMat;
-                const uint32_t dst = lane_tmem + S::kACol + ab * (NMAT * 64);
-                if (NMAT == 2)
-                    w4_convert_tile<GPT>(codes, codes + S::kCodes, row, mul, dst + mat * 64);
-                else
-                    w4_convert_half<GPT>(codes, codes + S::kCodes, row, mul, grp, dst + grp * 32);
+                const uint8_t* codes = smem + s * S::kStage + S::kXBytes;
+                w4_convert_half<GPT>(codes, codes + S::kCodes, row, mul, half, dst0 + ab * 64);
                 tc::tmem_wait_st();
                 tc::fence_before_sync();
                 __syncwarp();
@@ -565,8 +458,72 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
             }
             mul = next_mul;
         }
-        if (!waited) asm volatile("griddepcontrol.wait;" ::: "memory");
-        while (ok && tk_tile < tiles) ok = take();
+    } else {
+        regs_more<kRegsTake>();
+        const int grp = (warp - 12) >> 2, wq = warp & 3, row = wq * 32 + lane;
+        const uint32_t src = tmem + ((uint32_t)(wq * 32) << 16) + grp * COLS;
+        const uint32_t taken0 = tc::cluster_addr(taken, 0);
+        const int mat = NMAT == 2 ? row >> 6 : 0, cn = (int)rank * kCh + (NMAT == 2 ? row & 63 : row);
+        float* xch = reinterpret_cast<float*>(smem + S::kXchOff) + grp * 32 * kW4Rows;
+        asm volatile("griddepcontrol.wait;" ::: "memory");  // before y is written, and xinv read
+        uint32_t ph = 0;
+        bool ok = true;  // a warp whose wait ran out stores nothing more, but stays for the group's barriers
+        for (int tile = pair; tile < tiles; tile += npairs) {
+            const int n = (tile % cols) * (2 * kCh) + cn, t0 = (tile / cols) * TOK + grp * COLS;
+            const float inv = 1.0f / (n < p.n ? __ldg(p.rowmul[mat] + n) : 1.0f);
+            const float bias = NMAT == 1 && p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
+            float sum[COLS];
+            for (int kb = 0; kb < kt; kb += seg_blocks) {
+                ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(done, ph));
+                if (!ok) break;
+                ph ^= 1;
+                tc::fence_after_sync();
+                if (kb == 0) {
+#pragma unroll
+                    for (int c = 0; c < COLS / 16; ++c) tmem_ld_x16(src + c * 16, reinterpret_cast<uint32_t*>(sum) + c * 16);
+                    tc::tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int c = 0; c < COLS / 16; ++c) {
+                        uint32_t r[16];
+                        tmem_ld_x16(src + c * 16, r);
+                        tc::tmem_wait_ld();
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) sum[c * 16 + j] += __uint_as_float(r[j]);
+                    }
+                }
+                tc::fence_before_sync();
+                __syncwarp();
+                if (lane == 0) tc::mbar_arrive_cluster(taken0);
+            }
+            // ---- the tile's sums are here, the MMAs go on
+#pragma unroll
+            for (int j = 0; j < COLS; ++j) sum[j] *= inv;
+            if (p.xinv) w4_times_xinv<COLS>(p.xinv, t0, sum);
+            if (NMAT == 1) {
+                if (ok) w4_put<COLS>(p, t0, n, [&](int j) { return sum[j] + bias; });
+            } else {
+                // gate lanes finish the first half of the tokens, up lanes the second: each hands the other its
+                // values of 32 tokens at a time
+                constexpr int H = COLS / 2;
+                const bool up = mat == 1;
+#pragma unroll
+                for (int r = 0; r < H / 32; ++r) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) xch[j * kW4Rows + row] = up ? sum[r * 32 + j] : sum[H + r * 32 + j];
+                    group_sync(grp);
+                    if (ok)
+                        w4_put<32>(p, t0 + (up ? H : 0) + r * 32, n, [&](int j) {
+                            const float mine = up ? sum[H + r * 32 + j] : sum[r * 32 + j], other = xch[j * kW4Rows + (row ^ 64)];
+                            const float gv = up ? other : mine, uv = up ? mine : other;
+                            // a 16-bit result: the approximate exponential and division (a few 2^-22) are far below
+                            // its rounding
+                            return p.y_dtype == SBQ_F32 ? w4_silu(gv) * uv : __fdividef(gv, 1.0f + __expf(-gv)) * uv;
+                        });
+                    group_sync(grp);
+                }
+            }
+        }
     }
     tc::fence_before_sync();
     tc::cluster_sync();
@@ -583,7 +540,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kW4Threads, 1)
 // ---------------------------------------------------------------------------------------------
 constexpr int kSTok4 = 64;
 template <int PARTS>
-using W4Small = W4Shape<kSTok4, kSTok4, PARTS, 1, 2, 256, 108 * 1024>;
+using W4Small = W4Shape<kSTok4, kSTok4, PARTS, 2, 256, 108 * 1024, 0>;
 
 template <int PARTS, int NMAT, int GPT>
 __global__ void __launch_bounds__(kW4Threads, 2)
@@ -799,7 +756,7 @@ struct W4Maps {
     CUtensorMap x, lo, w[2], s[2];
 };
 
-// x in boxes of `x_rows` tokens, codes and scales in boxes of `w_rows` channels.
+// x in boxes of `x_rows` tokens, codes and scales in boxes of `w_rows` channels (per matrix).
 static int make_maps(W4Maps& m, const W4Call& c, const W4Acts& x, int x_rows, int w_rows) {
     const uint64_t xd[2] = {(uint64_t)c.k, (uint64_t)c.m}, xs[1] = {(uint64_t)x.ld * 2};
     const uint32_t xb[2] = {64, (uint32_t)x_rows};
@@ -821,12 +778,12 @@ static int make_maps(W4Maps& m, const W4Call& c, const W4Acts& x, int x_rows, in
 }
 
 template <class K>
-static cudaError_t launch_maps(K kernel, dim3 grid, int smem, int parts, cudaStream_t s, const W4Maps& m, const GemmW4Params& p) {
+static cudaError_t launch_maps(K kernel, dim3 grid, int threads, int smem, int parts, cudaStream_t s, const W4Maps& m, const GemmW4Params& p) {
     cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
-    cfg.blockDim = dim3(kW4Threads);
+    cfg.blockDim = dim3((unsigned)threads);
     cfg.dynamicSmemBytes = (size_t)smem;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -841,12 +798,13 @@ static cudaError_t launch_maps(K kernel, dim3 grid, int smem, int parts, cudaStr
     return cudaLaunchKernelEx(&cfg, kernel, m.x, m.lo, m.w[0], m.w[1], m.s[0], m.s[1], p);
 }
 
-template <int PARTS, int NMAT, bool SEG, int GPT>
-static cudaError_t launch_pair_w4(const W4Maps& m, const GemmW4Params& p, cudaStream_t s) {
-    using Shape = W4PairShape<PARTS, NMAT, SEG>;
-    const int64_t tiles = ceil_div(p.n, 2 * kW4Rows) * ceil_div(p.m, Shape::TOK), pairs = w4_sm_count() / 2;
-    return launch_maps(gemm_w4_pair_kernel<PARTS, NMAT, SEG, GPT>, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))),
-                       Shape::S::kBytes, 0, s, m, p);
+template <int PARTS, int NMAT, int TOK, int GPT>
+static cudaError_t launch_pair_w4(const W4Maps& m, GemmW4Params p, cudaStream_t s) {
+    using S = W4Pair<PARTS, NMAT, TOK>;
+    const int64_t tiles = ceil_div(p.n, 2 * kW4Rows / NMAT) * ceil_div(p.m, TOK), pairs = w4_sm_count() / 2;
+    p.seg_blocks = p.y_dtype == SBQ_F32 ? S::kSegBlocks : p.kt;
+    return launch_maps(gemm_w4_pair_kernel<PARTS, NMAT, TOK, GPT>, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))),
+                       kPairThreads, S::kBytes, 0, s, m, p);
 }
 
 template <int PARTS, int NMAT, int GPT>
@@ -854,8 +812,8 @@ static cudaError_t launch_gemm_w4(int tok, const W4Maps& m, const GemmW4Params& 
     if (tok == kSTok4)
         return launch_maps(gemm_w4_small_kernel<PARTS, NMAT, GPT>,
                            dim3((unsigned)ceil_div(p.n, kW4Rows / NMAT), (unsigned)ceil_div(p.m, kSTok4), (unsigned)p.parts),
-                           W4Small<PARTS>::kBytes, p.parts, s, m, p);
-    return tok == 128 ? launch_pair_w4<PARTS, NMAT, true, GPT>(m, p, s) : launch_pair_w4<PARTS, NMAT, false, GPT>(m, p, s);
+                           kW4Threads, W4Small<PARTS>::kBytes, p.parts, s, m, p);
+    return tok == 128 ? launch_pair_w4<PARTS, NMAT, 128, GPT>(m, p, s) : launch_pair_w4<PARTS, NMAT, 256, GPT>(m, p, s);
 }
 
 template <int PARTS, int NMAT>
@@ -889,12 +847,14 @@ int gemm_w4_run(const W4Call& c, const W4Acts& x) {
         const int64_t tiles = ceil_div(c.n, ch) * ceil_div(c.m, kSTok4);
         while (p.parts < 8 && tiles * (2 * p.parts) * 8 <= (int64_t)2 * sms * 7 && p.kt / (2 * p.parts) >= 2) p.parts *= 2;
     } else {
-        // one accumulator per tile for 16-bit results (see the top), unless that leaves pairs without a tile
-        const int64_t cols = ceil_div(c.n, 2 * kW4Rows), wide = cols * ceil_div(c.m, 256 / nmat);
-        tok = c.y_dtype == SBQ_F32 || wide * 10 < (int64_t)(sms / 2) * 9 ? 128 : 256;
+        // tokens per tile by the modelled time: rounds of tiles over the pairs, a 128-token block taking 5/8 of a
+        // 256-token one
+        const int64_t cols = ceil_div(c.n, 2 * ch), pairs = sms / 2;
+        const int64_t wide = ceil_div(cols * ceil_div(c.m, 256), pairs) * 8, narrow = ceil_div(cols * ceil_div(c.m, 128), pairs) * 5;
+        tok = narrow < wide ? 128 : 256;
     }
     W4Maps maps;
-    const int st = tok == kSTok4 ? make_maps(maps, c, x, kSTok4, ch) : make_maps(maps, c, x, tok / nmat / 2, kW4Rows);
+    const int st = make_maps(maps, c, x, tok == kSTok4 ? kSTok4 : tok / 2, ch);
     if (st) return st;
     const cudaError_t e = x.part[1] ? (nmat == 2 ? launch_gemm_w4_g<2, 2>(c.gpt, tok, maps, p, c.stream)
                                                  : launch_gemm_w4_g<2, 1>(c.gpt, tok, maps, p, c.stream))
