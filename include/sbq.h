@@ -388,9 +388,10 @@ SBQ_API int sbq_w4_pack(const int8_t* q, int64_t ldq, const void* scale, int64_t
 SBQ_API int sbq_w4_unpack(const void* packed, const void* scales, int64_t n, int64_t k, int group, int8_t* q,
                           int64_t ldq, void* scale, int64_t lds, void* stream);
 
-/* Workspace of sbq_linear_w4 / sbq_mlp_gateup_w4 for x [m, k]: the activation's fp16 parts (fp32 x at
- * every m, bf16 x above 16 rows), 0 otherwise. */
-SBQ_API size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t k, int x_dtype);
+/* Workspace of sbq_linear_w4 (matrices = 1) / sbq_mlp_gateup_w4 (2) on the current device: the activation's
+ * fp16 parts (fp32 x at every m, bf16 x above 16 rows) and, above 128 rows, the partial sums of tiles that are
+ * cut along k.  Its contents need not be kept between calls. */
+SBQ_API size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_dtype, int matrices);
 
 /* y[m, n] = sum_k x[m, k] * q[n, k] * s[n, k / group] (+ bias[n]); x and y SBQ_F32, SBQ_F16 or SBQ_BF16.
  * q * s enters the product exactly, bf16 x too, fp32 x with 22 bits; sums are fp32.  Up to 16 rows: the

@@ -41,6 +41,9 @@ __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, u
 struct GemmW4Params {
     int m, n, kt, parts;
     int seg_blocks;  // blocks of 128 k per accumulation segment
+    // pair kernel: rounds of whole tiles, then tail_tiles tiles cut into tail_parts parts along k
+    int rounds, tail_tiles, tail_parts;
+    float* partial;  // [tail tile][part][token][lane of both CTAs]: sums of a cut tile's parts, or null
     const float* rowmul[2];
     const float* bias;
     const float* xinv;
@@ -213,9 +216,12 @@ __device__ __forceinline__ void w4_finish(const GemmW4Params& p, const float (&v
 // MMAs go on, and scale and store a finished tile under the next one's MMAs.  Registers are dealt to the roles
 // by setmaxnreg: a taker holds up to 128 fp32 sums.
 //
-// TOK = 256 (the accumulator and four operand buffers fill tensor memory).  An MMA of 128 tokens whose A operand
-// comes from tensor memory takes about 100 cycles, not half of the 256-token one's 128-150, so 128-token tiles
-// serve only products that have too few 256-token tiles for the GPU.
+// Tiles are 256 tokens wide (the accumulator and four operand buffers fill tensor memory): an MMA of 128 tokens
+// whose A operand comes from tensor memory takes about 100 cycles, not half of the 256-token one's 128-150.  The
+// last token tile's MMAs are as wide as its tokens.
+//
+// The tiles of the last, incomplete round are cut along k so that every pair has a part; a cut tile's parts go to
+// `partial` as fp32 sums and w4_reduce_kernel adds them in order.
 // ---------------------------------------------------------------------------------------------
 constexpr int kPairThreads = 640;
 constexpr int kRegsIssue = 40, kRegsConvert = 56, kRegsTake = 160;
@@ -226,8 +232,37 @@ __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.
 template <int N>
 __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-template <int PARTS, int NMAT, int TOK>
-using W4Pair = W4Shape<TOK / 2, TOK, PARTS, 1, 512, 224 * 1024, NMAT == 2 ? 32 * 1024 : 0>;
+constexpr int kTok = 256;  // tokens of a tile
+template <int PARTS, int NMAT>
+using W4Pair = W4Shape<kTok / 2, kTok, PARTS, 1, 512, 224 * 1024, NMAT == 2 ? 32 * 1024 : 0>;
+
+// One piece of a pair's work: blocks kb0 .. kb1 - 1 of a tile; slot: its place in `partial`, -1 for a whole tile.
+struct W4Item {
+    int tile, kb0, kb1, slot;
+};
+
+__device__ __forceinline__ int w4_items(const GemmW4Params& p, int pair) {
+    return p.rounds + (pair < p.tail_tiles * p.tail_parts ? 1 : 0);
+}
+
+__device__ __forceinline__ W4Item w4_item(const GemmW4Params& p, int pair, int npairs, int i) {
+    W4Item w;
+    if (i < p.rounds) {
+        w.tile = i * npairs + pair, w.kb0 = 0, w.kb1 = p.kt, w.slot = -1;
+    } else {
+        const int P = p.tail_parts, part = pair % P;
+        w.tile = p.rounds * npairs + pair / P;
+        w.kb0 = part * p.kt / P, w.kb1 = (part + 1) * p.kt / P;
+        w.slot = P > 1 ? pair : -1;
+    }
+    return w;
+}
+
+// Tokens of the MMAs of a tile: its rows of x rounded up to 32.
+__device__ __forceinline__ int w4_tile_tokens(int m, int t0) {
+    const int left = (m - t0 + 31) & ~31;
+    return left < kTok ? left : kTok;
+}
 
 template <class T>
 __device__ __forceinline__ T w4_round(float v);
@@ -273,14 +308,14 @@ __device__ __forceinline__ void w4_times_xinv(const float* xinv, int t0, float* 
     }
 }
 
-template <int PARTS, int NMAT, int TOK, int GPT>
+template <int PARTS, int NMAT, int GPT>
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     gemm_w4_pair_kernel(const __grid_constant__ CUtensorMap map_x, const __grid_constant__ CUtensorMap map_lo,
                         const __grid_constant__ CUtensorMap map_w, const __grid_constant__ CUtensorMap map_w2,
                         const __grid_constant__ CUtensorMap map_s, const __grid_constant__ CUtensorMap map_s2,
                         const __grid_constant__ GemmW4Params p) {
-    using S = W4Pair<PARTS, NMAT, TOK>;
-    constexpr int NS = S::kStages, NA = S::kABufs, COLS = TOK / 2;  // COLS: tokens per taker warpgroup
+    using S = W4Pair<PARTS, NMAT>;
+    constexpr int NS = S::kStages, NA = S::kABufs, COLS = kTok / 2;  // COLS: tokens per taker warpgroup
     constexpr int kCh = kW4Rows / NMAT;                             // channels of this CTA's tile
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -295,9 +330,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t rank = tc::cluster_ctarank();
     const bool leader = rank == 0;
-    // tiles of this pair: pair, pair + npairs, ... (channels fastest); segments of seg_blocks blocks in each
-    const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1), kt = p.kt, seg_blocks = p.seg_blocks;
-    const int cols = (p.n + 2 * kCh - 1) / (2 * kCh), tiles = cols * ((p.m + TOK - 1) / TOK);
+    const int pair = (int)(blockIdx.x >> 1), npairs = (int)(gridDim.x >> 1);
+    const int cols = (p.n + 2 * kCh - 1) / (2 * kCh);  // tiles are numbered channels first
+    const int items = w4_items(p, pair);
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < NS; ++s) {
@@ -338,7 +373,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             };
             auto load_x = [&](int s, int tile, int kb) {
                 uint8_t* xs = smem + s * S::kStage;
-                const int tr = (tile / cols) * TOK + (int)rank * (TOK / 2);
+                const int t0 = (tile / cols) * kTok, tr = t0 + (int)rank * (w4_tile_tokens(p.m, t0) / 2);
                 const uint32_t xb = tc::cluster_addr(&ready[s], 0);
                 if (leader) tc::mbar_arrive_expect_tx(&ready[s], 2 * S::kXBytes);
 #pragma unroll
@@ -349,43 +384,46 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             };
             // codes of the first stages before the wait for the previous kernel, x after it
             int pre = 0;
-            for (int tile = pair, kb = 0; tile < tiles && pre < NS; ++pre) {
-                load_w(pre, tile, kb);
-                if (++kb == kt) kb = 0, tile += npairs;
+            for (int i = 0; i < items && pre < NS; ++i) {
+                const W4Item w = w4_item(p, pair, npairs, i);
+                for (int kb = w.kb0; kb < w.kb1 && pre < NS; ++kb) load_w(pre++, w.tile, kb);
             }
             asm volatile("griddepcontrol.wait;" ::: "memory");
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
             int s = 0, g = 0;
             uint32_t ph = 1;  // of the blocks that used the stages before
             bool ok = true;
-            for (int tile = pair; tile < tiles && ok; tile += npairs)
-                for (int kb = 0; kb < kt; ++kb, ++g) {
+            for (int i = 0; i < items && ok; ++i) {
+                const W4Item w = w4_item(p, pair, npairs, i);
+                for (int kb = w.kb0; kb < w.kb1; ++kb, ++g) {
                     if (g >= pre) {
                         if (!tc::mbar_wait(&conv_done[s], ph) || !tc::mbar_wait(&mma_done[s], ph)) {
                             ok = false;
                             break;
                         }
-                        load_w(s, tile, kb);
+                        load_w(s, w.tile, kb);
                     }
-                    load_x(s, tile, kb);
+                    load_x(s, w.tile, kb);
                     if (++s == NS) s = 0, ph ^= 1;
                 }
+            }
         } else if (warp == 1 && lane == 0 && leader) {
             // One thread issues everything, so its instructions per block are kept few: a descriptor is the first
             // stage's plus a multiple of 16 bytes, ring positions are counted along.
-            constexpr uint32_t idesc = tc::idesc_f16(2 * kW4Rows, TOK, false);
             const uint64_t desc0 = tc::smem_desc(smem, tc::kSwizzle128B, 1024);
             const uint32_t bar_done0 = tc::cluster_addr(mma_done, 0), bar_done1 = tc::cluster_addr(mma_done, 1);
             const uint32_t bar_seg0 = tc::cluster_addr(done, 0), bar_seg1 = tc::cluster_addr(done, 1);
             int s = 0, ab = 0, seg = 0;  // stage, operand buffer, segment
             uint32_t ph = 0;
             bool ok = true;
-            for (int tile = pair; tile < tiles && ok; tile += npairs) {
+            for (int i = 0; i < items && ok; ++i) {
+                const W4Item w = w4_item(p, pair, npairs, i);
+                const uint32_t idesc = tc::idesc_f16(2 * kW4Rows, w4_tile_tokens(p.m, (w.tile / cols) * kTok), false);
                 int left = 0;  // blocks left in the segment
-                for (int kb = 0; kb < kt; ++kb) {
+                for (int kb = w.kb0; kb < w.kb1; ++kb) {
                     const bool fresh = left == 0;
                     if (fresh) {
-                        left = seg_blocks < kt - kb ? seg_blocks : kt - kb;
+                        left = p.seg_blocks < w.kb1 - kb ? p.seg_blocks : w.kb1 - kb;
                         if (seg > 0 && !tc::mbar_wait(taken, (seg - 1) & 1)) {
                             ok = false;
                             break;
@@ -423,19 +461,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const uint32_t ready0 = tc::cluster_addr(ready, 0);
         const float* rowmul = p.rowmul[NMAT == 2 ? row >> 6 : 0];
         const int cn = (int)rank * kCh + (NMAT == 2 ? row & 63 : row);
-        auto mul_of = [&](int tile) {
-            const int n = (tile % cols) * (2 * kCh) + cn;
-            return tile < tiles && n < p.n ? __ldg(rowmul + n) : 1.0f;
+        auto mul_of = [&](int i) {
+            const int n = i < items ? (w4_item(p, pair, npairs, i).tile % cols) * (2 * kCh) + cn : p.n;
+            return n < p.n ? __ldg(rowmul + n) : 1.0f;
         };
         // ring positions are counted along: stage s in its phase ph, operand buffer ab, and the stage sa of the
         // block that used that buffer before, in its phase pa
         int g = 0, s = 0, ab = 0, sa = 0;
         uint32_t ph = 0, pa = 0;
         bool ok = true;
-        float mul = mul_of(pair);
-        for (int tile = pair; tile < tiles && ok; tile += npairs) {
-            const float next_mul = mul_of(tile + npairs);
-            for (int kb = 0; kb < kt; ++kb, ++g) {
+        float mul = mul_of(0);
+        for (int i = 0; i < items && ok; ++i) {
+            const W4Item w = w4_item(p, pair, npairs, i);
+            const float next_mul = mul_of(i + 1);
+            for (int kb = w.kb0; kb < w.kb1; ++kb, ++g) {
                 if (g >= NA) {
                     // the operand buffer was last read by block g - NA.  Every warp takes every block, and
                     // NA <= NS, so each barrier is at most one phase from the one awaited
@@ -468,17 +507,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         asm volatile("griddepcontrol.wait;" ::: "memory");  // before y is written, and xinv read
         uint32_t ph = 0;
         bool ok = true;  // a warp whose wait ran out stores nothing more, but stays for the group's barriers
-        for (int tile = pair; tile < tiles; tile += npairs) {
-            const int n = (tile % cols) * (2 * kCh) + cn, t0 = (tile / cols) * TOK + grp * COLS;
+        for (int i = 0; i < items; ++i) {
+            const W4Item w = w4_item(p, pair, npairs, i);
+            const int n = (w.tile % cols) * (2 * kCh) + cn, t0 = (w.tile / cols) * kTok + grp * COLS;
             const float inv = 1.0f / (n < p.n ? __ldg(p.rowmul[mat] + n) : 1.0f);
             const float bias = NMAT == 1 && p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
             float sum[COLS];
-            for (int kb = 0; kb < kt; kb += seg_blocks) {
+            for (int kb = w.kb0; kb < w.kb1; kb += p.seg_blocks) {
                 ok = ok && __all_sync(0xffffffffu, tc::mbar_wait(done, ph));
                 if (!ok) break;
                 ph ^= 1;
                 tc::fence_after_sync();
-                if (kb == 0) {
+                if (kb == w.kb0) {
 #pragma unroll
                     for (int c = 0; c < COLS / 16; ++c) tmem_ld_x16(src + c * 16, reinterpret_cast<uint32_t*>(sum) + c * 16);
                     tc::tmem_wait_ld();
@@ -497,6 +537,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 if (lane == 0) tc::mbar_arrive_cluster(taken0);
             }
             // ---- the tile's sums are here, the MMAs go on
+            if (w.slot >= 0) {
+                float* out = p.partial + ((int64_t)w.slot * kTok + grp * COLS) * (2 * kW4Rows) + (int)rank * kW4Rows + row;
+                if (ok) {
+#pragma unroll
+                    for (int j = 0; j < COLS; ++j)
+                        if (t0 + j < p.m) __stcg(out + j * (2 * kW4Rows), sum[j]);
+                }
+                continue;
+            }
 #pragma unroll
             for (int j = 0; j < COLS; ++j) sum[j] *= inv;
             if (p.xinv) w4_times_xinv<COLS>(p.xinv, t0, sum);
@@ -531,6 +580,47 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         tc::fence_after_sync();
         tc::tmem_dealloc_pair(tmem, 512);
     }
+}
+
+// Cut tiles: one CTA per tile and 4 tokens (two matrices: 8), one thread per lane of the pair (two matrices: 4 of the
+// 8 tokens of a channel's two lanes).  Every thread's loads of a part are independent of each other.
+template <int NMAT>
+__global__ void __launch_bounds__(2 * kW4Rows) w4_reduce_kernel(const GemmW4Params p, int npairs) {
+    constexpr int kCh = kW4Rows / NMAT, kLanes = 2 * kW4Rows, T = 4;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int cols = (p.n + 2 * kCh - 1) / (2 * kCh);
+    const int cut = (int)blockIdx.y, tile = p.rounds * npairs + cut;
+    const int tid = (int)threadIdx.x, ch = NMAT == 2 ? tid & 127 : tid;
+    const int j0 = ((int)blockIdx.x * NMAT + (NMAT == 2 ? tid >> 7 : 0)) * T, t0 = (tile / cols) * kTok + j0;
+    const int lane0 = NMAT == 2 ? (ch >> 6) * kW4Rows + (ch & 63) : ch;
+    const int n = (tile % cols) * (2 * kCh) + ch;
+    if (n >= p.n || t0 >= p.m) return;
+    const int count = p.m - t0 < T ? p.m - t0 : T;
+    const float* base = p.partial + ((int64_t)cut * p.tail_parts * kTok + j0) * kLanes + lane0;
+    float v[NMAT][T];
+#pragma unroll
+    for (int a = 0; a < NMAT; ++a)
+#pragma unroll
+        for (int j = 0; j < T; ++j) v[a][j] = 0.0f;
+#pragma unroll 2
+    for (int q = 0; q < p.tail_parts; ++q, base += (int64_t)kTok * kLanes) {
+#pragma unroll
+        for (int a = 0; a < NMAT; ++a)
+#pragma unroll
+            for (int j = 0; j < T; ++j) v[a][j] += j < count ? __ldcg(base + j * kLanes + a * 64) : 0.0f;
+    }
+    const float bias = NMAT == 1 && p.bias ? __ldg(p.bias + n) : 0.0f;
+#pragma unroll
+    for (int a = 0; a < NMAT; ++a) {
+        const float inv = 1.0f / __ldg(p.rowmul[a] + n);
+#pragma unroll
+        for (int j = 0; j < T; ++j) {
+            v[a][j] *= inv;
+            if (p.xinv && j < count) v[a][j] *= __ldg(p.xinv + t0 + j);
+        }
+    }
+    w4_put<T>(p, t0, n, [&](int j) { return NMAT == 2 ? w4_silu(v[0][j]) * v[NMAT - 1][j] : v[0][j] + bias; });
 }
 
 // ---------------------------------------------------------------------------------------------
@@ -798,32 +888,57 @@ static cudaError_t launch_maps(K kernel, dim3 grid, int threads, int smem, int p
     return cudaLaunchKernelEx(&cfg, kernel, m.x, m.lo, m.w[0], m.w[1], m.s[0], m.s[1], p);
 }
 
-template <int PARTS, int NMAT, int TOK, int GPT>
-static cudaError_t launch_pair_w4(const W4Maps& m, GemmW4Params p, cudaStream_t s) {
-    using S = W4Pair<PARTS, NMAT, TOK>;
-    const int64_t tiles = ceil_div(p.n, 2 * kW4Rows / NMAT) * ceil_div(p.m, TOK), pairs = w4_sm_count() / 2;
-    p.seg_blocks = p.y_dtype == SBQ_F32 ? S::kSegBlocks : p.kt;
-    return launch_maps(gemm_w4_pair_kernel<PARTS, NMAT, TOK, GPT>, dim3((unsigned)(2 * (tiles < pairs ? tiles : pairs))),
-                       kPairThreads, S::kBytes, 0, s, m, p);
-}
-
 template <int PARTS, int NMAT, int GPT>
-static cudaError_t launch_gemm_w4(int tok, const W4Maps& m, const GemmW4Params& p, cudaStream_t s) {
+static cudaError_t launch_gemm_w4(int tok, int npairs, const W4Maps& m, GemmW4Params p, cudaStream_t s) {
     if (tok == kSTok4)
         return launch_maps(gemm_w4_small_kernel<PARTS, NMAT, GPT>,
                            dim3((unsigned)ceil_div(p.n, kW4Rows / NMAT), (unsigned)ceil_div(p.m, kSTok4), (unsigned)p.parts),
                            kW4Threads, W4Small<PARTS>::kBytes, p.parts, s, m, p);
-    return tok == 128 ? launch_pair_w4<PARTS, NMAT, 128, GPT>(m, p, s) : launch_pair_w4<PARTS, NMAT, 256, GPT>(m, p, s);
+    using S = W4Pair<PARTS, NMAT>;
+    p.seg_blocks = p.y_dtype == SBQ_F32 ? S::kSegBlocks : p.kt;
+    return launch_maps(gemm_w4_pair_kernel<PARTS, NMAT, GPT>, dim3(2 * (unsigned)npairs), kPairThreads, S::kBytes, 0, s, m, p);
 }
 
 template <int PARTS, int NMAT>
-static cudaError_t launch_gemm_w4_g(int gpt, int tok, const W4Maps& m, const GemmW4Params& p, cudaStream_t s) {
-    if (gpt == 1) return launch_gemm_w4<PARTS, NMAT, 1>(tok, m, p, s);
-    if (gpt == 2) return launch_gemm_w4<PARTS, NMAT, 2>(tok, m, p, s);
-    return launch_gemm_w4<PARTS, NMAT, 4>(tok, m, p, s);
+static cudaError_t launch_gemm_w4_g(int gpt, int tok, int npairs, const W4Maps& m, const GemmW4Params& p, cudaStream_t s) {
+    if (gpt == 1) return launch_gemm_w4<PARTS, NMAT, 1>(tok, npairs, m, p, s);
+    if (gpt == 2) return launch_gemm_w4<PARTS, NMAT, 2>(tok, npairs, m, p, s);
+    return launch_gemm_w4<PARTS, NMAT, 4>(tok, npairs, m, p, s);
 }
 
 constexpr int64_t kW4SmallRows = 128;
+
+// The pair kernel's schedule: whole rounds of tiles over the pairs, the tiles left over cut into parts along k.
+// Cutting is worth its cost (storing the sums, a second launch, reading them: about 13 us and 50 ns for every part's
+// 256 KiB) by a model of the time: a block of 128 k takes about 0.55 us, with an fp32 activation's two parts 1.1 us.
+// Measured on B200, uncut and cut: fp32 300 x 12288 x 4096 (32 tiles on 74 pairs) 140 and 85 us, fp32 512 x 2560 x 9728
+// (2 tiles left of 76) 67 and 53 us; fp16 512 x 2560 x 9728 31 and 35 us, fp16 2048 x 4096 x 12288 (14 left of
+// 384) 143 and 144 us: those two stay uncut.
+struct W4Plan {
+    int npairs, rounds, tail_tiles, tail_parts;
+};
+
+static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, bool split, int nmat) {
+    const int64_t tiles = ceil_div(n, 2 * kW4Rows / nmat) * ceil_div(m, kTok), pairs = w4_sm_count() / 2, kt = w4_tiles_k(k);
+    W4Plan pl{};
+    pl.rounds = (int)(tiles / pairs);
+    pl.tail_tiles = (int)(tiles % pairs);
+    pl.tail_parts = 1;
+    const double block = split ? 1.1 : 0.55;
+    double best = (double)kt * block;
+    for (int64_t parts = 2; parts <= 16 && pl.tail_tiles > 0 && parts * pl.tail_tiles <= pairs && 2 * parts <= kt; ++parts) {
+        const double t = (double)ceil_div(kt, parts) * block + 13.0 + 0.05 * (double)(parts * pl.tail_tiles);
+        if (t < best) best = t, pl.tail_parts = (int)parts;
+    }
+    pl.npairs = pl.rounds > 0 ? (int)pairs : pl.tail_tiles * pl.tail_parts;
+    return pl;
+}
+
+size_t gemm_w4_workspace(int64_t m, int64_t n, int64_t k, bool split, int nmat) {
+    if (m <= kW4SmallRows) return 0;
+    const W4Plan pl = w4_plan(m, n, k, split, nmat);
+    return pl.tail_parts > 1 ? (size_t)pl.tail_tiles * pl.tail_parts * kTok * 2 * kW4Rows * 4 : 0;
+}
 
 int gemm_w4_run(const W4Call& c, const W4Acts& x) {
     const int nmat = c.w[1].packed ? 2 : 1, ch = kW4Rows / nmat, sms = w4_sm_count();
@@ -839,27 +954,40 @@ int gemm_w4_run(const W4Call& c, const W4Acts& x) {
     p.y = c.y;
     p.ldy = c.ldy;
     p.y_dtype = c.y_dtype;
-    int tok;
-    if (c.m <= kW4SmallRows) {
-        tok = kSTok4;
+    const int tok = c.m <= kW4SmallRows ? kSTok4 : kTok;
+    W4Plan pl{};
+    if (tok == kSTok4) {
         // k parts: the largest power of two up to 8 that keeps the grid within 7/8 of the CTA slots (two per
         // SM; a cluster needs all of its CTAs at once) and gives every part at least two tiles
         const int64_t tiles = ceil_div(c.n, ch) * ceil_div(c.m, kSTok4);
         while (p.parts < 8 && tiles * (2 * p.parts) * 8 <= (int64_t)2 * sms * 7 && p.kt / (2 * p.parts) >= 2) p.parts *= 2;
     } else {
-        // tokens per tile by the modelled time: rounds of tiles over the pairs, a 128-token block taking 5/8 of a
-        // 256-token one
-        const int64_t cols = ceil_div(c.n, 2 * ch), pairs = sms / 2;
-        const int64_t wide = ceil_div(cols * ceil_div(c.m, 256), pairs) * 8, narrow = ceil_div(cols * ceil_div(c.m, 128), pairs) * 5;
-        tok = narrow < wide ? 128 : 256;
+        pl = w4_plan(c.m, c.n, c.k, x.part[1] != nullptr, nmat);
+        p.rounds = pl.rounds;
+        p.tail_tiles = pl.tail_tiles;
+        p.tail_parts = pl.tail_parts;
+        p.partial = static_cast<float*>(x.scratch);
     }
     W4Maps maps;
-    const int st = make_maps(maps, c, x, tok == kSTok4 ? kSTok4 : tok / 2, ch);
+    const int st = tok == kSTok4 ? make_maps(maps, c, x, kSTok4, ch) : make_maps(maps, c, x, kTok / 2, ch);
     if (st) return st;
-    const cudaError_t e = x.part[1] ? (nmat == 2 ? launch_gemm_w4_g<2, 2>(c.gpt, tok, maps, p, c.stream)
-                                                 : launch_gemm_w4_g<2, 1>(c.gpt, tok, maps, p, c.stream))
-                                    : (nmat == 2 ? launch_gemm_w4_g<1, 2>(c.gpt, tok, maps, p, c.stream)
-                                                 : launch_gemm_w4_g<1, 1>(c.gpt, tok, maps, p, c.stream));
+    cudaError_t e = x.part[1] ? (nmat == 2 ? launch_gemm_w4_g<2, 2>(c.gpt, tok, pl.npairs, maps, p, c.stream)
+                                           : launch_gemm_w4_g<2, 1>(c.gpt, tok, pl.npairs, maps, p, c.stream))
+                              : (nmat == 2 ? launch_gemm_w4_g<1, 2>(c.gpt, tok, pl.npairs, maps, p, c.stream)
+                                           : launch_gemm_w4_g<1, 1>(c.gpt, tok, pl.npairs, maps, p, c.stream));
+    if (e == cudaSuccess && p.tail_parts > 1) {
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3((unsigned)(kTok / (4 * nmat)), (unsigned)pl.tail_tiles);
+        cfg.blockDim = dim3(2 * kW4Rows);
+        cfg.stream = c.stream;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[0].val.programmaticStreamSerializationAllowed = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        e = nmat == 2 ? cudaLaunchKernelEx(&cfg, w4_reduce_kernel<2>, p, pl.npairs)
+                      : cudaLaunchKernelEx(&cfg, w4_reduce_kernel<1>, p, pl.npairs);
+    }
     if (e != cudaSuccess) return set_error(SBQ_ERR_CUDA, "gemm_w4 launch: %s", cudaGetErrorString(e));
     return check_launch("gemm_w4");
 }

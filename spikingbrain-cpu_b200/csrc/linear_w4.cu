@@ -107,6 +107,12 @@ static bool w4_needs_parts(int64_t m, int x_dtype) {
     return x_dtype == SBQ_F32 || (x_dtype == SBQ_BF16 && m > kW4GemvRows);
 }
 
+// The activation's parts and factors; the factors are read 32 at a time, up to the largest token tile.
+static size_t act_bytes(int64_t m, int64_t k, int x_dtype) {
+    if (!w4_needs_parts(m, x_dtype)) return 0;
+    return (x_dtype == SBQ_F32 ? 2 : 1) * align256((size_t)m * k * 2) + (size_t)ceil_div(m, 256) * 1024;
+}
+
 static int check_w4_call(const void* x, int x_dtype, int64_t ldx, const W4Call& c, int group, int nmat) {
     if (!x || !c.y) return set_error(SBQ_ERR_INVALID_ARGUMENT, "null pointer");
     for (int i = 0; i < nmat; ++i) {
@@ -141,12 +147,15 @@ static int w4_run(const void* x, int x_dtype, int64_t ldx, const W4Call& c, int 
     a.bf16 = x_dtype == SBQ_BF16;
     a.part[0] = x;
     a.ld = ldx;
-    if (w4_needs_parts(c.m, x_dtype)) {
-        const size_t need = sbq_linear_w4_workspace_bytes(c.m, c.k, x_dtype);
-        if (!workspace) return set_error(SBQ_ERR_INVALID_ARGUMENT, "this activation type needs a workspace of %zu bytes", need);
+    const size_t need = sbq_linear_w4_workspace_bytes(c.m, c.n, c.k, x_dtype, nmat);
+    if (need) {
+        if (!workspace) return set_error(SBQ_ERR_INVALID_ARGUMENT, "this call needs a workspace of %zu bytes", need);
         if (reinterpret_cast<uintptr_t>(workspace) % 256)
             return set_error(SBQ_ERR_ALIGNMENT, "workspace must be 256-byte aligned");
         if (workspace_bytes < need) return set_error(SBQ_ERR_WORKSPACE, "workspace needs %zu bytes", need);
+    }
+    a.scratch = static_cast<uint8_t*>(workspace) + act_bytes(c.m, c.k, x_dtype);
+    if (w4_needs_parts(c.m, x_dtype)) {
         const size_t one = align256((size_t)c.m * c.k * 2);
         uint8_t* ws = static_cast<uint8_t*>(workspace);
         ActParams p{};
@@ -172,10 +181,9 @@ static int w4_run(const void* x, int x_dtype, int64_t ldx, const W4Call& c, int 
 
 using namespace sbq;
 
-extern "C" size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t k, int x_dtype) {
-    if (m <= 0 || k <= 0 || !w4_needs_parts(m, x_dtype)) return 0;
-    // the factors are read 32 at a time: rounded up to the largest token tile
-    return (x_dtype == SBQ_F32 ? 2 : 1) * align256((size_t)m * k * 2) + (size_t)ceil_div(m, 256) * 1024;
+extern "C" size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_dtype, int matrices) {
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
+    return act_bytes(m, k, x_dtype) + (m > kW4GemvRows ? gemm_w4_workspace(m, n, k, x_dtype == SBQ_F32, matrices == 2 ? 2 : 1) : 0);
 }
 
 extern "C" int sbq_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* packed, const void* scales,

@@ -25,10 +25,12 @@ struct W4Acts {
     int64_t ld;
     const float* inv;
     bool bf16;
+    void* scratch;  // gemm_w4_workspace bytes
 };
 
 int gemv_w4_run(const W4Call& c, const W4Acts& x);  // up to 16 rows
 int gemm_w4_run(const W4Call& c, const W4Acts& x);  // fp16 parts only
+size_t gemm_w4_workspace(int64_t m, int64_t n, int64_t k, bool split, int nmat);
 int w4_sm_count();
 
 inline int w4_elem(int dtype) { return dtype == SBQ_F32 ? 4 : 2; }

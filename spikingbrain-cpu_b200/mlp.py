@@ -110,7 +110,7 @@ class FusedGatedMLP(nn.Module):
                 return self._run_int4(x, m, k, ldx, h, ldh, dev)
         gate, code = self.gate_proj, _DTYPE_CODE[x.dtype]
         g, u = gate._buffers, self.up_proj._buffers
-        ws, ws_bytes = _int4_workspace(m, k, code, dev)
+        ws, ws_bytes = _int4_workspace(m, gate.out_features, k, code, 2, dev)
         status = L.load().sbq_mlp_gateup_w4(
             x.data_ptr(), code, ldx, g["packed"].data_ptr(), g["scales"].data_ptr(), g["rowmul"].data_ptr(),
             u["packed"].data_ptr(), u["scales"].data_ptr(), u["rowmul"].data_ptr(), gate.group, m, gate.out_features, k,

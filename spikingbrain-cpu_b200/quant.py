@@ -521,7 +521,7 @@ class Int4Linear(nn.Module):
             with torch.cuda.device(dev):
                 return self._run(x, m, k, ldx, out, ldy, dev)
         b, code, bias = self._buffers, _DTYPE_CODE[x.dtype], self._parameters.get("bias")
-        ws, ws_bytes = _int4_workspace(m, k, code, dev)
+        ws, ws_bytes = _int4_workspace(m, self.out_features, k, code, 1, dev)
         status = L.load().sbq_linear_w4(
             x.data_ptr(), code, ldx, b["packed"].data_ptr(), b["scales"].data_ptr(), b["rowmul"].data_ptr(), self.group,
             None if bias is None else bias.data_ptr(), m, self.out_features, k, out.data_ptr(), _DTYPE_CODE[out.dtype], ldy,
@@ -546,11 +546,11 @@ class Int4Linear(nn.Module):
                                                                        self.bias is not None, self.group)
 
 
-def _int4_workspace(m: int, k: int, x_code: int, device: torch.device):
-    """(tensor or None, bytes) for the activation's fp16 parts, from torch's caching allocator."""
-    if x_code == L.F16:
+def _int4_workspace(m: int, n: int, k: int, x_code: int, matrices: int, device: torch.device):
+    """(tensor or None, bytes) of a 4-bit call's workspace, from torch's caching allocator."""
+    if m <= 16 and x_code != L.F32:
         return None, 0
-    nbytes = int(L.load().sbq_linear_w4_workspace_bytes(m, k, x_code))
+    nbytes = L.load().sbq_linear_w4_workspace_bytes(m, n, k, x_code, matrices)
     return (torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes) if nbytes else (None, 0)
 
 
