@@ -3,12 +3,16 @@
 //   y[m, n] = sum_g s[n, g] * (sum_{k in g} x[m, k] q[n, k]) (+ bias[n])         m <= 16
 //   h[m, n] = silu(gate[m, n]) * up[m, n], gate and up as y with their own weights
 //
-// One warp takes a 16-channel tile row (or every W-th 128-column tile of it): per tile two 16-byte loads
-// of codes per lane, q in fp16 or bf16 (exact integers), m16n8k16 tensor-core products with the rows
-// of x as the n dimension, fp32 partial sums per group that are scaled and added in fp32.  So the
-// weight takes part exactly and every sum is fp32.
-#include <atomic>
-
+// The weight's bytes bound it: half a byte and a share of a scale per weight, read once.  A CTA's warps split the k
+// tiles of a 16-channel tile row (W warps per tile row); a warp walks through its tiles of all of its CTA's tile
+// rows as one stream and keeps DEPTH - 1 of them on the way into shared memory (each lane copies what it will read
+// itself, so no barrier is needed; held in registers the same depth spilled), also across tile rows and, at the
+// start, across the wait for the previous kernel.  Per tile: two 16-byte reads of codes per lane, q in fp16 or bf16 (exact
+// integers), m16n8k16 tensor-core products with the rows of x as the n dimension (columns past m repeat row 0 and
+// are dropped), fp32 partial sums per group that are scaled and added in fp32.  So the weight takes part exactly
+// and every sum is fp32; the order of the additions is fixed.
+//
+// With two streams (gate and up, or two tile rows of one weight) a fragment of x serves two tiles.
 #include "w4.cuh"
 #include "w4_host.cuh"
 
@@ -18,7 +22,7 @@ constexpr int kG4Warps = 8;
 constexpr int kG4Threads = kG4Warps * 32;
 
 struct GemvW4Params {
-    const void* x[2];        // 16-bit activation [m, k]; x[1]: low part of a split fp32 activation
+    const uint8_t* x[2];     // 16-bit activation [m, k]; x[1]: low part of a split fp32 activation
     int64_t ldx;
     const float* xinv;       // per row factor of a split activation, or null
     const uint8_t* w[2];     // codes (gate and up of the fused form)
@@ -31,173 +35,294 @@ struct GemvW4Params {
     int kt_total;            // 128-column tiles
     int tile_rows;
     int wsplit;              // warps per tile row (a power of two up to 8)
+    int units;               // CTA-sized pieces: 8 / wsplit tile rows per stream each
 };
 
-template <int MT>
-struct XFrag4 {
-    uint4 v[MT][4];  // [row block][word]: 8 consecutive columns of row 8 * block + g
+// Copies of `BYTES` (4, 8, 16) from global to shared memory, counted in groups per thread.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global.L2::256B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(dst), "l"(src), "n"(BYTES) : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+__device__ __forceinline__ uint32_t word_of(const uint4& v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
+
+// Shared memory of one instance: [warp][slot][stream]: codes (1 KiB), then every lane's scales.
+template <int NSTR, int GPT>
+struct GemvW4Smem {
+    static constexpr int kDepth = NSTR == 2 ? 4 : 6;
+    static constexpr int kTile = kW4TileBytes + 128 * GPT;
+    static constexpr int kWarp = kDepth * NSTR * kTile;
+    static constexpr int kBytes = kG4Warps * kWarp;
 };
 
-// One word (8 columns x rows g, g + 8): two k16 products per row block.
-template <bool BF16, int MT, int PARTS>
-__device__ __forceinline__ void w4_word_mma(float (&part)[MT][4], uint32_t wa, uint32_t wb, int w,
-                                            const XFrag4<MT> (&xf)[PARTS]) {
-    uint32_t a[4], b[4];
-    if (BF16) {
-        w4_to_bf16(wa, a);
-        w4_to_bf16(wb, b);
-    } else {
-        w4_to_half(wa, a);
-        w4_to_half(wb, b);
-    }
+template <bool BF16, int MT, int PARTS, int NSTR, bool GATED, int GPT>
+__global__ void __launch_bounds__(kG4Threads, MT * PARTS * NSTR == 1 ? 3 : 2) gemv_w4_kernel(const GemvW4Params p) {
+    using SM = GemvW4Smem<NSTR, GPT>;
+    constexpr int DEPTH = SM::kDepth;
+    __shared__ float red[2][kG4Warps][NSTR][MT * 8][17];
+    extern __shared__ __align__(128) uint8_t ring[];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    const int W = p.wsplit, rows_per_unit = kG4Warps / W, KT = p.kt_total, ks = warp % W;
+    const int cnt = (KT - ks + W - 1) / W;  // this warp's tiles of a tile row (W <= KT)
+    const int my_units = (p.units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x, total = my_units * cnt;
+
+    // ---- the stream of tiles: (unit, k tile) of the next copy, and its slot
+    int pu = blockIdx.x, pk = ks, pslot = 0;
+    const uint8_t* wp[NSTR];
+    const uint32_t* sp[NSTR];
+    uint8_t* const mine = ring + warp * SM::kWarp + lane * 16;           // this lane's codes of slot 0
+    uint8_t* const mine_s = ring + warp * SM::kWarp + kW4TileBytes + lane * 4 * GPT;  // and scales
+    auto seek = [&]() {
 #pragma unroll
-    for (int p = 0; p < PARTS; ++p)
+        for (int a = 0; a < NSTR; ++a) {
+            int tr = (pu * rows_per_unit + warp / W) * (GATED ? 1 : NSTR) + (GATED ? 0 : a);
+            tr = tr < p.tile_rows ? tr : p.tile_rows - 1;  // past the last tile row: its results are dropped
+            const int64_t tile = (int64_t)tr * KT + ks;
+            wp[a] = p.w[GATED ? a : 0] + tile * kW4TileBytes + lane * 16;
+            sp[a] = p.s[GATED ? a : 0] + (tile * 8 + g) * GPT;
+        }
+    };
+    auto issue = [&]() {
+        if (pu < p.units) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const uint4 v = xf[p].v[mt][w];
-            if (BF16) {
-                mma_bf16(part[mt], a[0], b[0], a[1], b[1], v.x, v.y);
-                mma_bf16(part[mt], a[2], b[2], a[3], b[3], v.z, v.w);
-            } else {
-                mma_f16(part[mt], a[0], b[0], a[1], b[1], v.x, v.y);
-                mma_f16(part[mt], a[2], b[2], a[3], b[3], v.z, v.w);
+            for (int a = 0; a < NSTR; ++a) {
+                const int off = (pslot * NSTR + a) * SM::kTile;
+                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(mine + off);
+                copy_async<16>(dst, wp[a]);
+                copy_async<16>(dst + 512, wp[a] + 512);
+                copy_async<4 * GPT>((uint32_t)__cvta_generic_to_shared(mine_s + off), sp[a]);
+                wp[a] += (int64_t)W * kW4TileBytes;
+                sp[a] += W * 8 * GPT;
+            }
+            pk += W;
+            if (pk >= KT) {
+                pk = ks;
+                pu += gridDim.x;
+                if (pu < p.units) seek();
             }
         }
-}
-
-template <bool BF16, int MT, int PARTS, int NMAT, int GPT>
-__global__ void __launch_bounds__(kG4Threads) gemv_w4_kernel(const GemvW4Params p) {
-    __shared__ float red[kG4Warps][NMAT][MT * 8][17];
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-    const int W = p.wsplit, rows_per_cta = kG4Warps / W;
-    const int tr = blockIdx.x * rows_per_cta + warp / W, ks = warp % W;
-    asm volatile("griddepcontrol.wait;" ::: "memory");
+        if (++pslot == DEPTH) pslot = 0;
+        copy_commit();
+    };
+    seek();
+#pragma unroll
+    for (int d = 0; d < DEPTH - 1; ++d) issue();
+    asm volatile("griddepcontrol.wait;" ::: "memory");  // x, and y
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    float acc[NMAT][MT][4];
+
+    const uint8_t* xp[PARTS][MT];
 #pragma unroll
-    for (int a = 0; a < NMAT; ++a)
+    for (int q = 0; q < PARTS; ++q)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+        for (int mt = 0; mt < MT; ++mt) {
+            const int row = 8 * mt + g < p.m ? 8 * mt + g : 0;
+            xp[q][mt] = p.x[q] + ((int64_t)row * p.ldx + 8 * t) * 2;
+        }
+    float acc[NSTR][MT][4];
+    auto clear = [&]() {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) acc[a][mt][e] = 0.0f;
-    if (tr < p.tile_rows) {
-        for (int kt = ks; kt < p.kt_total; kt += W) {
-            const int64_t tile = (int64_t)tr * p.kt_total + kt;
-            XFrag4<MT> xf[PARTS];
+        for (int a = 0; a < NSTR; ++a)
 #pragma unroll
-            for (int q = 0; q < PARTS; ++q)
+            for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) acc[a][mt][e] = 0.0f;
+    };
+    clear();
+
+    auto consume = [&](const uint4 (&ca)[NSTR], const uint4 (&cb)[NSTR], const uint32_t (&sc)[NSTR][GPT], int kt) {
+        const bool whole = (kt + 1) * kW4TileCols <= p.k;
+#pragma unroll
+        for (int gi = 0; gi < GPT; ++gi) {
+            float part[NSTR][MT][4];
+#pragma unroll
+            for (int a = 0; a < NSTR; ++a)
 #pragma unroll
                 for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        const int row = 8 * mt + g, c = kt * kW4TileCols + 32 * w + 8 * t;
-                        xf[q].v[mt][w] = make_uint4(0, 0, 0, 0);
-                        if (row < p.m && c < p.k)
-                            xf[q].v[mt][w] = *reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(p.x[q]) +
-                                                                             ((int64_t)row * p.ldx + c) * 2);
-                    }
+                    for (int e = 0; e < 4; ++e) part[a][mt][e] = 0.0f;
 #pragma unroll
-            for (int a = 0; a < NMAT; ++a) {
-                const uint8_t* src = p.w[a] + tile * kW4TileBytes + lane * 16;
-                const uint4 wa = ld_stream(src), wb = ld_stream(src + 512);
-                const uint32_t wa_[4] = {wa.x, wa.y, wa.z, wa.w}, wb_[4] = {wb.x, wb.y, wb.z, wb.w};
+            for (int w = gi * (4 / GPT); w < (gi + 1) * (4 / GPT); ++w) {
+                uint4 xv[PARTS][MT];
+                const int c = kt * kW4TileCols + 32 * w;
 #pragma unroll
-                for (int gi = 0; gi < GPT; ++gi) {
-                    float part[MT][4];
-#pragma unroll
-                    for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) part[mt][e] = 0.0f;
-#pragma unroll
-                    for (int w = gi * (4 / GPT); w < (gi + 1) * (4 / GPT); ++w)
-                        w4_word_mma<BF16, MT, PARTS>(part, wa_[w], wb_[w], w, xf);
-                    const uint32_t sc = __ldg(p.s[a] + (tile * 8 + g) * GPT + gi);
-                    const float s0 = __uint_as_float(sc << 16), s1 = __uint_as_float(sc & 0xFFFF0000u);
+                for (int q = 0; q < PARTS; ++q)
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        acc[a][mt][0] = fmaf(s0, part[mt][0], acc[a][mt][0]);
-                        acc[a][mt][1] = fmaf(s0, part[mt][1], acc[a][mt][1]);
-                        acc[a][mt][2] = fmaf(s1, part[mt][2], acc[a][mt][2]);
-                        acc[a][mt][3] = fmaf(s1, part[mt][3], acc[a][mt][3]);
+                        // x past k must read as zero (0 * inf is not), and not be touched
+                        xv[q][mt] = make_uint4(0, 0, 0, 0);
+                        if (whole || c + 8 * t < p.k) xv[q][mt] = *reinterpret_cast<const uint4*>(xp[q][mt] + (int64_t)c * 2);
                     }
+#pragma unroll
+                for (int a = 0; a < NSTR; ++a) {
+                    uint32_t h0[4], h1[4];
+                    if (BF16) {
+                        w4_to_bf16(word_of(ca[a], w), h0);
+                        w4_to_bf16(word_of(cb[a], w), h1);
+                    } else {
+                        w4_to_half(word_of(ca[a], w), h0);
+                        w4_to_half(word_of(cb[a], w), h1);
+                    }
+#pragma unroll
+                    for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+                        for (int mt = 0; mt < MT; ++mt) {
+                            const uint4 v = xv[q][mt];
+                            if (BF16) {
+                                mma_bf16(part[a][mt], h0[0], h1[0], h0[1], h1[1], v.x, v.y);
+                                mma_bf16(part[a][mt], h0[2], h1[2], h0[3], h1[3], v.z, v.w);
+                            } else {
+                                mma_f16(part[a][mt], h0[0], h1[0], h0[1], h1[1], v.x, v.y);
+                                mma_f16(part[a][mt], h0[2], h1[2], h0[3], h1[3], v.z, v.w);
+                            }
+                        }
+                }
+            }
+#pragma unroll
+            for (int a = 0; a < NSTR; ++a) {
+                const float s0 = __uint_as_float(sc[a][gi] << 16), s1 = __uint_as_float(sc[a][gi] & 0xFFFF0000u);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    acc[a][mt][0] = fmaf(s0, part[a][mt][0], acc[a][mt][0]);
+                    acc[a][mt][1] = fmaf(s0, part[a][mt][1], acc[a][mt][1]);
+                    acc[a][mt][2] = fmaf(s1, part[a][mt][2], acc[a][mt][2]);
+                    acc[a][mt][3] = fmaf(s1, part[a][mt][3], acc[a][mt][3]);
                 }
             }
         }
-    }
+    };
+
+    // ---- end of a unit: the warps' sums meet in shared memory (two buffers: one barrier per unit)
+    int done = 0;
+    auto finish = [&]() {
+        const int unit = (int)blockIdx.x + done * (int)gridDim.x;
+        float(*rb)[NSTR][MT * 8][17] = red[done & 1];
 #pragma unroll
-    for (int a = 0; a < NMAT; ++a)
+        for (int a = 0; a < NSTR; ++a)
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt)
+            for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) red[warp][a][8 * mt + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[a][mt][e];
-    __syncthreads();
-    for (int e = threadIdx.x; e < rows_per_cta * MT * 8 * 16; e += kG4Threads) {
-        const int r = e & 15, tl = (e >> 4) % rows_per_cta, tok = (e >> 4) / rows_per_cta;
-        const int64_t n = (int64_t)(blockIdx.x * rows_per_cta + tl) * 16 + r;
-        if (tok >= p.m || n >= p.n) continue;
-        float v[NMAT];
-#pragma unroll
-        for (int a = 0; a < NMAT; ++a) {
-            v[a] = 0.0f;
-            for (int w = 0; w < W; ++w) v[a] += red[tl * W + w][a][tok][r];
-            if (p.xinv) v[a] *= p.xinv[tok];
+                for (int e = 0; e < 4; ++e) rb[warp][a][8 * mt + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[a][mt][e];
+        asm volatile("bar.sync 0, %0;" ::"n"(kG4Threads) : "memory");
+        const int outs = GATED ? 1 : NSTR;
+        for (int e = threadIdx.x; e < rows_per_unit * outs * 16 * p.m; e += kG4Threads) {
+            const int r = e & 15, q = (e >> 4) % (rows_per_unit * outs), tok = (e >> 4) / (rows_per_unit * outs);
+            const int tl = q / outs, a0 = q % outs;
+            const int64_t n = ((int64_t)(unit * rows_per_unit + tl) * outs + a0) * 16 + r;
+            if (n >= p.n) continue;
+            float v[2] = {0.0f, 0.0f};
+            for (int w = 0; w < W; ++w) {
+                v[0] += rb[tl * W + w][a0][tok][r];
+                if (GATED) v[1] += rb[tl * W + w][NSTR - 1][tok][r];
+            }
+            if (p.xinv) {
+                const float f = __ldg(p.xinv + tok);
+                v[0] *= f, v[1] *= f;
+            }
+            const float out = GATED ? w4_silu(v[0]) * v[1] : p.bias ? v[0] + __ldg(p.bias + n) : v[0];
+            w4_store(p.y, p.y_dtype, (int64_t)tok * p.ldy + n, out);
         }
-        float out = v[0];
-        if (NMAT == 2)
-            out = w4_silu(v[0]) * v[NMAT - 1];
-        else if (p.bias)
-            out += p.bias[n];
-        w4_store(p.y, p.y_dtype, (int64_t)tok * p.ldy + n, out);
+        ++done;
+        clear();
+    };
+
+    int kt = ks, slot = 0;
+    for (int i = 0; i < total; ++i) {
+        copy_wait<DEPTH - 2>();  // tile i is here
+        uint4 ca[NSTR], cb[NSTR];
+        uint32_t sc[NSTR][GPT];
+#pragma unroll
+        for (int a = 0; a < NSTR; ++a) {
+            const int off = (slot * NSTR + a) * SM::kTile;
+            ca[a] = *reinterpret_cast<const uint4*>(mine + off);
+            cb[a] = *reinterpret_cast<const uint4*>(mine + off + 512);
+#pragma unroll
+            for (int gi = 0; gi < GPT; ++gi) sc[a][gi] = *reinterpret_cast<const uint32_t*>(mine_s + off + 4 * gi);
+        }
+        issue();  // into the slot of tile i - 1, whose values have been used
+        if (++slot == DEPTH) slot = 0;
+        consume(ca, cb, sc, kt);
+        kt += W;
+        if (kt >= KT) {
+            kt = ks;
+            finish();
+        }
     }
+    copy_wait<0>();
 }
 
-template <bool BF16, int MT, int PARTS, int NMAT>
-static cudaError_t launch_gemv_w4(const GemvW4Params& p, int gpt, cudaStream_t s) {
-    const unsigned grid = (unsigned)ceil_div(p.tile_rows, kG4Warps / p.wsplit);
-    switch (gpt) {
-        case 1: return w4_launch(gemv_w4_kernel<BF16, MT, PARTS, NMAT, 1>, grid, kG4Threads, 0, s, p);
-        case 2: return w4_launch(gemv_w4_kernel<BF16, MT, PARTS, NMAT, 2>, grid, kG4Threads, 0, s, p);
-        default: return w4_launch(gemv_w4_kernel<BF16, MT, PARTS, NMAT, 4>, grid, kG4Threads, 0, s, p);
+template <bool BF16, int MT, int PARTS, int NSTR, bool GATED, int GPT>
+static cudaError_t launch_gemv_w4(GemvW4Params p, cudaStream_t s) {
+    auto kernel = gemv_w4_kernel<BF16, MT, PARTS, NSTR, GATED, GPT>;
+    constexpr int smem = GemvW4Smem<NSTR, GPT>::kBytes;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    if (e != cudaSuccess) return e;
+    // CTAs that fit on an SM at once (the same on every device the library runs on)
+    static const int per_sm = [&] {
+        int c = 0;
+        return cudaOccupancyMaxActiveBlocksPerMultiprocessor(&c, kernel, kG4Threads, smem) == cudaSuccess && c > 0 ? c : 1;
+    }();
+    const int slots = per_sm * w4_sm_count(), rows = GATED ? 1 : NSTR;
+    // Warps per tile row: the fewest steps on the longest path - rounds of units over the CTA slots, each a warp's
+    // tiles and about two more for the joining of the sums.
+    int64_t best = INT64_MAX;
+    for (int w = 1; w <= 8 && w <= p.kt_total; w *= 2) {
+        const int64_t units = ceil_div(p.tile_rows, (int64_t)(kG4Warps / w) * rows);
+        const int64_t steps = ceil_div(units, slots) * (ceil_div(p.kt_total, w) * NSTR + 2);
+        if (steps <= best) best = steps, p.wsplit = w, p.units = (int)units;
     }
+    return w4_launch(kernel, (unsigned)(p.units < slots ? p.units : slots), kG4Threads, smem, s, p);
 }
 
-template <int MT, int NMAT>
-static cudaError_t launch_gemv_w4_x(const GemvW4Params& p, bool bf16, bool split, int gpt, cudaStream_t s) {
-    if (split) return launch_gemv_w4<false, MT, 2, NMAT>(p, gpt, s);
-    if (bf16) return launch_gemv_w4<true, MT, 1, NMAT>(p, gpt, s);
-    return launch_gemv_w4<false, MT, 1, NMAT>(p, gpt, s);
+template <bool BF16, int MT, int PARTS, int NSTR, bool GATED>
+static cudaError_t launch_gemv_w4_g(const GemvW4Params& p, int gpt, cudaStream_t s) {
+    if (gpt == 1) return launch_gemv_w4<BF16, MT, PARTS, NSTR, GATED, 1>(p, s);
+    if (gpt == 2) return launch_gemv_w4<BF16, MT, PARTS, NSTR, GATED, 2>(p, s);
+    return launch_gemv_w4<BF16, MT, PARTS, NSTR, GATED, 4>(p, s);
+}
+
+template <int MT, int NSTR, bool GATED>
+static cudaError_t launch_gemv_w4_x(const GemvW4Params& p, bool bf16, int gpt, cudaStream_t s) {
+    if (p.x[1]) return launch_gemv_w4_g<false, MT, 2, NSTR, GATED>(p, gpt, s);
+    if (bf16) return launch_gemv_w4_g<true, MT, 1, NSTR, GATED>(p, gpt, s);
+    return launch_gemv_w4_g<false, MT, 1, NSTR, GATED>(p, gpt, s);
 }
 
 int gemv_w4_run(const W4Call& c, const W4Acts& x) {
-    for (int64_t m0 = 0; m0 < c.m; m0 += 16) {
-        GemvW4Params p{};
-        p.m = (int)(c.m - m0 < 16 ? c.m - m0 : 16);
-        p.ldx = x.ld;
-        for (int i = 0; i < 2; ++i) p.x[i] = x.part[i] ? static_cast<const uint8_t*>(x.part[i]) + m0 * x.ld * 2 : nullptr;
-        p.xinv = x.inv ? x.inv + m0 : nullptr;
-        for (int i = 0; i < 2; ++i) {
-            p.w[i] = c.w[i].packed;
-            p.s[i] = reinterpret_cast<const uint32_t*>(c.w[i].scales);
-        }
-        p.bias = c.bias;
-        p.y = static_cast<uint8_t*>(c.y) + m0 * c.ldy * w4_elem(c.y_dtype);
-        p.ldy = c.ldy;
-        p.y_dtype = c.y_dtype;
-        p.n = (int)c.n;
-        p.k = (int)c.k;
-        p.kt_total = (int)w4_tiles_k(c.k);
-        p.tile_rows = (int)ceil_div(c.n, kTileRows);
-        p.wsplit = 1;
-        while (p.wsplit < 8 && p.tile_rows * (int64_t)p.wsplit < (int64_t)w4_sm_count() * 16 && 2 * p.wsplit <= p.kt_total)
-            p.wsplit *= 2;
-        const bool two = c.w[1].packed != nullptr, bf16 = x.bf16, split = x.part[1] != nullptr;
-        cudaError_t e;
-        if (p.m > 8)
-            e = two ? launch_gemv_w4_x<2, 2>(p, bf16, split, c.gpt, c.stream) : launch_gemv_w4_x<2, 1>(p, bf16, split, c.gpt, c.stream);
-        else
-            e = two ? launch_gemv_w4_x<1, 2>(p, bf16, split, c.gpt, c.stream) : launch_gemv_w4_x<1, 1>(p, bf16, split, c.gpt, c.stream);
-        if (e != cudaSuccess) return set_error(SBQ_ERR_CUDA, "gemv_w4 launch: %s", cudaGetErrorString(e));
+    GemvW4Params p{};
+    p.m = (int)c.m;
+    p.ldx = x.ld;
+    p.xinv = x.inv;
+    for (int i = 0; i < 2; ++i) {
+        p.x[i] = static_cast<const uint8_t*>(x.part[i]);
+        p.w[i] = c.w[i].packed;
+        p.s[i] = reinterpret_cast<const uint32_t*>(c.w[i].scales);
     }
+    p.bias = c.bias;
+    p.y = c.y;
+    p.ldy = c.ldy;
+    p.y_dtype = c.y_dtype;
+    p.n = (int)c.n;
+    p.k = (int)c.k;
+    p.kt_total = (int)w4_tiles_k(c.k);
+    p.tile_rows = (int)ceil_div(c.n, kTileRows);
+    // two tile rows per warp where there are plenty of them
+    const bool two = p.tile_rows >= 8 * w4_sm_count();
+    cudaError_t e;
+    if (p.m > 8)
+        e = c.w[1].packed ? launch_gemv_w4_x<2, 2, true>(p, x.bf16, c.gpt, c.stream)
+            : two         ? launch_gemv_w4_x<2, 2, false>(p, x.bf16, c.gpt, c.stream)
+                          : launch_gemv_w4_x<2, 1, false>(p, x.bf16, c.gpt, c.stream);
+    else
+        e = c.w[1].packed ? launch_gemv_w4_x<1, 2, true>(p, x.bf16, c.gpt, c.stream)
+            : two         ? launch_gemv_w4_x<1, 2, false>(p, x.bf16, c.gpt, c.stream)
+                          : launch_gemv_w4_x<1, 1, false>(p, x.bf16, c.gpt, c.stream);
+    if (e != cudaSuccess) return set_error(SBQ_ERR_CUDA, "gemv_w4 launch: %s", cudaGetErrorString(e));
     return check_launch("gemv_w4");
 }
 
