@@ -52,6 +52,26 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 
 __device__ __forceinline__ uint32_t word_of(const uint4& v, int w) { return w == 0 ? v.x : w == 1 ? v.y : w == 2 ? v.z : v.w; }
 
+// m16n8k16 product, d = a b (first) or d += a b.
+template <bool BF16>
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                          uint32_t b1, bool first) {
+    if (!first) {
+        BF16 ? mma_bf16(d, a0, a1, a2, a3, b0, b1) : mma_f16(d, a0, a1, a2, a3, b0, b1);
+        return;
+    }
+    if (BF16)
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+    else
+        asm volatile(
+            "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
+
 // Shared memory of one instance: [warp][slot][stream]: codes (1 KiB), then every lane's scales.
 template <int NSTR, int GPT>
 struct GemvW4Smem {
@@ -73,11 +93,15 @@ __global__ void __launch_bounds__(kG4Threads, MT * PARTS * NSTR == 1 ? 3 : 2) ge
     const int my_units = (p.units - (int)blockIdx.x + (int)gridDim.x - 1) / (int)gridDim.x, total = my_units * cnt;
 
     // ---- the stream of tiles: (unit, k tile) of the next copy, and its slot
-    int pu = blockIdx.x, pk = ks, pslot = 0;
+    int pu = blockIdx.x, pk = ks;
     const uint8_t* wp[NSTR];
     const uint32_t* sp[NSTR];
-    uint8_t* const mine = ring + warp * SM::kWarp + lane * 16;           // this lane's codes of slot 0
-    uint8_t* const mine_s = ring + warp * SM::kWarp + kW4TileBytes + lane * 4 * GPT;  // and scales
+    // this lane's codes in a slot are at 16 * lane (+ 512), its scales at kW4TileBytes + 4 GPT * lane
+    uint8_t* const ring0 = ring + warp * SM::kWarp + lane * 16;
+    const int scale_off = kW4TileBytes + lane * (4 * GPT - 16);
+    constexpr int kSlot = NSTR * SM::kTile;
+    const uint32_t put0 = (uint32_t)__cvta_generic_to_shared(ring0);
+    uint32_t put = put0;
     auto seek = [&]() {
 #pragma unroll
         for (int a = 0; a < NSTR; ++a) {
@@ -92,11 +116,10 @@ __global__ void __launch_bounds__(kG4Threads, MT * PARTS * NSTR == 1 ? 3 : 2) ge
         if (pu < p.units) {
 #pragma unroll
             for (int a = 0; a < NSTR; ++a) {
-                const int off = (pslot * NSTR + a) * SM::kTile;
-                const uint32_t dst = (uint32_t)__cvta_generic_to_shared(mine + off);
+                const uint32_t dst = put + a * SM::kTile;
                 copy_async<16>(dst, wp[a]);
                 copy_async<16>(dst + 512, wp[a] + 512);
-                copy_async<4 * GPT>((uint32_t)__cvta_generic_to_shared(mine_s + off), sp[a]);
+                copy_async<4 * GPT>(dst + scale_off, sp[a]);
                 wp[a] += (int64_t)W * kW4TileBytes;
                 sp[a] += W * 8 * GPT;
             }
@@ -107,7 +130,7 @@ __global__ void __launch_bounds__(kG4Threads, MT * PARTS * NSTR == 1 ? 3 : 2) ge
                 if (pu < p.units) seek();
             }
         }
-        if (++pslot == DEPTH) pslot = 0;
+        put = put == put0 + (DEPTH - 1) * kSlot ? put0 : put + kSlot;
         copy_commit();
     };
     seek();
@@ -116,13 +139,14 @@ __global__ void __launch_bounds__(kG4Threads, MT * PARTS * NSTR == 1 ? 3 : 2) ge
     asm volatile("griddepcontrol.wait;" ::: "memory");  // x, and y
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
+    // this lane's x of the tile that is consumed next: rows g (and 8 + g), columns 8 t .. of each word
     const uint8_t* xp[PARTS][MT];
 #pragma unroll
     for (int q = 0; q < PARTS; ++q)
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const int row = 8 * mt + g < p.m ? 8 * mt + g : 0;
-            xp[q][mt] = p.x[q] + ((int64_t)row * p.ldx + 8 * t) * 2;
+            xp[q][mt] = p.x[q] + ((int64_t)row * p.ldx + 8 * t + ks * kW4TileCols) * 2;
         }
     float acc[NSTR][MT][4];
     auto clear = [&]() {
@@ -136,28 +160,32 @@ __global__ void __launch_bounds__(kG4Threads, MT * PARTS * NSTR == 1 ? 3 : 2) ge
     clear();
 
     auto consume = [&](const uint4 (&ca)[NSTR], const uint4 (&cb)[NSTR], const uint32_t (&sc)[NSTR][GPT], int kt) {
-        const bool whole = (kt + 1) * kW4TileCols <= p.k;
+        constexpr bool AHEAD = PARTS * MT < 4;  // the tile's x at once, or (64 registers of it) word by word
+        uint4 xv[4][PARTS][MT];
+        const int left = p.k - kt * kW4TileCols - 8 * t;  // columns of x from this lane's first on
+        auto load_x = [&](int w0, int w1) {
 #pragma unroll
-        for (int gi = 0; gi < GPT; ++gi) {
-            float part[NSTR][MT][4];
-#pragma unroll
-            for (int a = 0; a < NSTR; ++a)
-#pragma unroll
-                for (int mt = 0; mt < MT; ++mt)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) part[a][mt][e] = 0.0f;
-#pragma unroll
-            for (int w = gi * (4 / GPT); w < (gi + 1) * (4 / GPT); ++w) {
-                uint4 xv[PARTS][MT];
-                const int c = kt * kW4TileCols + 32 * w;
+            for (int w = w0; w < w1; ++w)
 #pragma unroll
                 for (int q = 0; q < PARTS; ++q)
 #pragma unroll
                     for (int mt = 0; mt < MT; ++mt) {
-                        // x past k must read as zero (0 * inf is not), and not be touched
-                        xv[q][mt] = make_uint4(0, 0, 0, 0);
-                        if (whole || c + 8 * t < p.k) xv[q][mt] = *reinterpret_cast<const uint4*>(xp[q][mt] + (int64_t)c * 2);
+                        if (left >= kW4TileCols - 24) {
+                            xv[w][q][mt] = *reinterpret_cast<const uint4*>(xp[q][mt] + 64 * w);
+                        } else {
+                            // x past k must read as zero (0 * inf is not), and not be touched
+                            xv[w][q][mt] = make_uint4(0, 0, 0, 0);
+                            if (32 * w < left) xv[w][q][mt] = *reinterpret_cast<const uint4*>(xp[q][mt] + 64 * w);
+                        }
                     }
+        };
+        if (AHEAD) load_x(0, 4);
+#pragma unroll
+        for (int gi = 0; gi < GPT; ++gi) {
+            float part[NSTR][MT][4];
+#pragma unroll
+            for (int w = gi * (4 / GPT); w < (gi + 1) * (4 / GPT); ++w) {
+                if (!AHEAD) load_x(w, w + 1);
 #pragma unroll
                 for (int a = 0; a < NSTR; ++a) {
                     uint32_t h0[4], h1[4];
@@ -172,14 +200,9 @@ __global__ void __launch_bounds__(kG4Threads, MT * PARTS * NSTR == 1 ? 3 : 2) ge
                     for (int q = 0; q < PARTS; ++q)
 #pragma unroll
                         for (int mt = 0; mt < MT; ++mt) {
-                            const uint4 v = xv[q][mt];
-                            if (BF16) {
-                                mma_bf16(part[a][mt], h0[0], h1[0], h0[1], h1[1], v.x, v.y);
-                                mma_bf16(part[a][mt], h0[2], h1[2], h0[3], h1[3], v.z, v.w);
-                            } else {
-                                mma_f16(part[a][mt], h0[0], h1[0], h0[1], h1[1], v.x, v.y);
-                                mma_f16(part[a][mt], h0[2], h1[2], h0[3], h1[3], v.z, v.w);
-                            }
+                            const uint4 v = xv[w][q][mt];
+                            mma_first<BF16>(part[a][mt], h0[0], h1[0], h0[1], h1[1], v.x, v.y, w == gi * (4 / GPT) && q == 0);
+                            mma_first<BF16>(part[a][mt], h0[2], h1[2], h0[3], h1[3], v.z, v.w, false);
                         }
                 }
             }
@@ -208,11 +231,15 @@ __global__ void __launch_bounds__(kG4Threads, MT * PARTS * NSTR == 1 ? 3 : 2) ge
             for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) rb[warp][a][8 * mt + 2 * t + (e & 1)][g + 8 * (e >> 1)] = acc[a][mt][e];
-        asm volatile("bar.sync 0, %0;" ::"n"(kG4Threads) : "memory");
-        const int outs = GATED ? 1 : NSTR;
-        for (int e = threadIdx.x; e < rows_per_unit * outs * 16 * p.m; e += kG4Threads) {
-            const int r = e & 15, q = (e >> 4) % (rows_per_unit * outs), tok = (e >> 4) / (rows_per_unit * outs);
-            const int tl = q / outs, a0 = q % outs;
+        // the W warps of a tile row, by a barrier of their own
+        const int tl = warp / W;
+        if (W == 1)
+            __syncwarp();
+        else
+            asm volatile("bar.sync %0, %1;" ::"r"(1 + tl), "r"(32 * W) : "memory");
+        constexpr int outs = GATED ? 1 : NSTR;
+        for (int e = ks * 32 + lane; e < outs * 16 * p.m; e += 32 * W) {
+            const int r = e & 15, a0 = (e >> 4) % outs, tok = (e >> 4) / outs;
             const int64_t n = ((int64_t)(unit * rows_per_unit + tl) * outs + a0) * 16 + r;
             if (n >= p.n) continue;
             float v[2] = {0.0f, 0.0f};
@@ -231,24 +258,31 @@ __global__ void __launch_bounds__(kG4Threads, MT * PARTS * NSTR == 1 ? 3 : 2) ge
         clear();
     };
 
-    int kt = ks, slot = 0;
+    int kt = ks;
+    const uint8_t* get = ring0;
     for (int i = 0; i < total; ++i) {
         copy_wait<DEPTH - 2>();  // tile i is here
         uint4 ca[NSTR], cb[NSTR];
         uint32_t sc[NSTR][GPT];
 #pragma unroll
         for (int a = 0; a < NSTR; ++a) {
-            const int off = (slot * NSTR + a) * SM::kTile;
-            ca[a] = *reinterpret_cast<const uint4*>(mine + off);
-            cb[a] = *reinterpret_cast<const uint4*>(mine + off + 512);
+            const uint8_t* src = get + a * SM::kTile;
+            ca[a] = *reinterpret_cast<const uint4*>(src);
+            cb[a] = *reinterpret_cast<const uint4*>(src + 512);
 #pragma unroll
-            for (int gi = 0; gi < GPT; ++gi) sc[a][gi] = *reinterpret_cast<const uint32_t*>(mine_s + off + 4 * gi);
+            for (int gi = 0; gi < GPT; ++gi) sc[a][gi] = *reinterpret_cast<const uint32_t*>(src + scale_off + 4 * gi);
         }
         issue();  // into the slot of tile i - 1, whose values have been used
-        if (++slot == DEPTH) slot = 0;
+        get = get == ring0 + (DEPTH - 1) * kSlot ? ring0 : get + kSlot;
         consume(ca, cb, sc, kt);
         kt += W;
-        if (kt >= KT) {
+        const bool end = kt >= KT;
+        const int64_t step = (int64_t)(end ? ks - kt + W : W) * (2 * kW4TileCols);
+#pragma unroll
+        for (int q = 0; q < PARTS; ++q)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) xp[q][mt] += step;
+        if (end) {
             kt = ks;
             finish();
         }
