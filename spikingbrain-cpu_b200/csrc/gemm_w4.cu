@@ -65,10 +65,9 @@ struct W4Shape {
     static constexpr int kABufs0 = (TMEM - kACol) / 64;
     static constexpr int kABufs1 = kABufs0 < 4 ? kABufs0 : 4;
     static constexpr int kABufs = kABufs1 < kStages ? kABufs1 : kStages;  // 64 columns per 128 k
-    static constexpr int kSegBlocks = kSegSteps / (8 * PARTS);
     static constexpr int kXchOff = kStages * kStage;
     static constexpr int kBarOff = kXchOff + XCH;
-    static constexpr int kBytes = kBarOff + 512 + kW4Rows * 8 + 1024;
+    static constexpr int kBytes = kBarOff + 512 + 1024;  // barriers, alignment
     static_assert(kStages >= 2 && kABufs >= 2, "pipeline depth");
     static_assert((4 * kStages + 4) * 8 + 4 <= 512, "barriers");
     static_assert(kBytes <= 227 * 1024, "shared memory");
@@ -134,45 +133,6 @@ __device__ __forceinline__ void w4_convert_half(const uint8_t* codes, const uint
     tmem_st_x16(tmem_dst + 16, h);
 }
 
-// All 128 columns of channel `row` -> 64 tensor-memory columns.
-template <int GPT>
-__device__ __forceinline__ void w4_convert_tile(const uint8_t* codes, const uint8_t* scales, int row, float rowmul,
-                                                uint32_t tmem_dst) {
-    uint32_t s2[GPT], c2[GPT];
-    w4_scales<GPT>(scales, row, rowmul, 0, s2, c2, GPT);
-    uint4 raw[4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t)
-        raw[t] = *reinterpret_cast<const uint4*>(codes + row * 64 + ((t ^ ((row >> 1) & 3)) << 4));
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-        uint32_t h[32];
-        const int ga = half * GPT / 2, gb = (2 * half + 1) * GPT / 4;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            w4_convert_word(half ? raw[t].z : raw[t].x, s2[ga], c2[ga], h + 4 * t);
-            w4_convert_word(half ? raw[t].w : raw[t].y, s2[gb], c2[gb], h + 16 + 4 * t);
-        }
-        tc::tmem_st_32x32b_x32(tmem_dst + half * 32, h);
-    }
-}
-
-// Adds `COLS` accumulator columns at `taddr` to a thread's sums (FIRST: takes them).
-template <int COLS>
-__device__ __forceinline__ void w4_take_segment(uint32_t taddr, float (&sum)[COLS], bool first) {
-#pragma unroll
-    for (int c = 0; c < COLS / 32; ++c) {
-        uint32_t r[32];
-        tc::tmem_ld_32x32b_x32(taddr + c * 32, r);
-        tc::tmem_wait_ld();
-#pragma unroll
-        for (int j = 0; j < 32; ++j) {
-            const float v = __uint_as_float(r[j]);
-            sum[32 * c + j] = first ? v : sum[32 * c + j] + v;
-        }
-    }
-}
-
 // Channel of tensor-memory lane `row` (CTA's first channel n0): with two matrices lanes 0..63 are the
 // gate's channels n0.., lanes 64..127 the up projection's.
 template <int NMAT>
@@ -180,30 +140,6 @@ __device__ __forceinline__ int w4_channel(int n0, int row) { return n0 + (NMAT =
 
 // Up to 128 named-barrier threads of one converter warpgroup.
 __device__ __forceinline__ void group_sync(int grp) { asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory"); }
-
-// Epilogue of one 32-token slice: v holds lane `row`'s sums of tokens tb.., already scaled.  With two matrices
-// the up lanes hand theirs over through `xch` ([token][64]) and the gate lanes finish.
-template <int NMAT>
-__device__ __forceinline__ void w4_finish(const GemmW4Params& p, const float (&v)[32], int tb, int n, int row, int grp,
-                                          float bias, float* xch, bool ok) {
-    if (NMAT == 2) {
-        if (row >= 64) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j) xch[j * 64 + (row & 63)] = v[j];
-        }
-        group_sync(grp);
-        if (row < 64 && n < p.n && ok) {
-#pragma unroll
-            for (int j = 0; j < 32; ++j)
-                if (tb + j < p.m) w4_store(p.y, p.y_dtype, (int64_t)(tb + j) * p.ldy + n, w4_silu(v[j]) * xch[j * 64 + row]);
-        }
-        group_sync(grp);
-    } else if (n < p.n && ok) {
-#pragma unroll
-        for (int j = 0; j < 32; ++j)
-            if (tb + j < p.m) w4_store(p.y, p.y_dtype, (int64_t)(tb + j) * p.ldy + n, v[j] + bias);
-    }
-}
 
 // ---------------------------------------------------------------------------------------------
 // More than 128 rows: CTA pairs (cta_group::2), persistent.  A pair computes tiles of 256 channels x TOK tokens one
@@ -626,11 +562,13 @@ __global__ void __launch_bounds__(2 * kW4Rows) w4_reduce_kernel(const GemmW4Para
 // ---------------------------------------------------------------------------------------------
 // 17..128 rows: 128 channels x 64 tokens per CTA, two CTAs per SM, k split over the CTAs of a cluster when
 // the tiles alone are too few: each pushes its fp32 sums into the shared memory of the CTA that owns the
-// channel, which adds them in part order.
+// channel, which adds them in part order.  The two converter warpgroups take alternate blocks (each warp on half of
+// every block, as in the pair kernel, was 15 % slower: with two CTAs on an SM the waits of a block count) and both
+// take the sums, 32 tokens each.
 // ---------------------------------------------------------------------------------------------
 constexpr int kSTok4 = 64;
 template <int PARTS>
-using W4Small = W4Shape<kSTok4, kSTok4, PARTS, 2, 256, 108 * 1024, 0>;
+using W4Small = W4Shape<kSTok4, kSTok4, PARTS, 1, 256, 108 * 1024, 0>;
 
 template <int PARTS, int NMAT, int GPT>
 __global__ void __launch_bounds__(kW4Threads, 2)
@@ -649,10 +587,8 @@ __global__ void __launch_bounds__(kW4Threads, 2)
     uint64_t* conv_done = ready + NS;
     uint64_t* mma_done = conv_done + NS;
     uint64_t* done = mma_done + NS;
-    uint64_t* taken = done + 2;
-    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 2);
-    float* s_mul = reinterpret_cast<float*>(smem + S::kBarOff + 512);
-    float* s_bias = s_mul + kW4Rows;
+    uint64_t* taken = done + 1;
+    uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(taken + 1);
     float* recv = reinterpret_cast<float*>(smem);
 
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -668,10 +604,8 @@ __global__ void __launch_bounds__(kW4Threads, 2)
             tc::mbar_init(&conv_done[s], 4);
             tc::mbar_init(&mma_done[s], 1);
         }
-        tc::mbar_init(&done[0], 1);
-        tc::mbar_init(&done[1], 1);
-        tc::mbar_init(&taken[0], 8);
-        tc::mbar_init(&taken[1], 8);
+        tc::mbar_init(done, 1);
+        tc::mbar_init(taken, 8);
         tc::fence_mbar_init();
         tc::prefetch_tmap(&map_x);
         tc::prefetch_tmap(&map_w);
@@ -681,11 +615,6 @@ __global__ void __launch_bounds__(kW4Threads, 2)
         tc::tmem_alloc(tmem_slot, 256);
         tc::tmem_relinquish();
     }
-    for (int i = threadIdx.x; i < kW4Rows; i += blockDim.x) {
-        const int n = w4_channel<NMAT>(n0, i);
-        s_mul[i] = n < p.n ? p.rowmul[NMAT == 2 ? i >> 6 : 0][n] : 1.0f;
-        s_bias[i] = p.bias && n < p.n ? p.bias[n] : 0.0f;
-    }
     tc::fence_before_sync();
     __syncthreads();
     tc::fence_after_sync();
@@ -694,8 +623,7 @@ __global__ void __launch_bounds__(kW4Threads, 2)
 
     if (warp == 0) {
         if (lane == 0) {
-            auto load_w = [&](int i) {
-                const int s = i % NS, kb = kb0 + i;
+            auto load_w = [&](int s, int kb) {
                 uint8_t* ws = smem + s * S::kStage + S::kXBytes;
                 tc::mbar_arrive_expect_tx(&wfull[s], S::kCodes + 256 * GPT);
                 tc::tma_load_4d(ws, &map_w, &wfull[s], 0, 0, kb, n0 / 16);
@@ -705,8 +633,7 @@ __global__ void __launch_bounds__(kW4Threads, 2)
                     tma_load_3d(ws + S::kCodes + 128 * GPT, &map_s2, &wfull[s], 0, kb, n0 / 16);
                 }
             };
-            auto load_x = [&](int i) {
-                const int s = i % NS, kb = kb0 + i;
+            auto load_x = [&](int s, int kb) {
                 uint8_t* xs = smem + s * S::kStage;
                 tc::mbar_arrive_expect_tx(&ready[s], S::kXBytes);
 #pragma unroll
@@ -716,69 +643,98 @@ __global__ void __launch_bounds__(kW4Threads, 2)
                 }
             };
             const int pre = nkb < NS ? nkb : NS;
-            for (int i = 0; i < pre; ++i) load_w(i);
+            for (int i = 0; i < pre; ++i) load_w(i, kb0 + i);
             asm volatile("griddepcontrol.wait;" ::: "memory");
             asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-            for (int i = 0; i < pre; ++i) load_x(i);
+            for (int i = 0; i < pre; ++i) load_x(i, kb0 + i);
+            int s = 0;
+            uint32_t ph = 0;
             for (int i = pre; i < nkb; ++i) {
-                const int s = i % NS;
-                const uint32_t ph = (i / NS) & 1;
-                if (!tc::mbar_wait(&conv_done[s], ph ^ 1)) break;
-                if (!tc::mbar_wait(&mma_done[s], ph ^ 1)) break;
-                load_w(i);
-                load_x(i);
+                if (!tc::mbar_wait(&conv_done[s], ph)) break;
+                if (!tc::mbar_wait(&mma_done[s], ph)) break;
+                load_w(s, kb0 + i);
+                load_x(s, kb0 + i);
+                if (++s == NS) s = 0, ph ^= 1;
             }
         }
     } else if (warp == 1) {
         if (lane == 0) {
-            constexpr uint32_t idesc = tc::idesc_f16(kW4Rows, kSTok4, false);
+            const int tokens = p.m - t0 < kSTok4 ? (p.m - t0 + 15) & ~15 : kSTok4;
+            const uint32_t idesc = tc::idesc_f16(kW4Rows, tokens, false);
+            const uint64_t desc0 = tc::smem_desc(smem, tc::kSwizzle128B, 1024);
+            int s = 0, ab = 0, seg = 0, left = 0;
+            uint32_t ph = 0;
             for (int i = 0; i < nkb; ++i) {
-                const int s = i % NS, seg = i / S::kSegBlocks;
-                const bool fresh = i % S::kSegBlocks == 0;
-                if (fresh && seg >= 2 && !tc::mbar_wait(&taken[seg & 1], ((seg >> 1) - 1) & 1)) break;
-                if (!tc::mbar_wait(&ready[s], (i / NS) & 1)) break;
+                const bool fresh = left == 0;
+                if (fresh) {
+                    left = p.seg_blocks < nkb - i ? p.seg_blocks : nkb - i;
+                    if (seg > 0 && !tc::mbar_wait(taken, (seg - 1) & 1)) break;
+                }
+                if (!tc::mbar_wait(&ready[s], ph)) break;
                 tc::fence_after_sync();
-                const uint8_t* xs = smem + s * S::kStage;
-                const uint32_t d = tmem + (seg & 1) * kSTok4, a = tmem + S::kACol + (i % NA) * 64;
+                const uint64_t xd = desc0 + (uint64_t)(s * (S::kStage / 16));
+                const uint32_t op = tmem + S::kACol + ab * 64;
 #pragma unroll
                 for (int j = 0; j < 8; ++j)
 #pragma unroll
-                    for (int q = 0; q < PARTS; ++q) {
-                        const uint64_t bd = tc::smem_desc(xs + ((j >> 2) * PARTS + q) * S::kXSub + (j & 3) * 32, tc::kSwizzle128B, 1024);
-                        tc::mma_f16_ts(d, a + j * 8, bd, idesc, !(fresh && j == 0 && q == 0));
-                    }
+                    for (int q = 0; q < PARTS; ++q)
+                        tc::mma_f16_ts(tmem, op + j * 8, xd + (((j >> 2) * PARTS + q) * S::kXSub + (j & 3) * 32) / 16, idesc,
+                                       j == 0 && q == 0 ? !fresh : 1u);
                 tc::mma_commit(&mma_done[s]);
-                if (i + 1 == nkb || (i + 1) % S::kSegBlocks == 0) tc::mma_commit(&done[seg & 1]);
+                if (--left == 0) {
+                    tc::mma_commit(done);
+                    ++seg;
+                }
+                if (++s == NS) s = 0, ph ^= 1;
+                if (++ab == NA) ab = 0;
             }
         }
     } else if (warp >= 4) {
-        const int grp = (warp - 4) >> 2, wq = (warp - 4) & 3, row = wq * 32 + lane;
+        const int half = (warp - 4) >> 2, wq = warp & 3, row = wq * 32 + lane;
         const uint32_t lane_tmem = tmem + ((uint32_t)(wq * 32) << 16);
-        const float mul = s_mul[row];
-        int taken_segs = 0;
+        const int n = w4_channel<NMAT>(n0, row);
+        const float mul = n < p.n ? __ldg(p.rowmul[NMAT == 2 ? row >> 6 : 0] + n) : 1.0f;
+        // the next segment to take: its parity and its last block
+        uint32_t tk_ph = 0;
+        int tk_last = p.seg_blocks < nkb ? p.seg_blocks - 1 : nkb - 1;
 #pragma unroll
         for (int j = 0; j < 32; ++j) sum[j] = 0.0f;
         auto take = [&]() -> bool {
-            if (!__all_sync(0xffffffffu, tc::mbar_wait(&done[taken_segs & 1], (taken_segs >> 1) & 1))) return false;
+            if (!__all_sync(0xffffffffu, tc::mbar_wait(done, tk_ph))) return false;
+            tk_ph ^= 1;
             tc::fence_after_sync();
-            w4_take_segment<32>(lane_tmem + (taken_segs & 1) * kSTok4 + grp * 32, sum, false);
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                uint32_t r[16];
+                tmem_ld_x16(lane_tmem + half * 32 + c * 16, r);
+                tc::tmem_wait_ld();
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sum[c * 16 + j] += __uint_as_float(r[j]);
+            }
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&taken[taken_segs & 1]);
-            ++taken_segs;
+            if (lane == 0) tc::mbar_arrive(taken);
+            // the last segment has no next: past the end
+            tk_last = tk_last == nkb - 1 ? nkb : tk_last + p.seg_blocks < nkb - 1 ? tk_last + p.seg_blocks : nkb - 1;
             return true;
         };
         bool ok = true;
-        for (int i = grp; i < nkb; i += 2) {
+        for (int i = half; i < nkb; i += 2) {
             const int s = i % NS;
             if (i >= NA) {
+                // the operand buffer's last reader, block i - NA; a segment is taken when its last block's MMAs
+                // are done, or this warp's next block would wait for MMAs that wait for the taking
                 const int prev = i - NA;
                 if (!__all_sync(0xffffffffu, tc::mbar_wait(&mma_done[prev % NS], (prev / NS) & 1))) { ok = false; break; }
+                while (ok && tk_last < prev + 2) ok = take();
+                if (!ok) break;
             }
             if (!__all_sync(0xffffffffu, tc::mbar_wait(&wfull[s], (i / NS) & 1))) { ok = false; break; }
             tc::fence_after_sync();
             const uint8_t* codes = smem + s * S::kStage + S::kXBytes;
-            w4_convert_tile<GPT>(codes, codes + S::kCodes, row, mul, lane_tmem + S::kACol + (i % NA) * 64);
+            const uint32_t dst = lane_tmem + S::kACol + (i % NA) * 64;
+            w4_convert_half<GPT>(codes, codes + S::kCodes, row, mul, 0, dst);
+            w4_convert_half<GPT>(codes, codes + S::kCodes, row, mul, 1, dst + 32);
             tc::tmem_wait_st();
             tc::fence_before_sync();
             __syncwarp();
@@ -786,20 +742,28 @@ __global__ void __launch_bounds__(kW4Threads, 2)
                 tc::mbar_arrive(&ready[s]);
                 tc::mbar_arrive(&conv_done[s]);
             }
-            if (i - NA + 1 >= (taken_segs + 1) * S::kSegBlocks && !(ok = take())) break;
         }
-        while (ok && taken_segs * S::kSegBlocks < nkb) ok = take();
+        while (ok && tk_last < nkb) ok = take();
         asm volatile("griddepcontrol.wait;" ::: "memory");  // before y is written, and xinv read
         const float inv = 1.0f / mul;
 #pragma unroll
         for (int j = 0; j < 32; ++j) sum[j] *= inv;
         if (p.parts == 1) {
-            const int tb = t0 + grp * 32;
-            if (p.xinv) {
+            const int tb = t0 + half * 32;
+            if (p.xinv) w4_times_xinv<32>(p.xinv, tb, sum);
+            const float bias = p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
+            if (NMAT == 1) {
+                if (ok) w4_put<32>(p, tb, n, [&](int j) { return sum[j] + bias; });
+            } else {
+                // the up lanes hand their values to the gate lanes, which finish; no load is on its way into the ring
+                float* xch = recv + half * 32 * 64;
+                if (row >= 64) {
 #pragma unroll
-                for (int j = 0; j < 32; ++j) sum[j] *= tb + j < p.m ? p.xinv[tb + j] : 0.0f;
+                    for (int j = 0; j < 32; ++j) xch[j * 64 + (row & 63)] = sum[j];
+                }
+                group_sync(half);
+                if (row < 64 && ok) w4_put<32>(p, tb, n, [&](int j) { return w4_silu(sum[j]) * xch[j * 64 + row]; });
             }
-            w4_finish<NMAT>(p, sum, tb, w4_channel<NMAT>(n0, row), row, grp, s_bias[row], recv + grp * 32 * 64, ok);
         }
     }
     if (p.parts > 1) {
@@ -809,9 +773,9 @@ __global__ void __launch_bounds__(kW4Threads, 2)
         tc::cluster_sync();
         const int share = kCh / p.parts;  // a power of two, at least 8
         if (warp >= 4) {
-            const int grp = (warp - 4) >> 2, row = ((warp - 4) & 3) * 32 + lane;
+            const int half = (warp - 4) >> 2, row = (warp & 3) * 32 + lane;
             const int mat = NMAT == 2 ? row >> 6 : 0, c = NMAT == 2 ? row & 63 : row, owner = c / share;
-            const uint32_t dst = tc::cluster_addr(recv + ((part * kSTok4 + grp * 32) * NMAT + mat) * share + c % share, (uint32_t)owner);
+            const uint32_t dst = tc::cluster_addr(recv + ((part * kSTok4 + half * 32) * NMAT + mat) * share + c % share, (uint32_t)owner);
 #pragma unroll
             for (int j = 0; j < 32; ++j)
                 asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(dst + (uint32_t)(j * NMAT * share * 4)), "f"(sum[j]) : "memory");
@@ -819,7 +783,7 @@ __global__ void __launch_bounds__(kW4Threads, 2)
         tc::cluster_sync();
         asm volatile("griddepcontrol.wait;" ::: "memory");
         for (int e = threadIdx.x; e < share * kSTok4; e += blockDim.x) {
-            const int c = e % share, t = e / share, ch = part * share + c, n = n0 + ch;
+            const int c = e % share, t = e / share, n = n0 + part * share + c;
             if (t0 + t >= p.m || n >= p.n) continue;
             float v[NMAT];
 #pragma unroll
@@ -828,7 +792,7 @@ __global__ void __launch_bounds__(kW4Threads, 2)
                 for (int q = 0; q < p.parts; ++q) v[a] += recv[((q * kSTok4 + t) * NMAT + a) * share + c];
                 if (p.xinv) v[a] *= p.xinv[t0 + t];
             }
-            const float out = NMAT == 2 ? w4_silu(v[0]) * v[NMAT - 1] : v[0] + s_bias[ch];
+            const float out = NMAT == 2 ? w4_silu(v[0]) * v[NMAT - 1] : p.bias ? v[0] + __ldg(p.bias + n) : v[0];
             w4_store(p.y, p.y_dtype, (int64_t)(t0 + t) * p.ldy + n, out);
         }
     }
@@ -890,13 +854,13 @@ static cudaError_t launch_maps(K kernel, dim3 grid, int threads, int smem, int p
 
 template <int PARTS, int NMAT, int GPT>
 static cudaError_t launch_gemm_w4(int tok, int npairs, const W4Maps& m, GemmW4Params p, cudaStream_t s) {
+    p.seg_blocks = p.y_dtype == SBQ_F32 ? kSegSteps / (8 * PARTS) : p.kt;
     if (tok == kSTok4)
         return launch_maps(gemm_w4_small_kernel<PARTS, NMAT, GPT>,
                            dim3((unsigned)ceil_div(p.n, kW4Rows / NMAT), (unsigned)ceil_div(p.m, kSTok4), (unsigned)p.parts),
                            kW4Threads, W4Small<PARTS>::kBytes, p.parts, s, m, p);
-    using S = W4Pair<PARTS, NMAT>;
-    p.seg_blocks = p.y_dtype == SBQ_F32 ? S::kSegBlocks : p.kt;
-    return launch_maps(gemm_w4_pair_kernel<PARTS, NMAT, GPT>, dim3(2 * (unsigned)npairs), kPairThreads, S::kBytes, 0, s, m, p);
+    return launch_maps(gemm_w4_pair_kernel<PARTS, NMAT, GPT>, dim3(2 * (unsigned)npairs), kPairThreads,
+                       W4Pair<PARTS, NMAT>::kBytes, 0, s, m, p);
 }
 
 template <int PARTS, int NMAT>
@@ -957,8 +921,9 @@ int gemm_w4_run(const W4Call& c, const W4Acts& x) {
     const int tok = c.m <= kW4SmallRows ? kSTok4 : kTok;
     W4Plan pl{};
     if (tok == kSTok4) {
-        // k parts: the largest power of two up to 8 that keeps the grid within 7/8 of the CTA slots (two per
-        // SM; a cluster needs all of its CTAs at once) and gives every part at least two tiles
+        // k parts per tile (the cluster size): the largest power of two up to 8 that keeps the grid within 7/8 of the
+        // CTA slots (two per SM) and gives every part at least two blocks.  A cluster needs all of its CTAs in one
+        // GPC at once: 64 x 4096 x 12288 (96 tiles) takes 20.1 us with 2 parts, 28.2 us with 3 (288 of 296 slots)
         const int64_t tiles = ceil_div(c.n, ch) * ceil_div(c.m, kSTok4);
         while (p.parts < 8 && tiles * (2 * p.parts) * 8 <= (int64_t)2 * sms * 7 && p.kt / (2 * p.parts) >= 2) p.parts *= 2;
     } else {

@@ -24,7 +24,7 @@ int w4_sm_count() {
 // Row r of x times 2^(14 - e), 2^e <= max |x[r]| < 2^(e + 1) over its finite values, as fp16 (bf16 x:
 // exact unless an element is below 2^-31 of the row's largest) or as two fp16 parts hi + lo (fp32 x: 22
 // bits, the difference x - hi is exact).  Infinities and NaN stay what they are.  inv[r] = 2^(e - 14).
-constexpr int kActThreads = 256;
+constexpr int kActThreads = 512;
 
 struct ActParams {
     const void* x;
@@ -52,35 +52,49 @@ __device__ __forceinline__ void act_load8(const void* x, int64_t i, float (&v)[8
     }
 }
 
-template <bool F32>
+// One row per CTA.  V chunks of 8 columns per thread stay in registers between the maximum and the conversion; V = 0:
+// any k, the row is read twice.
+template <bool F32, int V>
 __global__ void __launch_bounds__(kActThreads) w4_acts_kernel(const ActParams p) {
     __shared__ float part[kActThreads / 32];
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int64_t row = blockIdx.x, x0 = row * p.ldx, o0 = row * p.k;
-    float big = 0.0f;
-    for (int c = threadIdx.x * 8; c < p.k; c += kActThreads * 8) {
-        float v[8];
-        act_load8<F32>(p.x, x0 + c, v);
+    constexpr int kStep = kActThreads * 8;
+    float keep[V ? V : 1][8], big = 0.0f;
+    auto widen = [&](const float (&v)[8]) {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (isfinite(v[i])) big = fmaxf(big, fabsf(v[i]));
+    };
+    if (V) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = threadIdx.x * 8 + i * kStep;
+            if (c < p.k) act_load8<F32>(p.x, x0 + c, keep[i]);
+        }
+#pragma unroll
+        for (int i = 0; i < V; ++i)
+            if ((int)threadIdx.x * 8 + i * kStep < p.k) widen(keep[i]);
+    } else {
+        for (int c = threadIdx.x * 8; c < p.k; c += kStep) {
+            act_load8<F32>(p.x, x0 + c, keep[0]);
+            widen(keep[0]);
+        }
     }
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
     if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = big;
     __syncthreads();
-    big = part[0];
+    big = part[threadIdx.x & (kActThreads / 32 - 1)];
 #pragma unroll
-    for (int i = 1; i < kActThreads / 32; ++i) big = fmaxf(big, part[i]);
+    for (int o = 16; o > 0; o >>= 1) big = fmaxf(big, __shfl_xor_sync(0xffffffffu, big, o));
     // exponents clamped so that both the factor and its inverse are normal numbers
     int e = big > 0.0f ? 14 - ilogbf(big) : 0;
     e = e > 126 ? 126 : e < -126 ? -126 : e;
     const float mul = scalbnf(1.0f, e);
     if (threadIdx.x == 0) p.inv[row] = scalbnf(1.0f, -e);
-    for (int c = threadIdx.x * 8; c < p.k; c += kActThreads * 8) {
-        float v[8];
-        act_load8<F32>(p.x, x0 + c, v);
+    auto put = [&](const float (&v)[8], int c) {
         uint32_t h[4], l[4];
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
@@ -96,7 +110,26 @@ __global__ void __launch_bounds__(kActThreads) w4_acts_kernel(const ActParams p)
         }
         *reinterpret_cast<uint4*>(p.hi + o0 + c) = make_uint4(h[0], h[1], h[2], h[3]);
         if (F32) *reinterpret_cast<uint4*>(p.lo + o0 + c) = make_uint4(l[0], l[1], l[2], l[3]);
+    };
+    if (V) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = threadIdx.x * 8 + i * kStep;
+            if (c < p.k) put(keep[i], c);
+        }
+    } else {
+        for (int c = threadIdx.x * 8; c < p.k; c += kStep) {
+            act_load8<F32>(p.x, x0 + c, keep[0]);
+            put(keep[0], c);
+        }
     }
+}
+
+template <bool F32>
+static cudaError_t launch_acts(const ActParams& p, int64_t m, cudaStream_t s) {
+    if (p.k <= kActThreads * 8) return w4_launch(w4_acts_kernel<F32, 1>, (unsigned)m, kActThreads, 0, s, p);
+    if (p.k <= kActThreads * 24) return w4_launch(w4_acts_kernel<F32, 3>, (unsigned)m, kActThreads, 0, s, p);
+    return w4_launch(w4_acts_kernel<F32, 0>, (unsigned)m, kActThreads, 0, s, p);
 }
 
 constexpr int64_t kW4GemvRows = 16;  // up to this many rows: the decode product
@@ -165,8 +198,7 @@ static int w4_run(const void* x, int x_dtype, int64_t ldx, const W4Call& c, int 
         p.lo = x_dtype == SBQ_F32 ? reinterpret_cast<__half*>(ws + one) : nullptr;
         p.inv = reinterpret_cast<float*>(ws + (x_dtype == SBQ_F32 ? 2 : 1) * one);
         p.k = (int)c.k;
-        const cudaError_t e = x_dtype == SBQ_F32 ? w4_launch(w4_acts_kernel<true>, (unsigned)c.m, kActThreads, 0, c.stream, p)
-                                                 : w4_launch(w4_acts_kernel<false>, (unsigned)c.m, kActThreads, 0, c.stream, p);
+        const cudaError_t e = x_dtype == SBQ_F32 ? launch_acts<true>(p, c.m, c.stream) : launch_acts<false>(p, c.m, c.stream);
         if (e != cudaSuccess) return set_error(SBQ_ERR_CUDA, "w4 activation parts launch: %s", cudaGetErrorString(e));
         a.part[0] = p.hi;
         a.part[1] = p.lo;
