@@ -43,15 +43,15 @@ __device__ __forceinline__ void ld8(const void* p, int dtype, int64_t i, float (
     }
     const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
     const uint32_t u[4] = {a.x, a.y, a.z, a.w};
+    if (dtype == SBQ_F16) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (dtype == SBQ_F16) {
+        for (int j = 0; j < 4; ++j) {
             const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&u[j]));
             v[2 * j] = f.x, v[2 * j + 1] = f.y;
-        } else {
-            v[2 * j] = __uint_as_float(u[j] << 16);
-            v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
         }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(u[j] << 16), v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
     }
 }
 
@@ -63,12 +63,15 @@ __device__ __forceinline__ void st8(void* p, int dtype, int64_t i, const float (
         return;
     }
     uint32_t u[4];
+    if (dtype == SBQ_F16) {
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        if (dtype == SBQ_F16) {
+        for (int j = 0; j < 4; ++j) {
             const __half2 h = __floats2half2_rn(v[2 * j], v[2 * j + 1]);
             u[j] = *reinterpret_cast<const uint32_t*>(&h);
-        } else {
+        }
+    } else {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
             const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * j], v[2 * j + 1]);
             u[j] = *reinterpret_cast<const uint32_t*>(&h);
         }
@@ -76,212 +79,381 @@ __device__ __forceinline__ void st8(void* p, int dtype, int64_t i, const float (
     *reinterpret_cast<uint4*>(static_cast<uint16_t*>(p) + i) = make_uint4(u[0], u[1], u[2], u[3]);
 }
 
-__device__ __forceinline__ float gate_act(float g, int act) {
-    if (act == SBQ_GATE_SIGMOID) return 1.0f / (1.0f + expf(-g));
-    if (act == SBQ_GATE_SILU) return g / (1.0f + expf(-g));
-    if (act == SBQ_GATE_TANH) return tanhf(g);
-    return g;
+// Eight fp32 weights from column c on, any c in [0, d - 8]: three aligned quads and a shift that is the same for a
+// row (eight single loads cost three times the L1 cycles).
+__device__ __forceinline__ void ld8_weight(const float* w, int c, int d, float (&o)[8]) {
+    const int s = c & 3;
+    const float4* q = reinterpret_cast<const float4*>(w + (c - s));
+    const float4 a = __ldg(q), b = __ldg(q + 1);
+    // the third quad holds columns of this chunk only if s > 0, and all of it may lie past the end
+    float4 e = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    if (s > 0) {
+        if (c - s + 12 <= d) {
+            e = __ldg(q + 2);
+        } else {
+            const float* t = w + (c - s + 8);
+            e.x = __ldg(t);
+            if (s > 1) e.y = __ldg(t + 1);
+            if (s > 2) e.z = __ldg(t + 2);
+        }
+    }
+    const float v[12] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w, e.x, e.y, e.z, e.w};
+    if (s == 0) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = v[i];
+    } else if (s == 1) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = v[i + 1];
+    } else if (s == 2) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = v[i + 2];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) o[i] = v[i + 3];
+    }
 }
 
-// Sum over the TPR threads of a row (TPR = 32: a warp; otherwise the whole CTA).  `part` holds one float
-// per warp; two calls in a row use different buffers, so one barrier per call is enough.
+// Elements lo .. hi - 1 of eight.
+__device__ __forceinline__ void st8_some(void* p, int dtype, int64_t i, int lo, int hi, const float (&v)[8]) {
+    if (dtype == SBQ_F32) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j >= lo && j < hi) static_cast<float*>(p)[i + j] = v[j];
+    } else if (dtype == SBQ_F16) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j >= lo && j < hi) static_cast<__half*>(p)[i + j] = __float2half_rn(v[j]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            if (j >= lo && j < hi) static_cast<__nv_bfloat16*>(p)[i + j] = __float2bfloat16_rn(v[j]);
+    }
+}
+
+__device__ __forceinline__ float ex2_approx(float v) {
+    float r;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+__device__ __forceinline__ float rcp_approx(float v) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
+    return r;
+}
+
+// 1 / (1 + 2^(-g log2 e)) from the hardware's power of two and reciprocal: relative error a few 2^-22 where the
+// gate is not 0 or 1 to fp32.  (expf and an exact division made the gated step instruction-bound.)
+__device__ __forceinline__ float sigmoid_approx(float g) { return rcp_approx(1.0f + ex2_approx(-1.44269504f * g)); }
+
+__device__ __forceinline__ void gate_act8(float (&g)[8], int act) {
+    if (act == SBQ_GATE_SIGMOID) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = sigmoid_approx(g[i]);
+    } else if (act == SBQ_GATE_SILU) {
+        // g * sigmoid(g): an infinite negative g gives -inf * 0 = NaN, where the limit is 0
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] *= sigmoid_approx(g[i]);
+    } else if (act == SBQ_GATE_TANH) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = tanhf(g[i]);
+    }
+}
+
+// Threads per row: TPR (8, 16, 32: several rows per CTA, a row's threads are neighbouring lanes) or, for TPR = 0, the
+// whole CTA, of any number of warps.
+template <int TPR>
+__device__ __forceinline__ int row_threads() { return TPR ? TPR : (int)blockDim.x; }
+
+// Sum over a row's threads.  `part` holds one float per warp; two calls in a row use different buffers, so one
+// barrier per call is enough.
 template <int TPR>
 __device__ __forceinline__ float row_sum(float v, float* part) {
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
-    if (TPR == 32) return v;
+    for (int o = (TPR ? TPR : 32) / 2; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
+    if (TPR) return v;
     const int lane = threadIdx.x & 31;
     if (lane == 0) part[threadIdx.x >> 5] = v;
     __syncthreads();
-    v = lane < TPR / 32 ? part[lane] : 0.0f;
+    v = lane < (int)(blockDim.x >> 5) ? part[lane] : 0.0f;
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     return v;
 }
 
-constexpr int norm_threads(int tpr) { return tpr == 32 ? 256 : tpr; }
+// How a row is cut into chunks of 8 elements per thread.
+//   kAligned  every access of a chunk is aligned (the weights' too);
+//   kShifted  the rows of all operands start at the same distance `phase` past an 8-element boundary (any width,
+//             contiguous operands): the chunks start `phase` elements before the row, so that their accesses are
+//             aligned.  A row's first and last chunk are read whole where that stays inside the operand (the
+//             neighbours' elements are dropped) and stored element by element; weights by shifted quads;
+//   kStrided  anything else: a thread's elements lie a row's threads apart, so that the narrow accesses of a warp are neighbours.
+enum NormMode { kAligned, kShifted, kStrided };
 
-// Element i (0..7) of a thread's chunk v: eight neighbours (VEC), or a stride of TPR so that the narrow
-// accesses of a warp stay next to each other.
-template <int TPR, bool VEC>
-__device__ __forceinline__ int norm_col(int v, int i, int tid) {
-    return VEC ? (v * TPR + tid) * 8 + i : (v * 8 + i) * TPR + tid;
+template <int TPR, int MODE>
+__device__ __forceinline__ int norm_col(int v, int i, int tid, int phase) {
+    const int n = row_threads<TPR>();
+    if (MODE == kStrided) return (v * 8 + i) * n + tid;
+    return (v * n + tid) * 8 + i - (MODE == kShifted ? phase : 0);
 }
 
-template <int TPR, bool VEC>
-__device__ __forceinline__ void norm_load(const void* p, int dtype, int64_t row0, int v, int tid, int d, float (&o)[8]) {
-    if (VEC) {
-        const int c = norm_col<TPR, true>(v, 0, tid);
-        if (c < d) {
-            ld8(p, dtype, row0 + c, o);
-            return;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = 0.0f;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = norm_col<TPR, false>(v, i, tid);
-            o[i] = c < d ? ld1(p, dtype, row0 + c) : 0.0f;
-        }
+// One chunk of row `row` (row stride ld) of an operand of m rows; outside the row: zeros.
+template <int TPR, int MODE>
+__device__ __forceinline__ void norm_load(const void* p, int dtype, int64_t row, int64_t ld, int v, int tid,
+                                          const NormParams& q, int phase, float (&o)[8]) {
+    const int c0 = norm_col<TPR, MODE>(v, 0, tid, phase), d = q.d;
+    const int64_t at = row * ld + c0;
+    if (MODE != kStrided && (MODE == kAligned ? c0 < d : c0 >= 0 && c0 + 8 <= d)) {
+        ld8(p, dtype, at, o);
+        return;
     }
-}
-
-template <int TPR, bool VEC>
-__device__ __forceinline__ void norm_store(void* p, int dtype, int64_t row0, int v, int tid, int d, const float (&o)[8]) {
-    if (VEC) {
-        const int c = norm_col<TPR, true>(v, 0, tid);
-        if (c < d) st8(p, dtype, row0 + c, o);
-    } else {
+    if (MODE == kShifted && c0 < d && at >= 0 && at + 8 <= (q.m - 1) * ld + d) {
+        ld8(p, dtype, at, o);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int c = norm_col<TPR, false>(v, i, tid);
-            if (c < d) w4_store(p, dtype, row0 + c, o[i]);
-        }
+        for (int i = 0; i < 8; ++i)
+            if ((unsigned)(c0 + i) >= (unsigned)d) o[i] = 0.0f;
+        return;
     }
-}
-
-// The gated branch of one chunk added to the scaled residual: o = a * r + b * act(gate) * (y * inv * w_post).
-template <int TPR, bool VEC>
-__device__ __forceinline__ void norm_combine(const NormParams& p, int64_t row, int v, int tid, float inv,
-                                             const float (&y)[8], const float (&r)[8], float (&o)[8]) {
-    float w[8], g[8];
-    if (p.w_post) norm_load<TPR, VEC>(p.w_post, SBQ_F32, 0, v, tid, p.d, w);
-    if (p.gate && p.gcol) norm_load<TPR, VEC>(p.gate, p.g_dtype, row * p.ldg, v, tid, p.d, g);
-    const float g0 = p.gate && !p.gcol ? ld1(p.gate, p.g_dtype, row * p.ldg) : 0.0f;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        float h = 0.0f;
-        if (p.y) {
-            h = y[i];
-            if (p.w_post) h = h * inv * w[i];
-            if (p.gate) h *= gate_act(p.gcol ? g[i] : g0, p.act);
-            h *= p.b;
-        }
-        o[i] = p.y ? fmaf(p.a, r[i], h) : p.a * r[i];
+        const int c = norm_col<TPR, MODE>(v, i, tid, phase);
+        o[i] = MODE != kAligned && (unsigned)c < (unsigned)d ? ld1(p, dtype, row * ld + c) : 0.0f;
     }
 }
 
-// One row per TPR threads, V chunks of 8 elements per thread.
-template <int TPR, int V, bool VEC>
-__global__ void __launch_bounds__(norm_threads(TPR)) norm_kernel(const NormParams p) {
+// The same of a vector [d].
+template <int TPR, int MODE>
+__device__ __forceinline__ void norm_load_vec(const void* p, int dtype, int v, int tid, int d, int phase, float (&o)[8]) {
+    const int c0 = norm_col<TPR, MODE>(v, 0, tid, phase);
+    if (MODE == kAligned && c0 < d) {
+        ld8(p, dtype, c0, o);
+        return;
+    }
+    if (MODE == kShifted && c0 >= 0 && c0 + 8 <= d && dtype == SBQ_F32 && !(reinterpret_cast<uintptr_t>(p) & 15)) {
+        ld8_weight(static_cast<const float*>(p), c0, d, o);
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int c = norm_col<TPR, MODE>(v, i, tid, phase);
+        o[i] = MODE != kAligned && (unsigned)c < (unsigned)d ? ld1(p, dtype, c) : 0.0f;
+    }
+}
+
+template <int TPR, int MODE>
+__device__ __forceinline__ void norm_store(void* p, int dtype, int64_t row0, int v, int tid, int d, int phase,
+                                           const float (&o)[8]) {
+    const int c0 = norm_col<TPR, MODE>(v, 0, tid, phase);
+    if (MODE == kStrided) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int c = norm_col<TPR, MODE>(v, i, tid, phase);
+            if (c < d) w4_store(p, dtype, row0 + c, o[i]);
+        }
+    } else if (MODE == kAligned ? c0 < d : c0 >= 0 && c0 + 8 <= d) {
+        st8(p, dtype, row0 + c0, o);
+    } else if (MODE == kShifted && c0 < d) {
+        st8_some(p, dtype, row0 + c0, c0 < 0 ? -c0 : 0, d - c0 < 8 ? d - c0 : 8, o);
+    }
+}
+
+template <int MODE>
+__device__ __forceinline__ int norm_phase(const NormParams& p, int64_t row) {
+    return MODE == kShifted ? (int)((row * p.ldr) & 7) : 0;
+}
+
+// The gate of one chunk, before its activation.
+template <int TPR, int MODE>
+__device__ __forceinline__ void norm_gate(const NormParams& p, int64_t row, int v, int tid, int phase, float (&g)[8]) {
+    if (!p.gcol) {
+        const float g0 = ld1(p.gate, p.g_dtype, row * p.ldg);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) g[i] = g0;
+    } else if (p.ldg) {
+        norm_load<TPR, MODE>(p.gate, p.g_dtype, row, p.ldg, v, tid, p, phase, g);
+    } else {
+        norm_load_vec<TPR, MODE>(p.gate, p.g_dtype, v, tid, p.d, phase, g);
+    }
+}
+
+// One chunk: r = a * r + b * act(g) * (y * inv * w_post).
+template <int TPR, int MODE, bool GATE>
+__device__ __forceinline__ void norm_combine(const NormParams& p, int v, int tid, int phase, float inv, float (&y)[8],
+                                             float (&g)[8], float (&r)[8]) {
+    if (!p.y) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] *= p.a;
+        return;
+    }
+    if (p.w_post) {
+        float w[8];
+        norm_load_vec<TPR, MODE>(p.w_post, SBQ_F32, v, tid, p.d, phase, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] = y[i] * inv * w[i];
+    }
+    if (GATE) {
+        gate_act8(g, p.act);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= g[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) r[i] = fmaf(p.a, r[i], p.b * y[i]);
+}
+
+// Columns of a chunk outside the row were loaded as zeros and stay zeros.
+__device__ __forceinline__ float square8(const float (&r)[8], float ss) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) ss = fmaf(r[i], r[i], ss);
+    return ss;
+}
+
+// V chunks of 8 elements per thread, everything a row needs from memory (but the weights) requested at the start.
+template <int TPR, int V, int MAXT, int MODE, bool GATE>
+__global__ void __launch_bounds__(MAXT) norm_kernel(const NormParams p) {
     __shared__ float part[2][32];
-    const int tid = TPR == 32 ? (int)(threadIdx.x & 31) : (int)threadIdx.x;
-    const int64_t row = TPR == 32 ? (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5) : (int64_t)blockIdx.x;
+    const int n = row_threads<TPR>(), tid = (int)threadIdx.x % n;
+    const int64_t first = TPR ? (int64_t)blockIdx.x * (MAXT / (TPR ? TPR : 1)) + threadIdx.x / n : (int64_t)blockIdx.x;
+    // rows that share a warp go on together: one past the end repeats the last row and stores nothing
+    const bool live = first < p.m;
+    const int64_t row = live ? first : p.m - 1;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (row >= p.m) return;  // whole warps; with TPR > 32 there is one row per CTA
-    float y[V][8], r[V][8];
+    const int phase = norm_phase<MODE>(p, row);
+    float y[V][8], r[V][8], g[GATE ? V : 1][8];
     float ss = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        if (p.y) norm_load<TPR, VEC>(p.y, p.y_dtype, row * p.ldy, v, tid, p.d, y[v]);
-        norm_load<TPR, VEC>(p.r, p.r_dtype, row * p.ldr, v, tid, p.d, r[v]);
+        if (p.y) norm_load<TPR, MODE>(p.y, p.y_dtype, row, p.ldy, v, tid, p, phase, y[v]);
+        norm_load<TPR, MODE>(p.r, p.r_dtype, row, p.ldr, v, tid, p, phase, r[v]);
+        if (GATE) norm_gate<TPR, MODE>(p, row, v, tid, phase, g[GATE ? v : 0]);
     }
     float inv = 1.0f;
     if (p.y && p.w_post) {
 #pragma unroll
-        for (int v = 0; v < V; ++v)
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(y[v][i], y[v][i], ss);
+        for (int v = 0; v < V; ++v) ss = square8(y[v], ss);
         inv = rsqrtf(row_sum<TPR>(ss, part[0]) / (float)p.d + p.eps);
     }
     ss = 0.0f;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        float o[8];
-        norm_combine<TPR, VEC>(p, row, v, tid, inv, y[v], r[v], o);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            r[v][i] = norm_col<TPR, VEC>(v, i, tid) < p.d ? o[i] : 0.0f;
-            ss = fmaf(r[v][i], r[v][i], ss);
-        }
-        if (p.r_out) norm_store<TPR, VEC>(p.r_out, p.r_dtype, row * p.ldro, v, tid, p.d, r[v]);
+        norm_combine<TPR, MODE, GATE>(p, v, tid, phase, inv, y[v], g[GATE ? v : 0], r[v]);
+        ss = square8(r[v], ss);
+        if (p.r_out && live) norm_store<TPR, MODE>(p.r_out, p.r_dtype, row * p.ldro, v, tid, p.d, phase, r[v]);
     }
     if (!p.x) return;
     inv = rsqrtf(row_sum<TPR>(ss, part[1]) / (float)p.d + p.eps);
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        float w[8], o[8];
-        norm_load<TPR, VEC>(p.w_pre, SBQ_F32, 0, v, tid, p.d, w);
+        float w[8];
+        norm_load_vec<TPR, MODE>(p.w_pre, SBQ_F32, v, tid, p.d, phase, w);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) o[i] = r[v][i] * inv * w[i];
-        norm_store<TPR, VEC>(p.x, p.x_dtype, row * p.ldx, v, tid, p.d, o);
+        for (int i = 0; i < 8; ++i) r[v][i] = r[v][i] * inv * w[i];
+        if (live) norm_store<TPR, MODE>(p.x, p.x_dtype, row * p.ldx, v, tid, p.d, phase, r[v]);
     }
 }
 
 // Rows longer than the registers of one CTA: the row is read again for each statistic (from L2), and
 // nothing is written before the last pass, so r_out may be r and x may be y.
-constexpr int kLongTpr = 512;
-template <bool VEC>
-__global__ void __launch_bounds__(kLongTpr) norm_long_kernel(const NormParams p) {
+constexpr int kLongThreads = 512;
+template <int MODE, bool GATE>
+__global__ void __launch_bounds__(kLongThreads) norm_long_kernel(const NormParams p) {
     __shared__ float part[2][32];
     const int tid = threadIdx.x;
     const int64_t row = blockIdx.x;
-    const int chunks = (p.d + kLongTpr * 8 - 1) / (kLongTpr * 8);
+    const int phase = norm_phase<MODE>(p, row), chunks = (p.d + phase + kLongThreads * 8 - 1) / (kLongThreads * 8);
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    float y[8], r[8], o[8], inv = 1.0f, ss = 0.0f;
+    float y[8], r[8], g[8], inv = 1.0f, ss = 0.0f;
     if (p.y && p.w_post) {
         for (int v = 0; v < chunks; ++v) {
-            norm_load<kLongTpr, VEC>(p.y, p.y_dtype, row * p.ldy, v, tid, p.d, y);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) ss = fmaf(y[i], y[i], ss);
+            norm_load<0, MODE>(p.y, p.y_dtype, row, p.ldy, v, tid, p, phase, y);
+            ss = square8(y, ss);
         }
-        inv = rsqrtf(row_sum<kLongTpr>(ss, part[0]) / (float)p.d + p.eps);
+        inv = rsqrtf(row_sum<0>(ss, part[0]) / (float)p.d + p.eps);
     }
     float inv2 = 1.0f;
     for (int pass = p.x ? 0 : 1; pass < 2; ++pass) {
         ss = 0.0f;
         for (int v = 0; v < chunks; ++v) {
-            if (p.y) norm_load<kLongTpr, VEC>(p.y, p.y_dtype, row * p.ldy, v, tid, p.d, y);
-            norm_load<kLongTpr, VEC>(p.r, p.r_dtype, row * p.ldr, v, tid, p.d, r);
-            norm_combine<kLongTpr, VEC>(p, row, v, tid, inv, y, r, o);
+            if (p.y) norm_load<0, MODE>(p.y, p.y_dtype, row, p.ldy, v, tid, p, phase, y);
+            norm_load<0, MODE>(p.r, p.r_dtype, row, p.ldr, v, tid, p, phase, r);
+            if (GATE) norm_gate<0, MODE>(p, row, v, tid, phase, g);
+            norm_combine<0, MODE, GATE>(p, v, tid, phase, inv, y, g, r);
             if (pass == 0) {
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (norm_col<kLongTpr, VEC>(v, i, tid) < p.d) ss = fmaf(o[i], o[i], ss);
+                ss = square8(r, ss);
             } else {
-                if (p.r_out) norm_store<kLongTpr, VEC>(p.r_out, p.r_dtype, row * p.ldro, v, tid, p.d, o);
+                if (p.r_out) norm_store<0, MODE>(p.r_out, p.r_dtype, row * p.ldro, v, tid, p.d, phase, r);
                 if (p.x) {
-                    norm_load<kLongTpr, VEC>(p.w_pre, SBQ_F32, 0, v, tid, p.d, r);
+                    norm_load_vec<0, MODE>(p.w_pre, SBQ_F32, v, tid, p.d, phase, y);
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) o[i] = o[i] * inv2 * r[i];
-                    norm_store<kLongTpr, VEC>(p.x, p.x_dtype, row * p.ldx, v, tid, p.d, o);
+                    for (int i = 0; i < 8; ++i) r[i] = r[i] * inv2 * y[i];
+                    norm_store<0, MODE>(p.x, p.x_dtype, row * p.ldx, v, tid, p.d, phase, r);
                 }
             }
         }
-        if (pass == 0) inv2 = rsqrtf(row_sum<kLongTpr>(ss, part[1]) / (float)p.d + p.eps);
+        if (pass == 0) inv2 = rsqrtf(row_sum<0>(ss, part[1]) / (float)p.d + p.eps);
     }
 }
 
-template <int TPR, int V>
-static cudaError_t launch_norm(const NormParams& p, bool vec, cudaStream_t s) {
-    const unsigned grid = (unsigned)(TPR == 32 ? ceil_div(p.m, 8) : p.m);
-    return vec ? w4_launch(norm_kernel<TPR, V, true>, grid, norm_threads(TPR), 0, s, p)
-               : w4_launch(norm_kernel<TPR, V, false>, grid, norm_threads(TPR), 0, s, p);
+// TPR = 0: `threads` for each row; otherwise 256 threads for 256 / TPR rows.
+template <int TPR, int V, int MAXT, int MODE>
+static cudaError_t launch_norm_m(const NormParams& p, int threads, cudaStream_t s) {
+    const unsigned grid = (unsigned)(TPR ? ceil_div(p.m, MAXT / (TPR ? TPR : 1)) : p.m);
+    return p.gate ? w4_launch(norm_kernel<TPR, V, MAXT, MODE, true>, grid, (unsigned)threads, 0, s, p)
+                  : w4_launch(norm_kernel<TPR, V, MAXT, MODE, false>, grid, (unsigned)threads, 0, s, p);
 }
 
-template <int V>
-static cudaError_t launch_norm_v(const NormParams& p, bool vec, cudaStream_t s) {
-    if (p.d <= 256 * V) return launch_norm<32, V>(p, vec, s);
-    if (p.d <= 512 * V) return launch_norm<64, V>(p, vec, s);
-    if (p.d <= 1024 * V) return launch_norm<128, V>(p, vec, s);
-    if (p.d <= 2048 * V) return launch_norm<256, V>(p, vec, s);
-    if (p.d <= 4096 * V) return launch_norm<512, V>(p, vec, s);
-    return vec ? w4_launch(norm_long_kernel<true>, (unsigned)p.m, kLongTpr, 0, s, p)
-               : w4_launch(norm_long_kernel<false>, (unsigned)p.m, kLongTpr, 0, s, p);
+template <int TPR, int V, int MAXT>
+static cudaError_t launch_norm(const NormParams& p, int mode, int threads, cudaStream_t s) {
+    if (mode == kAligned) return launch_norm_m<TPR, V, MAXT, kAligned>(p, threads, s);
+    if (mode == kShifted) return launch_norm_m<TPR, V, MAXT, kShifted>(p, threads, s);
+    return launch_norm_m<TPR, V, MAXT, kStrided>(p, threads, s);
+}
+
+template <int MODE>
+static cudaError_t launch_norm_long(const NormParams& p, cudaStream_t s) {
+    return p.gate ? w4_launch(norm_long_kernel<MODE, true>, (unsigned)p.m, kLongThreads, 0, s, p)
+                  : w4_launch(norm_long_kernel<MODE, false>, (unsigned)p.m, kLongThreads, 0, s, p);
+}
+
+// Chunks per thread by the row's width: one up to 1024 columns, and while there are no more rows than SMs (more threads
+// on each); two above, which leaves more loads in flight per thread.  Measured on B200, one and two chunks:
+// 100000 x 128 56 and 91 us, 16384 x 1024 45 and 49 us, 8192 x 4096 99 and 88 us.
+static cudaError_t launch_norm_any(const NormParams& p, int mode, cudaStream_t s) {
+    const int span = p.d + (mode == kShifted ? 7 : 0);
+    if (span <= 64) return launch_norm<8, 1, 256>(p, mode, 256, s);
+    if (span <= 128) return launch_norm<16, 1, 256>(p, mode, 256, s);
+    if (span <= 256) return launch_norm<32, 1, 256>(p, mode, 256, s);
+    const int one = (span + 255) / 256 * 32, two = (span + 511) / 512 * 32;  // threads for one or two chunks each
+    if (one <= 1024 && (span <= 1024 || p.m <= w4_sm_count())) return launch_norm<0, 1, 1024>(p, mode, one, s);
+    if (two <= 512) return launch_norm<0, 2, 512>(p, mode, two, s);
+    if (two <= 1024) return launch_norm<0, 2, 1024>(p, mode, two, s);
+    if (mode == kAligned) return launch_norm_long<kAligned>(p, s);
+    if (mode == kShifted) return launch_norm_long<kShifted>(p, s);
+    return launch_norm_long<kStrided>(p, s);
 }
 
 static bool norm_dtype(int t) { return t == SBQ_F32 || t == SBQ_F16 || t == SBQ_BF16; }
 
-// One operand: its type, stride and element alignment; *vec stays true while 8-element accesses are aligned.
-static int check_operand(const void* p, int dtype, int64_t ld, int64_t width, int64_t m, const char* what, bool* vec) {
+// What the operands' addresses allow: `aligned` 8-element accesses in every row, or rows that all start at the same
+// distance past an 8-element boundary (`shifted`; `step`: their stride modulo 8, -1 before the first operand).
+struct NormLayout {
+    bool aligned = true, shifted = true;
+    int step = -1;
+};
+
+// One operand: its type, stride and element alignment.  rows: whether it has m rows of d elements (else a vector).
+static int check_operand(const void* p, int dtype, int64_t ld, int64_t width, int64_t m, const char* what, NormLayout* l,
+                         bool rows) {
     if (!norm_dtype(dtype)) return set_error(SBQ_ERR_UNSUPPORTED, "%s dtype %d (f32, f16, bf16)", what, dtype);
     const int es = w4_elem(dtype);
     if (reinterpret_cast<uintptr_t>(p) % es) return set_error(SBQ_ERR_ALIGNMENT, "%s must be aligned to its element size", what);
     if (m > 1 && ld < width) return set_error(SBQ_ERR_INVALID_ARGUMENT, "%s row stride smaller than the row", what);
-    if (reinterpret_cast<uintptr_t>(p) % 16 || (m > 1 && (ld * es) % 16)) *vec = false;
+    if (reinterpret_cast<uintptr_t>(p) % 16 || (m > 1 && (ld * es) % 16)) l->aligned = false;
+    if (rows) {
+        const int step = m > 1 ? (int)(ld & 7) : 0;
+        if (reinterpret_cast<uintptr_t>(p) % 16 || (l->step >= 0 && l->step != step)) l->shifted = false;
+        l->step = step;
+    }
     return SBQ_OK;
 }
 
@@ -305,23 +477,24 @@ extern "C" int sbq_residual_norm(const sbq_residual_norm_args* a, void* stream) 
     if (a->gate_mode != SBQ_GATE_PER_COLUMN && a->gate_mode != SBQ_GATE_PER_ROW && a->gate_mode != SBQ_GATE_FULL)
         return set_error(SBQ_ERR_UNSUPPORTED, "gate mode %d", a->gate_mode);
     if (!(a->eps >= 0.0f)) return set_error(SBQ_ERR_INVALID_ARGUMENT, "eps must not be negative");
-    bool vec = d % 8 == 0;
+    NormLayout l;
+    l.aligned = d % 8 == 0;
     NormParams p{};
-    int st = check_operand(a->residual, a->residual_dtype, a->ld_residual, d, m, "residual", &vec);
-    if (!st && a->branch) st = check_operand(a->branch, a->branch_dtype, a->ld_branch, d, m, "branch", &vec);
+    int st = check_operand(a->residual, a->residual_dtype, a->ld_residual, d, m, "residual", &l, true);
+    if (!st && a->branch) st = check_operand(a->branch, a->branch_dtype, a->ld_branch, d, m, "branch", &l, true);
     if (!st && a->residual_out)
-        st = check_operand(a->residual_out, a->residual_dtype, a->ld_residual_out, d, m, "residual output", &vec);
-    if (!st && a->out) st = check_operand(a->out, a->out_dtype, a->ld_out, d, m, "output", &vec);
-    if (!st && a->gate && a->gate_mode == SBQ_GATE_FULL)
-        st = check_operand(a->gate, a->gate_dtype, a->ld_gate, d, m, "gate", &vec);
-    else if (!st && a->gate) {
-        bool row_vec = true;
-        st = check_operand(a->gate, a->gate_dtype, a->ld_gate, 0, 1, "gate", &row_vec);
-        if (a->gate_mode == SBQ_GATE_PER_COLUMN) vec = vec && row_vec;
+        st = check_operand(a->residual_out, a->residual_dtype, a->ld_residual_out, d, m, "residual output", &l, true);
+    if (!st && a->out) st = check_operand(a->out, a->out_dtype, a->ld_out, d, m, "output", &l, true);
+    if (!st && a->gate) {
+        NormLayout any;  // one gate per row sets no condition
+        const bool full = a->gate_mode == SBQ_GATE_FULL;
+        st = check_operand(a->gate, a->gate_dtype, a->ld_gate, full ? d : 0, full ? m : 1, "gate",
+                           a->gate_mode == SBQ_GATE_PER_ROW ? &any : &l, full);
     }
-    if (!st && a->pre_weight) st = check_operand(a->pre_weight, SBQ_F32, d, d, 1, "pre_weight", &vec);
-    if (!st && a->post_weight) st = check_operand(a->post_weight, SBQ_F32, d, d, 1, "post_weight", &vec);
+    if (!st && a->pre_weight) st = check_operand(a->pre_weight, SBQ_F32, d, d, 1, "pre_weight", &l, false);
+    if (!st && a->post_weight) st = check_operand(a->post_weight, SBQ_F32, d, d, 1, "post_weight", &l, false);
     if (st) return st;
+    const int mode = l.aligned ? kAligned : l.shifted ? kShifted : kStrided;
     p.y = a->branch, p.r = a->residual, p.gate = a->gate, p.w_post = a->post_weight, p.w_pre = a->pre_weight;
     p.r_out = a->residual_out, p.x = a->out;
     p.ldy = a->ld_branch, p.ldr = a->ld_residual, p.ldro = a->ld_residual_out, p.ldx = a->ld_out;
@@ -331,8 +504,7 @@ extern "C" int sbq_residual_norm(const sbq_residual_norm_args* a, void* stream) 
     p.act = a->gate_act, p.a = a->residual_scale, p.b = a->branch_scale, p.eps = a->eps;
     p.m = m, p.d = (int)d;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    // one chunk per thread while there are fewer rows than SMs (more threads on each row), else two
-    const cudaError_t e = m <= w4_sm_count() ? launch_norm_v<1>(p, vec, s) : launch_norm_v<2>(p, vec, s);
+    const cudaError_t e = launch_norm_any(p, mode, s);
     if (e != cudaSuccess) return set_error(SBQ_ERR_CUDA, "residual_norm launch: %s", cudaGetErrorString(e));
     return check_launch("residual_norm");
 }

@@ -124,8 +124,11 @@ def test_in_place_and_strides(sbq, d):
         yv = rows[:, 8:8 + d]
         wide[1:m + 1, 8:8 + d] = r
         got_r, got_x = sbq.residual_norm(yv, wide[1:m + 1, 8:8 + d], w, residual_out=wide[1:m + 1, 8:8 + d])
-        want_r, want_x = sbq.residual_norm(yv.contiguous(), r, w)
-        assert torch.equal(got_r, want_r) and torch.equal(got_x, want_x)
+        # r' has no sum in it here; x has one, whose order follows the layout of the rows: any order is within the
+        # bound of a chain of these additions, and need not equal another
+        assert torch.equal(got_r, sbq.residual_norm(yv.contiguous(), r, w)[0])
+        _, want_x, _, err_x = reference(yv, r, w, None, None, "none", 1.0, 1.0, 1e-6)
+        check(got_x, want_x, err_x)
         wide[1:m + 1, 8:8 + d] = 3.0
         assert (wide == 3.0).all()
         # addresses off by one element take the narrow accesses
