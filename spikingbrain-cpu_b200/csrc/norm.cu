@@ -415,17 +415,15 @@ static cudaError_t launch_norm_long(const NormParams& p, cudaStream_t s) {
                   : w4_launch(norm_long_kernel<MODE, false>, (unsigned)p.m, kLongThreads, 0, s, p);
 }
 
-// Chunks per thread by the row's width: one up to 1024 columns, and while there are no more rows than SMs (more threads
-// on each); two above, which leaves more loads in flight per thread.  Measured on B200, one and two chunks:
-// 100000 x 128 56 and 91 us, 16384 x 1024 45 and 49 us, 8192 x 4096 99 and 88 us.
+// One chunk per thread up to 8192 columns (1024 threads), on as many warps as the row fills.  Measured on B200, one and
+// two chunks: 8192 x 4096 with both norms 75 and 78 us, gated 3001 x 2560 26 and 31 us, 3001 x 2559 38 and 53 us.
 static cudaError_t launch_norm_any(const NormParams& p, int mode, cudaStream_t s) {
     const int span = p.d + (mode == kShifted ? 7 : 0);
     if (span <= 64) return launch_norm<8, 1, 256>(p, mode, 256, s);
     if (span <= 128) return launch_norm<16, 1, 256>(p, mode, 256, s);
     if (span <= 256) return launch_norm<32, 1, 256>(p, mode, 256, s);
     const int one = (span + 255) / 256 * 32, two = (span + 511) / 512 * 32;  // threads for one or two chunks each
-    if (one <= 1024 && (span <= 1024 || p.m <= w4_sm_count())) return launch_norm<0, 1, 1024>(p, mode, one, s);
-    if (two <= 512) return launch_norm<0, 2, 512>(p, mode, two, s);
+    if (one <= 1024) return launch_norm<0, 1, 1024>(p, mode, one, s);
     if (two <= 1024) return launch_norm<0, 2, 1024>(p, mode, two, s);
     if (mode == kAligned) return launch_norm_long<kAligned>(p, s);
     if (mode == kShifted) return launch_norm_long<kShifted>(p, s);
