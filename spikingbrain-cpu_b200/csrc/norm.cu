@@ -308,7 +308,7 @@ __device__ __forceinline__ float square8(const float (&r)[8], float ss) {
 
 // V chunks of 8 elements per thread, everything a row needs from memory (but the weights) requested at the start.
 template <int TPR, int V, int MAXT, int MODE, bool GATE>
-__global__ void __launch_bounds__(MAXT) norm_kernel(const NormParams p) {
+__global__ void __launch_bounds__(MAXT, MAXT == 512 ? (MODE == kAligned ? 4 : 3) : 1) norm_kernel(const NormParams p) {
     __shared__ float part[2][32];
     const int n = row_threads<TPR>(), tid = (int)threadIdx.x % n;
     const int64_t first = TPR ? (int64_t)blockIdx.x * (MAXT / (TPR ? TPR : 1)) + threadIdx.x / n : (int64_t)blockIdx.x;
@@ -417,12 +417,16 @@ static cudaError_t launch_norm_long(const NormParams& p, cudaStream_t s) {
 
 // One chunk per thread up to 8192 columns (1024 threads), on as many warps as the row fills.  Measured on B200, one and
 // two chunks: 8192 x 4096 with both norms 75 and 78 us, gated 3001 x 2560 26 and 31 us, 3001 x 2559 38 and 53 us.
+// What hides a row's chain of loads and sums is other rows on the SM: 32 registers per thread (40 for the
+// shifted accesses, which spill at 32) took the gated cases to 22 and 36 us; weights requested early, or
+// persistent CTAs that request their next row early, cost registers and were slower.
 static cudaError_t launch_norm_any(const NormParams& p, int mode, cudaStream_t s) {
     const int span = p.d + (mode == kShifted ? 7 : 0);
     if (span <= 64) return launch_norm<8, 1, 256>(p, mode, 256, s);
     if (span <= 128) return launch_norm<16, 1, 256>(p, mode, 256, s);
     if (span <= 256) return launch_norm<32, 1, 256>(p, mode, 256, s);
     const int one = (span + 255) / 256 * 32, two = (span + 511) / 512 * 32;  // threads for one or two chunks each
+    if (one <= 512) return launch_norm<0, 1, 512>(p, mode, one, s);
     if (one <= 1024) return launch_norm<0, 1, 1024>(p, mode, one, s);
     if (two <= 1024) return launch_norm<0, 2, 1024>(p, mode, two, s);
     if (mode == kAligned) return launch_norm_long<kAligned>(p, s);
