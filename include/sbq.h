@@ -388,15 +388,15 @@ SBQ_API int sbq_w4_pack(const int8_t* q, int64_t ldq, const void* scale, int64_t
 SBQ_API int sbq_w4_unpack(const void* packed, const void* scales, int64_t n, int64_t k, int group, int8_t* q,
                           int64_t ldq, void* scale, int64_t lds, void* stream);
 
-/* Workspace of sbq_linear_w4 (matrices = 1) / sbq_mlp_gateup_w4 (2) on the current device: the activation's
- * fp16 parts (fp32 x at every m, bf16 x above 16 rows) and, above 128 rows, the partial sums of tiles that are
- * cut along k.  Its contents need not be kept between calls. */
+/* Workspace of sbq_linear_w4 (matrices = 1) / sbq_mlp_gateup_w4 (2) on the current device: the activation where it
+ * is not read in place (fp32 x, bf16 x above 16 rows, k not a multiple of 16) and, above 128 rows, the partial
+ * sums of tiles that are cut along k.  Its contents need not be kept between calls. */
 SBQ_API size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_dtype, int matrices);
 
 /* y[m, n] = sum_k x[m, k] * q[n, k] * s[n, k / group] (+ bias[n]); x and y SBQ_F32, SBQ_F16 or SBQ_BF16.
- * q * s enters the product exactly, bf16 x too, fp32 x with 22 bits; sums are fp32.  Up to 16 rows: the
- * decode product; above: the tensor-memory product.  k a multiple of 16 (zero-fill x past the weight's own
- * k), x rows 16-byte aligned, workspace 256-byte aligned (NULL when its size is 0). */
+ * q * s enters the product exactly, 16-bit x too, fp32 x with 22 bits; sums are fp32.  Up to 16 rows: the
+ * decode product; above: the tensor-memory product.  x rows 16-byte aligned when k is a multiple of 16 (any row stride
+ * otherwise), workspace 256-byte aligned (NULL when its size is 0). */
 SBQ_API int sbq_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* packed, const void* scales,
                           const float* rowmul, int group, const float* bias, int64_t m, int64_t n, int64_t k, void* y,
                           int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);

@@ -13,7 +13,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .quant import (_DTYPE_CODE, Int4Linear, Int8Linear, _in_place, _int4_workspace, _prepare_x, _ptr, _raw_stream, _stream,
+from .quant import (_DTYPE_CODE, Int4Linear, Int8Linear, _in_place, _int4_rows, _int4_workspace, _prepare_x, _ptr, _raw_stream, _stream,
                     _workspace)
 
 
@@ -45,11 +45,18 @@ class FusedGatedMLP(nn.Module):
             raise RuntimeError("a sharded FusedGatedMLP needs the gather between gate/up and down; use the stack")
         shape = x.shape
         dev = self.gate_proj.packed.device
-        x2, k16, on_host = _prepare_x(x, self.gate_proj.in_features, dev)
+        x2, on_host = self._rows(x, dev)
         m, n = x2.shape[0], self.gate_proj.out_features
         h = self.gateup_into(x2, torch.empty(m, n, dtype=self.h_dtype, device=dev))
         y = self.down_proj(h).reshape(*shape[:-1], self.down_proj.out_features)
         return y.to("cpu") if on_host else y
+
+    def _rows(self, x: torch.Tensor, dev: torch.device):
+        """(rows of x as the kernels take them, whether x came from the host)."""
+        if self.int4:
+            return _int4_rows(x, self.gate_proj.in_features, dev)
+        x2, _, on_host = _prepare_x(x, self.gate_proj.in_features, dev)
+        return x2, on_host
 
     def gateup(self, x: torch.Tensor) -> torch.Tensor:
         """The hidden activation alone: silu(gate(x)) * up(x) in ``h_dtype``, x as ``forward`` takes it."""
@@ -59,7 +66,7 @@ class FusedGatedMLP(nn.Module):
             h = torch.empty((*x.shape[:-1], n), dtype=self.h_dtype, device=dev)
             self._run_int4(x, x.numel() // k, k, k, h, n, dev)
             return h
-        x2, _, on_host = _prepare_x(x, k, dev)
+        x2, on_host = self._rows(x, dev)
         h = self.gateup_into(x2, torch.empty(x2.shape[0], n, dtype=self.h_dtype, device=dev)).view(*x.shape[:-1], n)
         return h.to("cpu") if on_host else h
 
@@ -75,7 +82,7 @@ class FusedGatedMLP(nn.Module):
     def gateup_into(self, x2: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
         """Low-level device call: silu(gate(x2)) * up(x2) into ``h`` [m, n] (fp16/fp32, unit column stride).
 
-        x2 is [m, k'] with 16-byte aligned rows (k' = in_features rounded up to 16).  The library
+        x2 is [m, k'] with 16-byte aligned rows (k' = in_features rounded up to 16; int4: in_features).  The library
         picks the kernel: the fused gate/up GEMV up to 16 rows; above, the gate GEMM into ``h`` and the
         up GEMM whose epilogue replaces it by silu(gate) * up (fp32 x split once into bf16 high / low
         parts in a workspace that both GEMMs read).
@@ -93,11 +100,11 @@ class FusedGatedMLP(nn.Module):
 
 
     def _gateup_int4(self, x2: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
-        m, n, k = x2.shape[0], self.gate_proj.out_features, (self.gate_proj.in_features + 15) // 16 * 16
+        m, n, k = x2.shape[0], self.gate_proj.out_features, self.gate_proj.in_features
         dev = self.gate_proj.packed.device
         if h.shape != (m, n) or (n > 1 and h.stride(1) != 1) or h.dtype not in _DTYPE_CODE or h.device != dev:
             raise ValueError("hidden activation must be an fp32/fp16/bf16 [%d, %d] view with unit column stride" % (m, n))
-        if x2.shape[1] != k or x2.stride(1) != 1 or x2.dtype not in _DTYPE_CODE or x2.device != dev:
+        if x2.shape[1] != k or (x2.stride(1) != 1 and k > 1) or x2.dtype not in _DTYPE_CODE or x2.device != dev:
             raise ValueError("input must be an fp32/fp16/bf16 [m, %d] view with unit column stride" % k)
         self._run_int4(x2, m, k, x2.stride(0) if m > 1 else k, h, h.stride(0) if m > 1 else n, dev)
         return h

@@ -406,9 +406,9 @@ def _raw_stream(device: torch.device) -> int:
 
 
 def _in_place(x: torch.Tensor, k: int, device: torch.device) -> bool:
-    """Whether the kernels can read x [..., k] where it is, as a decode loop passes it: no copy, no padding."""
-    return x.dtype in _DTYPE_CODE and x.shape[-1] == k and k % 16 == 0 and x.device == device and x.is_contiguous() \
-        and x.data_ptr() % 16 == 0
+    """Whether the library takes x [..., k] where it is, as a decode loop passes it."""
+    return x.dtype in _DTYPE_CODE and x.shape[-1] == k and x.device == device and x.is_contiguous() \
+        and (x.data_ptr() % 16 == 0 or k % 16 != 0)
 
 
 class Int4Linear(nn.Module):
@@ -500,18 +500,18 @@ class Int4Linear(nn.Module):
             dst.copy_(src)
 
     def forward_into(self, x2: torch.Tensor, out: torch.Tensor) -> torch.Tensor:
-        """Low-level device call: x2 [m, k'] (k' = in_features rounded up to 16, 16-byte aligned rows)
+        """Low-level device call: x2 [m, in_features] (16-byte aligned rows if in_features is a multiple of 16)
         into ``out`` [m, out_features] (fp32, fp16 or bf16, unit column stride, any row stride)."""
         m, n = x2.shape[0], self.out_features
         if out.shape != (m, n) or (out.stride(1) != 1 and n > 1) or out.dtype not in _DTYPE_CODE:
             raise ValueError("output must be an fp32/fp16/bf16 [%d, %d] view with unit column stride" % (m, n))
-        k16 = (self.in_features + 15) // 16 * 16
-        if x2.shape[1] != k16 or x2.stride(1) != 1 or x2.dtype not in _DTYPE_CODE:
-            raise ValueError("input must be an fp32/fp16/bf16 [m, %d] view with unit column stride" % k16)
+        k = self.in_features
+        if x2.shape[1] != k or (x2.stride(1) != 1 and k > 1) or x2.dtype not in _DTYPE_CODE:
+            raise ValueError("input must be an fp32/fp16/bf16 [m, %d] view with unit column stride" % k)
         dev = self._buffers["packed"].device
         if x2.device != dev or out.device != dev:
             raise ValueError("input and output must be on the weight's device %s" % dev)
-        self._run(x2, m, k16, x2.stride(0) if m > 1 else k16, out, out.stride(0) if m > 1 else n, dev)
+        self._run(x2, m, k, x2.stride(0) if m > 1 else k, out, out.stride(0) if m > 1 else n, dev)
         return out
 
     def _run(self, x: torch.Tensor, m: int, k: int, ldx: int, out: torch.Tensor, ldy: int, dev: torch.device) -> None:
@@ -535,9 +535,8 @@ class Int4Linear(nn.Module):
             out = torch.empty((*x.shape[:-1], n), dtype=self.out_dtype, device=dev)
             self._run(x, x.numel() // k, k, k, out, n, dev)
             return out
-        x2, k16, on_host = _prepare_x(x, k, dev)
-        out = torch.empty(x2.shape[0], n, dtype=self.out_dtype, device=dev)
-        self.forward_into(x2, out)
+        x2, on_host = _int4_rows(x, k, dev)
+        out = self.forward_into(x2, torch.empty(x2.shape[0], n, dtype=self.out_dtype, device=dev))
         out = out.view(*x.shape[:-1], n)
         return out.to("cpu") if on_host else out
 
@@ -546,9 +545,24 @@ class Int4Linear(nn.Module):
                                                                        self.bias is not None, self.group)
 
 
+def _int4_rows(x: torch.Tensor, k: int, device: torch.device):
+    """x flattened to rows [m, k] as the 4-bit calls take them, and whether it came from the host."""
+    if x.dim() == 0 or x.shape[-1] != k:
+        raise ValueError("input feature size %s does not match the weight's %d" % (x.shape[-1] if x.dim() else "()", k))
+    on_host = x.device.type != "cuda"
+    xd = x if x.device == device else x.to(device, non_blocking=True)
+    if xd.dtype not in _DTYPE_CODE:
+        xd = xd.float()
+    x2 = xd.reshape(-1, k)
+    if x2.shape[0] and ((x2.stride(1) != 1 and k > 1) or (x2.shape[0] > 1 and x2.stride(0) < k) or
+                        (k % 16 == 0 and (x2.data_ptr() % 16 or (x2.shape[0] > 1 and x2.stride(0) * _ELEM[x2.dtype] % 16)))):
+        x2 = x2.contiguous() if x2.data_ptr() % 16 == 0 or not x2.is_contiguous() else x2.clone()
+    return x2, on_host
+
+
 def _int4_workspace(m: int, n: int, k: int, x_code: int, matrices: int, device: torch.device):
     """(tensor or None, bytes) of a 4-bit call's workspace, from torch's caching allocator."""
-    if m <= 16 and x_code != L.F32:
+    if m <= 16 and x_code != L.F32 and k % 16 == 0:
         return None, 0
     nbytes = L.load().sbq_linear_w4_workspace_bytes(m, n, k, x_code, matrices)
     return (torch.empty(nbytes, dtype=torch.uint8, device=device), nbytes) if nbytes else (None, 0)

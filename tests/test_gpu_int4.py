@@ -209,6 +209,25 @@ def test_strided_rows_and_untouched_surroundings(sbq, m):
     assert torch.equal(lin(x3), lin(x3.view(-1, 96)).view(2, m, 40))
 
 
+@pytest.mark.parametrize("m", [1, 12, 30, 140])
+@pytest.mark.parametrize("k", [1, 7, 64, 90, 333, 4100, 13001])
+def test_rows_at_any_address(sbq, m, k):
+    """Widths that are multiples of nothing, rows at odd distances and odd first addresses; what lies beside the rows
+    (infinities here) has no part in the result."""
+    q, s = weight(33, k, 32, seed=50)
+    lin = sbq.Int4Linear.from_quantized(q, s, None, group=32)
+    for x_dtype in (F16, BF16, F32):
+        wide = torch.full((m, k + 5), float("inf"), dtype=x_dtype, device="cuda")
+        x = acts(m, k, x_dtype, seed=51)
+        wide[:, 3:3 + k] = x
+        check(lin(wide[:, 3:3 + k]), x, q, s, 32)
+        flat = torch.full((m * k + 1,), float("inf"), dtype=x_dtype, device="cuda")
+        flat[1:] = x.flatten()
+        check(lin(flat[1:].view(m, k)), x, q, s, 32)
+        check(lin(x.t().contiguous().t()), x, q, s, 32)
+        check(lin(x[:1].expand(m, k)), x[:1].expand(m, k).contiguous(), q, s, 32)
+
+
 def test_empty_and_host_inputs(sbq):
     q, s = weight(24, 64, 64, seed=21)
     lin = sbq.Int4Linear.from_quantized(q, s, None, group=64)
@@ -330,6 +349,8 @@ def test_refusals(sbq):
         lin.forward_into(torch.zeros(2, 64, device="cuda"), torch.zeros(2, 31, device="cuda"))
     with pytest.raises(ValueError, match="input must be"):
         lin.forward_into(torch.zeros(2, 80, device="cuda")[:, :48], torch.zeros(2, 32, device="cuda"))
+    with pytest.raises(ValueError, match="ALIGNMENT"):
+        lin.forward_into(torch.zeros(2, 80, device="cuda")[:, 1:65], torch.zeros(2, 32, device="cuda"))
     with pytest.raises(ValueError, match="int4"):
         sbq.FusedGatedMLP(lin, sbq.Int8Linear(torch.zeros(32, 64), None), lin)
     with pytest.raises(ValueError, match="grouped decode"):
@@ -340,7 +361,7 @@ def test_refusals(sbq):
     args = [x.data_ptr(), L.F32, 64, lin.packed.data_ptr(), lin.scales.data_ptr(), lin.rowmul.data_ptr(), 32, None, 2, 32, 64,
             y.data_ptr(), L.F32, 32, None, 0, None]
     for at, value, name in ((14, None, "INVALID"), (0, x.data_ptr() + 4, "ALIGNMENT"), (1, 3, "UNSUPPORTED"), (6, 16, "UNSUPPORTED"),
-                            (10, 60, "UNSUPPORTED"), (13, 31, "INVALID"), (3, lin.packed.data_ptr() + 16, "ALIGNMENT")):
+                            (10, 72, "INVALID"), (13, 31, "INVALID"), (3, lin.packed.data_ptr() + 16, "ALIGNMENT")):
         bad = list(args)
         bad[at] = value
         with pytest.raises(ValueError, match=name):
