@@ -831,9 +831,10 @@ static int make_maps(W4Maps& m, const W4Call& c, const W4Acts& x, int x_rows, in
     return st;
 }
 
-template <class K>
-static cudaError_t launch_maps(K kernel, dim3 grid, int threads, int smem, int parts, cudaStream_t s, const W4Maps& m, const GemmW4Params& p) {
-    cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+template <auto kernel>
+static cudaError_t launch_maps(dim3 grid, int threads, int smem, int parts, cudaStream_t s, const W4Maps& m, const GemmW4Params& p) {
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = w4_allow_smem(kernel, smem, allowed);
     if (e != cudaSuccess) return e;
     cudaLaunchConfig_t cfg{};
     cfg.gridDim = grid;
@@ -856,10 +857,10 @@ template <int PARTS, int NMAT, int GPT>
 static cudaError_t launch_gemm_w4(int tok, int npairs, const W4Maps& m, GemmW4Params p, cudaStream_t s) {
     p.seg_blocks = p.y_dtype == SBQ_F32 ? kSegSteps / (8 * PARTS) : p.kt;
     if (tok == kSTok4)
-        return launch_maps(gemm_w4_small_kernel<PARTS, NMAT, GPT>,
+        return launch_maps<gemm_w4_small_kernel<PARTS, NMAT, GPT>>(
                            dim3((unsigned)ceil_div(p.n, kW4Rows / NMAT), (unsigned)ceil_div(p.m, kSTok4), (unsigned)p.parts),
                            kW4Threads, W4Small<PARTS>::kBytes, p.parts, s, m, p);
-    return launch_maps(gemm_w4_pair_kernel<PARTS, NMAT, GPT>, dim3(2 * (unsigned)npairs), kPairThreads,
+    return launch_maps<gemm_w4_pair_kernel<PARTS, NMAT, GPT>>(dim3(2 * (unsigned)npairs), kPairThreads,
                        W4Pair<PARTS, NMAT>::kBytes, 0, s, m, p);
 }
 

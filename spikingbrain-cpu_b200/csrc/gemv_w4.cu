@@ -294,7 +294,8 @@ template <bool BF16, int MT, int PARTS, int NSTR, bool GATED, int GPT>
 static cudaError_t launch_gemv_w4(GemvW4Params p, cudaStream_t s) {
     auto kernel = gemv_w4_kernel<BF16, MT, PARTS, NSTR, GATED, GPT>;
     constexpr int smem = GemvW4Smem<NSTR, GPT>::kBytes;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = w4_allow_smem(kernel, smem, allowed);
     if (e != cudaSuccess) return e;
     // CTAs that fit on an SM at once (the same on every device the library runs on)
     static const int per_sm = [&] {

@@ -1,6 +1,8 @@
 // What the 4-bit entry points and kernels share on the host, and the device helpers of their epilogues.
 #pragma once
 
+#include <atomic>
+
 #include "w4.cuh"
 
 namespace sbq {
@@ -34,6 +36,20 @@ size_t gemm_w4_workspace(int64_t m, int64_t n, int64_t k, bool split, int nmat);
 int w4_sm_count();
 
 inline int w4_elem(int dtype) { return dtype == SBQ_F32 ? 4 : 2; }
+
+// Lets a kernel use `bytes` of dynamic shared memory on the current device: once per kernel and device (`done`, the
+// kernel's own), since the call costs as much host time as a tenth of a launch.
+template <class K>
+cudaError_t w4_allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    const uint64_t bit = dev < 64 ? uint64_t(1) << dev : 0;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t s = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (s == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return s;
+}
 
 // A launch as a programmatic dependent of the previous kernel on the stream.  Each kernel launched
 // this way reads nothing but packed weights before its griddepcontrol.wait and lets its own dependents

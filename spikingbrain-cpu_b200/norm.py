@@ -115,7 +115,7 @@ def residual_norm(branch: torch.Tensor | None, residual: torch.Tensor, pre_weigh
     x = None
     if pre_weight is not None:
         w = _weight(pre_weight, d, "pre_weight", dev)
-        x = torch.empty(shape, dtype=out_dtype, device=dev)
+        x = residual.new_empty(shape, dtype=out_dtype)
         a.pre_weight, a.out, a.ld_out = w.data_ptr(), x.data_ptr(), d
     if residual_out is not None:
         if residual_out.shape != shape or residual_out.dtype != residual.dtype or residual_out.device != dev:
@@ -129,7 +129,7 @@ def residual_norm(branch: torch.Tensor | None, residual: torch.Tensor, pre_weigh
     elif branch is None and residual_scale == 1.0:
         new = residual
     else:
-        new = torch.empty(shape, dtype=residual.dtype, device=dev)
+        new = torch.empty_like(residual, memory_format=torch.contiguous_format)
         a.residual_out, a.ld_residual_out = new.data_ptr(), d
     if m > 0 and (x is not None or new is not residual or residual_out is not None):
         status = L.load().sbq_residual_norm(ctypes.byref(a), _raw_stream(dev))

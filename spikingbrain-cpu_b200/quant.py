@@ -532,7 +532,7 @@ class Int4Linear(nn.Module):
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         k, n, dev = self.in_features, self.out_features, self._buffers["packed"].device
         if _in_place(x, k, dev):
-            out = torch.empty((*x.shape[:-1], n), dtype=self.out_dtype, device=dev)
+            out = x.new_empty((*x.shape[:-1], n), dtype=self.out_dtype)
             self._run(x, x.numel() // k, k, k, out, n, dev)
             return out
         x2, on_host = _int4_rows(x, k, dev)
