@@ -20,7 +20,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .quant import _DTYPE_CODE, INT4_FORMATS, DynamicInt8Linear, Int8Linear, _device, _ptr
+from .quant import _DTYPE_CODE, INT4_FORMATS, DynamicInt8Linear, Int4Linear, Int8Linear, _device, _ptr
 from .quant import make_linear as _make_linear_eager
 
 
@@ -107,7 +107,9 @@ class StreamingPacker:
         """quant.make_linear's signature and results (quant.py:100-111); int8 formats streamed
         (the others, int4 among them, are made on the current stream)."""
         if fmt not in ("int8", "int8-dyn"):
-            if fmt in ("float32", "bfloat16", "float16") + INT4_FORMATS:
+            if fmt in INT4_FORMATS:
+                return Int4Linear(weight, bias, group=int(fmt[6:]), device=self.device)
+            if fmt in ("float32", "bfloat16", "float16"):
                 return _make_linear_eager(fmt, weight, bias)
             raise ValueError("unknown weight format " + fmt)
         dyn = fmt == "int8-dyn"

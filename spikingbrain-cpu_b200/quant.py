@@ -333,7 +333,8 @@ def _int4_buffers(n: int, k: int, group: int, dev: torch.device):
     lib = L.load()
     return (torch.empty(int(lib.sbq_w4_packed_bytes(n, k)), dtype=torch.uint8, device=dev),
             torch.empty(int(lib.sbq_w4_scale_bytes(n, k, group)), dtype=torch.uint8, device=dev),
-            torch.empty((n + 15) // 16 * 16, dtype=torch.float32, device=dev))
+            # fp32 powers of two, held as their bits: a module's .half() or .to(dtype) leaves integer buffers alone
+            torch.empty((n + 15) // 16 * 16, dtype=torch.int32, device=dev))
 
 
 def pack_weight_int4(weight: torch.Tensor, group: int = 128, device=None):
@@ -443,9 +444,11 @@ class Int4Linear(nn.Module):
         """A module around buffers of ``pack_weight_int4`` / ``pack_int4``; they are adopted, not copied."""
         lib = L.load()
         group = _check_group(group)
-        if packed.numel() != int(lib.sbq_w4_packed_bytes(out_features, in_features)) or \
-                scales.numel() != int(lib.sbq_w4_scale_bytes(out_features, in_features, group)) or \
-                rowmul.numel() != (out_features + 15) // 16 * 16:
+        sizes = (int(lib.sbq_w4_packed_bytes(out_features, in_features)),
+                 int(lib.sbq_w4_scale_bytes(out_features, in_features, group)), (out_features + 15) // 16 * 16)
+        for t, size, dtype in zip((packed, scales, rowmul), sizes, (torch.uint8, torch.uint8, torch.int32)):
+            if t.numel() == size and t.dtype == dtype and t.is_contiguous() and t.is_cuda and t.device == packed.device:
+                continue
             raise ValueError("packed buffers do not match a [%d, %d] weight in groups of %d" % (out_features, in_features, group))
         mod = cls.__new__(cls)
         nn.Module.__init__(mod)
@@ -521,6 +524,8 @@ class Int4Linear(nn.Module):
             with torch.cuda.device(dev):
                 return self._run(x, m, k, ldx, out, ldy, dev)
         b, code, bias = self._buffers, _DTYPE_CODE[x.dtype], self._parameters.get("bias")
+        if bias is not None and bias.dtype != torch.float32:  # a module converted with .half() or .to(dtype)
+            bias = bias.float()
         ws, ws_bytes = _int4_workspace(m, self.out_features, k, code, 1, dev)
         status = L.load().sbq_linear_w4(
             x.data_ptr(), code, ldx, b["packed"].data_ptr(), b["scales"].data_ptr(), b["rowmul"].data_ptr(), self.group,

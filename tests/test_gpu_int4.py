@@ -297,6 +297,50 @@ def test_state_dict_round_trip(sbq):
             b.load_state_dict(bad)
 
 
+def test_converted_modules(sbq):
+    """.half() and .to(dtype) on a model leave the packed weight and the results as they were (the bias is rounded)."""
+    q, s = weight(40, 96, 32, seed=40)
+    bias = torch.arange(40.0) / 8  # exact in fp16
+    lin = sbq.Int4Linear.from_quantized(q, s, bias, group=32)
+    xs = [acts(m, 96, F16, seed=41) for m in (3, 30)]
+    want = [lin(x) for x in xs]
+    for convert in (lambda m: m.half(), lambda m: m.to(BF16), lambda m: m.to("cuda")):
+        box = convert(torch.nn.Sequential(sbq.Int4Linear.from_quantized(q, s, bias, group=32)))
+        assert all(torch.equal(box(x), w) for x, w in zip(xs, want))
+    with pytest.raises(ValueError, match="do not match"):
+        sbq.Int4Linear.from_packed(lin.packed, lin.scales, lin.rowmul.float(), 40, 96, None, 32)
+    with pytest.raises(ValueError, match="do not match"):
+        sbq.Int4Linear.from_packed(lin.packed, lin.scales, lin.rowmul, 40, 96, None, 64)
+
+
+def test_first_call_may_be_a_captured_one(sbq):
+    """Nothing needs a warm-up: kernels that have not run in this process, captured first (a process of its own)."""
+    import subprocess
+    import sys
+
+    from conftest import ROOT
+
+    code = """
+import importlib, torch
+sbq = importlib.import_module("spikingbrain-cpu_b200")
+q = torch.randint(-8, 8, (300, 512), dtype=torch.int8, device="cuda")
+s = torch.ones(300, 8, dtype=torch.bfloat16, device="cuda")
+lin = sbq.Int4Linear.from_quantized(q, s, None, group=64)
+w = torch.ones(300, device="cuda")
+for m in (1, 40, 300):
+    x = torch.randn(m, 512, device="cuda")
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        y = lin(x)
+        r, n = sbq.residual_norm(y, y, w)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, lin(x)) and torch.equal(n, sbq.residual_norm(y, y, w)[1])
+"""
+    done = subprocess.run([sys.executable, "-c", code], cwd=str(ROOT), capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0, done.stderr[-2000:]
+
+
 def test_formats_loader_and_groups(sbq):
     """Every way a user gets to the format: make_linear, the streaming loader, the module fusions."""
     for fmt in sbq.INT4_FORMATS:
