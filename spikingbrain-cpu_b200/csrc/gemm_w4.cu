@@ -43,6 +43,7 @@ struct GemmW4Params {
     int seg_blocks;  // blocks of 128 k per accumulation segment
     // pair kernel: rounds of whole tiles, then tail_tiles tiles cut into tail_parts parts along k
     int rounds, tail_tiles, tail_parts;
+    int tok;  // tokens of a tile: a multiple of 32 up to 256
     float* partial;  // [tail tile][part][token][lane of both CTAs]: sums of a cut tile's parts, or null
     const float* rowmul[2];
     const float* bias;
@@ -152,9 +153,10 @@ __device__ __forceinline__ void group_sync(int grp) { asm volatile("bar.sync %0,
 // MMAs go on, and scale and store a finished tile under the next one's MMAs.  Registers are dealt to the roles
 // by setmaxnreg: a taker holds up to 128 fp32 sums.
 //
-// Tiles are 256 tokens wide (the accumulator and four operand buffers fill tensor memory): an MMA of 128 tokens
-// whose A operand comes from tensor memory takes about 100 cycles, not half of the 256-token one's 128-150.  The
-// last token tile's MMAs are as wide as its tokens.
+// Tiles are up to 256 tokens wide (that accumulator and four operand buffers fill tensor memory).  An MMA of N tokens
+// whose A operand comes from tensor memory takes about 50 + 0.39 N cycles (N = 128: 100), so wide tiles are
+// the efficient ones and narrow ones serve products that would leave pairs without a tile.  The last token tile's
+// MMAs are as wide as its tokens.
 //
 // The tiles of the last, incomplete round are cut along k so that every pair has a part; a cut tile's parts go to
 // `partial` as fp32 sums and w4_reduce_kernel adds them in order.
@@ -168,7 +170,7 @@ __device__ __forceinline__ void regs_more() { asm volatile("setmaxnreg.inc.sync.
 template <int N>
 __device__ __forceinline__ void regs_less() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 
-constexpr int kTok = 256;  // tokens of a tile
+constexpr int kTok = 256;  // tokens of a tile, at most
 template <int PARTS, int NMAT>
 using W4Pair = W4Shape<kTok / 2, kTok, PARTS, 1, 512, 224 * 1024, NMAT == 2 ? 32 * 1024 : 0>;
 
@@ -195,9 +197,9 @@ __device__ __forceinline__ W4Item w4_item(const GemmW4Params& p, int pair, int n
 }
 
 // Tokens of the MMAs of a tile: its rows of x rounded up to 32.
-__device__ __forceinline__ int w4_tile_tokens(int m, int t0) {
-    const int left = (m - t0 + 31) & ~31;
-    return left < kTok ? left : kTok;
+__device__ __forceinline__ int w4_tile_tokens(const GemmW4Params& p, int t0) {
+    const int left = (p.m - t0 + 31) & ~31;
+    return left < p.tok ? left : p.tok;
 }
 
 template <class T>
@@ -309,9 +311,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             };
             auto load_x = [&](int s, int tile, int kb) {
                 uint8_t* xs = smem + s * S::kStage;
-                const int t0 = (tile / cols) * kTok, tr = t0 + (int)rank * (w4_tile_tokens(p.m, t0) / 2);
+                const int t0 = (tile / cols) * p.tok, tr = t0 + (int)rank * (w4_tile_tokens(p, t0) / 2);
                 const uint32_t xb = tc::cluster_addr(&ready[s], 0);
-                if (leader) tc::mbar_arrive_expect_tx(&ready[s], 2 * S::kXBytes);
+                if (leader) tc::mbar_arrive_expect_tx(&ready[s], (uint32_t)p.tok * (PARTS * 256));  // both CTAs' boxes
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     tc::tma_load_2d_pair(xs + h * PARTS * S::kXSub, &map_x, xb, kb * 128 + h * 64, tr);
@@ -354,7 +356,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             bool ok = true;
             for (int i = 0; i < items && ok; ++i) {
                 const W4Item w = w4_item(p, pair, npairs, i);
-                const uint32_t idesc = tc::idesc_f16(2 * kW4Rows, w4_tile_tokens(p.m, (w.tile / cols) * kTok), false);
+                const uint32_t idesc = tc::idesc_f16(2 * kW4Rows, w4_tile_tokens(p, (w.tile / cols) * p.tok), false);
                 int left = 0;  // blocks left in the segment
                 for (int kb = w.kb0; kb < w.kb1; ++kb) {
                     const bool fresh = left == 0;
@@ -436,7 +438,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     } else {
         regs_more<kRegsTake>();
         const int grp = (warp - 12) >> 2, wq = warp & 3, row = wq * 32 + lane;
-        const uint32_t src = tmem + ((uint32_t)(wq * 32) << 16) + grp * COLS;
+        const int half = p.tok / 2;  // tokens of this warpgroup
+        const uint32_t src = tmem + ((uint32_t)(wq * 32) << 16) + grp * half;
         const uint32_t taken0 = tc::cluster_addr(taken, 0);
         const int mat = NMAT == 2 ? row >> 6 : 0, cn = (int)rank * kCh + (NMAT == 2 ? row & 63 : row);
         float* xch = reinterpret_cast<float*>(smem + S::kXchOff) + grp * 32 * kW4Rows;
@@ -445,7 +448,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         bool ok = true;  // a warp whose wait ran out stores nothing more, but stays for the group's barriers
         for (int i = 0; i < items; ++i) {
             const W4Item w = w4_item(p, pair, npairs, i);
-            const int n = (w.tile % cols) * (2 * kCh) + cn, t0 = (w.tile / cols) * kTok + grp * COLS;
+            const int n = (w.tile % cols) * (2 * kCh) + cn, t0 = (w.tile / cols) * p.tok + grp * half;
             const float inv = 1.0f / (n < p.n ? __ldg(p.rowmul[mat] + n) : 1.0f);
             const float bias = NMAT == 1 && p.bias && n < p.n ? __ldg(p.bias + n) : 0.0f;
             float sum[COLS];
@@ -456,11 +459,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                 tc::fence_after_sync();
                 if (kb == w.kb0) {
 #pragma unroll
-                    for (int c = 0; c < COLS / 16; ++c) tmem_ld_x16(src + c * 16, reinterpret_cast<uint32_t*>(sum) + c * 16);
+                    for (int c = 0; c < COLS / 16; ++c)
+                        if (c * 16 < half) tmem_ld_x16(src + c * 16, reinterpret_cast<uint32_t*>(sum) + c * 16);
                     tc::tmem_wait_ld();
                 } else {
 #pragma unroll
                     for (int c = 0; c < COLS / 16; ++c) {
+                        if (c * 16 >= half) continue;
                         uint32_t r[16];
                         tmem_ld_x16(src + c * 16, r);
                         tc::tmem_wait_ld();
@@ -474,38 +479,41 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             }
             // ---- the tile's sums are here, the MMAs go on
             if (w.slot >= 0) {
-                float* out = p.partial + ((int64_t)w.slot * kTok + grp * COLS) * (2 * kW4Rows) + (int)rank * kW4Rows + row;
+                float* out = p.partial + ((int64_t)w.slot * kTok + grp * half) * (2 * kW4Rows) + (int)rank * kW4Rows + row;
                 if (ok) {
 #pragma unroll
                     for (int j = 0; j < COLS; ++j)
-                        if (t0 + j < p.m) __stcg(out + j * (2 * kW4Rows), sum[j]);
+                        if (j < half && t0 + j < p.m) __stcg(out + j * (2 * kW4Rows), sum[j]);
                 }
                 continue;
             }
 #pragma unroll
-            for (int j = 0; j < COLS; ++j) sum[j] *= inv;
-            if (p.xinv) w4_times_xinv<COLS>(p.xinv, t0, sum);
-            if (NMAT == 1) {
-                if (ok) w4_put<COLS>(p, t0, n, [&](int j) { return sum[j] + bias; });
-            } else {
-                // gate lanes finish the first half of the tokens, up lanes the second: each hands the other its
-                // values of 32 tokens at a time
-                constexpr int H = COLS / 2;
+            for (int c = 0; c < COLS / 16; ++c) {
+                if (c * 16 >= half) continue;
+#pragma unroll
+                for (int j = 0; j < 16; ++j) sum[c * 16 + j] *= inv;
+                if (p.xinv) w4_times_xinv<16>(p.xinv, t0 + c * 16, sum + c * 16);
+                if (NMAT == 1 && ok) w4_put<16>(p, t0 + c * 16, n, [&](int j) { return sum[c * 16 + j] + bias; });
+            }
+            if (NMAT == 2) {
+                // of every 32 tokens the gate lanes finish the first 16, the up lanes the others: each hands the other its
+                // values.  Two buffers, so one barrier per 32 tokens
                 const bool up = mat == 1;
 #pragma unroll
-                for (int r = 0; r < H / 32; ++r) {
+                for (int c = 0; c < COLS / 32; ++c) {
+                    if (c * 32 >= half) continue;
+                    float* buf = xch + (c & 1) * 16 * kW4Rows;
 #pragma unroll
-                    for (int j = 0; j < 32; ++j) xch[j * kW4Rows + row] = up ? sum[r * 32 + j] : sum[H + r * 32 + j];
+                    for (int j = 0; j < 16; ++j) buf[j * kW4Rows + row] = up ? sum[c * 32 + j] : sum[c * 32 + 16 + j];
                     group_sync(grp);
                     if (ok)
-                        w4_put<32>(p, t0 + (up ? H : 0) + r * 32, n, [&](int j) {
-                            const float mine = up ? sum[H + r * 32 + j] : sum[r * 32 + j], other = xch[j * kW4Rows + (row ^ 64)];
+                        w4_put<16>(p, t0 + c * 32 + (up ? 16 : 0), n, [&](int j) {
+                            const float mine = up ? sum[c * 32 + 16 + j] : sum[c * 32 + j], other = buf[j * kW4Rows + (row ^ 64)];
                             const float gv = up ? other : mine, uv = up ? mine : other;
                             // a 16-bit result: the approximate exponential and division (a few 2^-22) are far below
                             // its rounding
                             return p.y_dtype == SBQ_F32 ? w4_silu(gv) * uv : __fdividef(gv, 1.0f + __expf(-gv)) * uv;
                         });
-                    group_sync(grp);
                 }
             }
         }
@@ -528,10 +536,10 @@ __global__ void __launch_bounds__(2 * kW4Rows) w4_reduce_kernel(const GemmW4Para
     const int cols = (p.n + 2 * kCh - 1) / (2 * kCh);
     const int cut = (int)blockIdx.y, tile = p.rounds * npairs + cut;
     const int tid = (int)threadIdx.x, ch = NMAT == 2 ? tid & 127 : tid;
-    const int j0 = ((int)blockIdx.x * NMAT + (NMAT == 2 ? tid >> 7 : 0)) * T, t0 = (tile / cols) * kTok + j0;
+    const int j0 = ((int)blockIdx.x * NMAT + (NMAT == 2 ? tid >> 7 : 0)) * T, t0 = (tile / cols) * p.tok + j0;
     const int lane0 = NMAT == 2 ? (ch >> 6) * kW4Rows + (ch & 63) : ch;
     const int n = (tile % cols) * (2 * kCh) + ch;
-    if (n >= p.n || t0 >= p.m) return;
+    if (n >= p.n || t0 >= p.m || j0 >= p.tok) return;
     const int count = p.m - t0 < T ? p.m - t0 : T;
     const float* base = p.partial + ((int64_t)cut * p.tail_parts * kTok + j0) * kLanes + lane0;
     float v[NMAT][T];
@@ -873,30 +881,36 @@ static cudaError_t launch_gemm_w4_g(int gpt, int tok, int npairs, const W4Maps& 
 
 constexpr int64_t kW4SmallRows = 128;
 
-// The pair kernel's schedule: whole rounds of tiles over the pairs, the tiles left over cut into parts along k.
-// Cutting is worth its cost (storing the sums, a second launch, reading them: about 13 us and 50 ns for every part's
-// 256 KiB) by a model of the time: a block of 128 k takes about 0.55 us, with an fp32 activation's two parts 1.1 us.
-// Measured on B200, uncut and cut: fp32 300 x 12288 x 4096 (32 tiles on 74 pairs) 140 and 85 us, fp32 512 x 2560 x 9728
-// (2 tiles left of 76) 67 and 53 us; fp16 512 x 2560 x 9728 31 and 35 us, fp16 2048 x 4096 x 12288 (14 left of
-// 384) 143 and 144 us: those two stay uncut.
+// The pair kernel's schedule: tokens per tile, whole rounds of tiles over the pairs, and the tiles left over cut into
+// parts along k.  It takes the shortest time by a model of a block of 128 k: eight MMAs (two parts of x: sixteen) of
+// 50 + 0.39 N cycles, or the conversion's 0.33 us, whichever is longer.  Cutting costs about 13 us (storing the sums,
+// a second launch, reading them) and 50 ns for every part's 256 KiB.
+// Measured on B200 at 256 tokens per tile, uncut and cut: fp32 300 x 12288 x 4096 (32 tiles on 74 pairs) 140 and 85 us,
+// fp32 512 x 2560 x 9728 (2 tiles left of 76) 67 and 53 us; fp16 512 x 2560 x 9728 31 and 35 us, fp16
+// 2048 x 4096 x 12288 (14 left of 384) 143 and 144 us: those two stay uncut.
 struct W4Plan {
-    int npairs, rounds, tail_tiles, tail_parts;
+    int tok, npairs, rounds, tail_tiles, tail_parts;
 };
 
 static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, bool split, int nmat) {
-    const int64_t tiles = ceil_div(n, 2 * kW4Rows / nmat) * ceil_div(m, kTok), pairs = w4_sm_count() / 2, kt = w4_tiles_k(k);
-    W4Plan pl{};
-    pl.rounds = (int)(tiles / pairs);
-    pl.tail_tiles = (int)(tiles % pairs);
-    pl.tail_parts = 1;
-    const double block = split ? 1.1 : 0.55;
-    double best = (double)kt * block;
-    for (int64_t parts = 2; parts <= 16 && pl.tail_tiles > 0 && parts * pl.tail_tiles <= pairs && 2 * parts <= kt; ++parts) {
-        const double t = (double)ceil_div(kt, parts) * block + 13.0 + 0.05 * (double)(parts * pl.tail_tiles);
-        if (t < best) best = t, pl.tail_parts = (int)parts;
+    const int64_t cols = ceil_div(n, 2 * kW4Rows / nmat), pairs = w4_sm_count() / 2, kt = w4_tiles_k(k);
+    W4Plan best{};
+    double best_t = 1e30;
+    // with two matrices a taker warpgroup finishes whole sets of 32 tokens
+    for (int tok = kTok; tok >= 32 * nmat; tok -= 32 * nmat) {
+        const int64_t tiles = cols * ceil_div(m, tok), rounds = tiles / pairs, tail = tiles % pairs;
+        const double mma = (split ? 16 : 8) * (50 + 0.39 * tok) / 1850, block = mma > 0.33 ? mma : 0.33;
+        W4Plan pl{tok, 0, (int)rounds, (int)tail, 1};
+        double least = (double)((rounds + (tail > 0)) * kt) * block;
+        for (int64_t parts = 2; parts <= 16 && tail > 0 && parts * tail <= pairs && 2 * parts <= kt; ++parts) {
+            const double t = (double)(rounds * kt + ceil_div(kt, parts)) * block + 13.0 + 0.05 * (double)(parts * tail);
+            if (t < least) least = t, pl.tail_parts = (int)parts;
+        }
+        pl.npairs = rounds > 0 ? (int)pairs : pl.tail_tiles * pl.tail_parts;
+        // a narrower tile must gain 3 %: it reads the weight more often than the model knows
+        if (least < 0.97 * best_t) best_t = least, best = pl;
     }
-    pl.npairs = pl.rounds > 0 ? (int)pairs : pl.tail_tiles * pl.tail_parts;
-    return pl;
+    return best;
 }
 
 size_t gemm_w4_workspace(int64_t m, int64_t n, int64_t k, bool split, int nmat) {
@@ -932,10 +946,11 @@ int gemm_w4_run(const W4Call& c, const W4Acts& x) {
         p.rounds = pl.rounds;
         p.tail_tiles = pl.tail_tiles;
         p.tail_parts = pl.tail_parts;
+        p.tok = pl.tok;
         p.partial = static_cast<float*>(x.scratch);
     }
     W4Maps maps;
-    const int st = tok == kSTok4 ? make_maps(maps, c, x, kSTok4, ch) : make_maps(maps, c, x, kTok / 2, ch);
+    const int st = tok == kSTok4 ? make_maps(maps, c, x, kSTok4, ch) : make_maps(maps, c, x, p.tok / 2, ch);
     if (st) return st;
     cudaError_t e = x.part[1] ? (nmat == 2 ? launch_gemm_w4_g<2, 2>(c.gpt, tok, pl.npairs, maps, p, c.stream)
                                            : launch_gemm_w4_g<2, 1>(c.gpt, tok, pl.npairs, maps, p, c.stream))

@@ -170,10 +170,11 @@ static bool w4_needs_parts(int64_t m, int64_t k, int x_dtype) {
     return x_dtype == SBQ_F32 || (x_dtype == SBQ_BF16 && m > kW4GemvRows) || k % 16 != 0;
 }
 
-// x in the workspace and its factors; the factors are read 32 at a time, up to the largest token tile.
+// x in the workspace and its factors; the factors are read 16 or 32 at a time, up to the end of the last token tile
+// (of at most 256).
 static size_t act_bytes(int64_t m, int64_t k, int x_dtype) {
     if (!w4_needs_parts(m, k, x_dtype)) return 0;
-    return (x_dtype == SBQ_F32 ? 2 : 1) * align256((size_t)m * round16(k) * 2) + (size_t)ceil_div(m, 256) * 1024;
+    return (x_dtype == SBQ_F32 ? 2 : 1) * align256((size_t)m * round16(k) * 2) + (size_t)ceil_div(m + 256, 256) * 1024;
 }
 
 static int check_w4_call(const void* x, int x_dtype, int64_t ldx, const W4Call& c, int group, int nmat) {
