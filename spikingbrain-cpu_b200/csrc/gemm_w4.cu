@@ -506,14 +506,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 #pragma unroll
                     for (int j = 0; j < 16; ++j) buf[j * kW4Rows + row] = up ? sum[c * 32 + j] : sum[c * 32 + 16 + j];
                     group_sync(grp);
-                    if (ok)
-                        w4_put<16>(p, t0 + c * 32 + (up ? 16 : 0), n, [&](int j) {
-                            const float mine = up ? sum[c * 32 + 16 + j] : sum[c * 32 + j], other = buf[j * kW4Rows + (row ^ 64)];
-                            const float gv = up ? other : mine, uv = up ? mine : other;
-                            // a 16-bit result: the approximate exponential and division (a few 2^-22) are far below
-                            // its rounding
-                            return p.y_dtype == SBQ_F32 ? w4_silu(gv) * uv : __fdividef(gv, 1.0f + __expf(-gv)) * uv;
-                        });
+                    float res[16];
+#pragma unroll
+                    for (int j = 0; j < 16; ++j) res[j] = buf[j * kW4Rows + (row ^ 64)];
+                    // a 16-bit result: the approximate exponential and division (a few 2^-22) are far below its
+                    // rounding
+                    if (p.y_dtype == SBQ_F32) {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j)
+                            res[j] = up ? w4_silu(res[j]) * sum[c * 32 + 16 + j] : w4_silu(sum[c * 32 + j]) * res[j];
+                    } else {
+#pragma unroll
+                        for (int j = 0; j < 16; ++j) {
+                            const float gv = up ? res[j] : sum[c * 32 + j], uv = up ? sum[c * 32 + 16 + j] : res[j];
+                            res[j] = __fdividef(gv, 1.0f + __expf(-gv)) * uv;
+                        }
+                    }
+                    if (ok) w4_put<16>(p, t0 + c * 32 + (up ? 16 : 0), n, [&](int j) { return res[j]; });
                 }
             }
         }
