@@ -8,6 +8,10 @@
 // A row is held in registers as fp32 between its loads and its stores, so y, r and the gate are read once
 // and r' and x written once; both statistics are fp32 sums over fp32 values, and x is taken from r' before
 // r' is rounded to the residual's type.
+//
+// The bytes bound it.  Measured on B200: 8192 x 4096, fp32 in and fp16 out, without a post norm 69.5 us (6.8 TB/s, 1.03 of
+// the measured copy rate), with it 75 us; 1 x 4096 2.9 us (a launch); 16-bit rows with a gate per element, which have
+// half the bytes per element and twice the arithmetic, 3001 x 2560 22 us (3.5 TB/s) and 3001 x 2559 36 us.
 #include "w4_host.cuh"
 
 namespace sbq {

@@ -17,7 +17,7 @@ quantiser on ``N(0, 0.02)`` weights.  The chain from layer to layer runs through
 attention path: h is quadratic in x, so a chain through down(h) is unstable under any constant
 scale (a layer input slightly below unit scale shrinks quadratically from layer to layer and
 reaches zero in fp16 within about twelve layers).  The model's residual stream and norms are not
-part of the quantised-linear path.
+part of the quantised-linear path here; ``ResidualStack`` runs them.
 
 Sharding (``world > 1``): rank r owns rows [r n / world, (r+1) n / world) of every projection and
 produces that slice of each output; x is replicated.  Two ways assemble the full activation before
@@ -41,7 +41,8 @@ import torch.nn as nn
 
 from . import workloads as W
 from .mlp import FusedGatedMLP
-from .quant import Int8Linear
+from .norm import ResidualNorm
+from .quant import INT4_FORMATS, Int4Linear, Int8Linear
 
 
 def _fold(k: int, second_moment: float = 1.0) -> float:
@@ -489,6 +490,66 @@ class ProjectionStack(nn.Module):
         if m <= 16:
             return len(self.layers) * 2 + (1 if self.peer is not None else 0) + (1 if self.overlap else 0)
         return len(self.layers) * 5
+
+
+class ResidualLayer(nn.Module):
+    """One block of a ``ResidualStack``: its projections and the norms that follow its two halves."""
+
+    def __init__(self, layer: int, hidden: int, inter: int, seed: int, fmt: str, gate_act: str, device):
+        super().__init__()
+        base = seed * 1000 + layer * 16
+
+        def linear(n: int, k: int, idx: int) -> nn.Module:
+            w = W.float_weight(n, k, seed=base + idx, device=device)
+            lin = Int4Linear(w, None, int(fmt[6:]), device) if fmt in INT4_FORMATS else Int8Linear(w, None, device=device)
+            lin.out_dtype = torch.float16
+            return lin
+
+        def weight(idx: int) -> torch.Tensor:
+            g = torch.Generator(device=device).manual_seed(base + idx)
+            return 1.0 + 0.1 * torch.randn(hidden, generator=g, device=device)
+
+        self.hidden = hidden
+        self.qkv, self.o = linear(3 * hidden, hidden, 0), linear(hidden, hidden, 4)
+        self.mlp = FusedGatedMLP(linear(inter, hidden, 6), linear(inter, hidden, 7), linear(hidden, inter, 8))
+        # a half's output is normalised and gated on its way into the residual stream, the sum for the next half
+        self.after_attention = ResidualNorm(weight(9), weight(10), gate_act)
+        self.after_mlp = ResidualNorm(weight(11), weight(12), gate_act)
+        self.register_buffer("gate_attention", weight(13))
+        self.register_buffer("gate_mlp", weight(14))
+
+    def forward(self, x: torch.Tensor, r: torch.Tensor):
+        """(residual, next block's input) from this block's input and the residual."""
+        v = self.qkv(x)[:, 2 * self.hidden:]
+        r, x = self.after_attention(self.o(v), r, self.gate_attention)
+        return self.after_mlp(self.mlp(x), r, self.gate_mlp)
+
+
+class ResidualStack(nn.Module):
+    """The model's blocks with their residual stream and norms (Block.forward, spikingbrain_cpu/model.py:388-392) around
+    the quantised projections, synthetic weights, one GPU: every row is a sequence of one token, whose attention
+    output is its own v.  ``fmt``: "int8" or one of the 4-bit formats.  The residual stays in fp32, the projections
+    read and write fp16; four launches of projections and two of norms per block.  ``CapturedStack`` captures it
+    like a ``ProjectionStack``.
+    """
+
+    def __init__(self, layers: int = W.LAYERS, hidden: int = W.HIDDEN, inter: int = W.INTER, seed: int = 0,
+                 fmt: str = "int4-g128", gate_act: str = "sigmoid", device="cuda"):
+        super().__init__()
+        if fmt != "int8" and fmt not in INT4_FORMATS:
+            raise ValueError("a residual stack runs int8 or int4 weights, got " + fmt)
+        device = torch.device(device)
+        self.device = torch.device("cuda", torch.cuda.current_device()) if device.index is None else device
+        self.hidden, self.inter = hidden, inter
+        self.layers = nn.ModuleList(ResidualLayer(i, hidden, inter, seed, fmt, gate_act, self.device) for i in range(layers))
+        self.first = ResidualNorm(torch.ones(hidden, device=self.device))
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        """fp16 or fp32 [m, hidden] -> fp16 [m, hidden], the normalised residual after the last block."""
+        r, x = self.first(None, x.float())
+        for layer in self.layers:
+            r, x = layer(x, r)
+        return x
 
 
 class DecodeProgram:
