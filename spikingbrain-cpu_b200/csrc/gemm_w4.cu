@@ -19,11 +19,12 @@
 //
 // Tensor-core accumulation truncates: measured on B200, the relative error of a sum grows by about 1.3e-8 per
 // k16 step (1.2e-5 at k = 12288).  Where the result is kept in fp32 the sum is therefore cut into segments
-// of kSegSteps steps, and each finished segment is added to fp32 registers (round to nearest).  16-bit results,
+// of kSegSteps = 32 steps, and each finished segment is added to fp32 registers (round to nearest): 3e-7 (bf16 x) to
+// 6e-7 (fp32 x) at any k from 512 to 12288, with 64 steps 1.2e-6.  16-bit results,
 // whose own rounding (2^-12 and up) is far above it, are summed in one piece.
 //
 // Measured on B200, groups of 128: 4096 x 4096 x 12288 fp16 270 us (1.52 PFLOP/s, 0.92 of cuBLAS's measured bf16 rate),
-// 2048 x 4096 x 12288 fp16 142 us, with fp32 results 153 us; gate/up 2048 x 4096 x 12288 295 us with bf16 x.  Long
+// 2048 x 4096 x 12288 fp16 143 us, with fp32 results 171 us (a segment ends in the wait for the accumulator to be read); gate/up 2048 x 4096 x 12288 295 us with bf16 x.  Long
 // products are bound by the tensor cores; one tile per pair (512 x 4096 x 4096, 24 us) by about 8 us of set-up, first
 // loads and stores and 0.5 us per block of 128 k; 64 x 4096 x 12288 (20 us) by x, read again for every 128 channels.
 #include "tc.cuh"
@@ -33,7 +34,7 @@ namespace sbq {
 
 constexpr int kW4Threads = 384;   // producer, MMA, tensor-memory, idle warp, two converter warpgroups
 constexpr int kW4Rows = 128;      // channels (tensor-memory lanes) per CTA
-constexpr int kSegSteps = 64;     // MMA steps per accumulation segment (measured error: 8e-7)
+constexpr int kSegSteps = 32;     // MMA steps per accumulation segment
 
 __device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2) {
     asm volatile(
@@ -899,9 +900,9 @@ constexpr int64_t kW4SmallRows = 128;
 // parts along k.  It takes the shortest time by a model of a block of 128 k: eight MMAs (two parts of x: sixteen) of
 // 50 + 0.39 N cycles, or the conversion's 0.33 us, whichever is longer.  Cutting costs about 13 us (storing the sums,
 // a second launch, reading them) and 50 ns for every part's 256 KiB.
-// Measured on B200 at 256 tokens per tile, uncut and cut: fp32 300 x 12288 x 4096 (32 tiles on 74 pairs) 140 and 85 us,
-// fp32 512 x 2560 x 9728 (2 tiles left of 76) 67 and 53 us; fp16 512 x 2560 x 9728 31 and 35 us, fp16
-// 2048 x 4096 x 12288 (14 left of 384) 143 and 144 us: those two stay uncut.
+// Measured on B200 at 256 tokens per tile, uncut and cut: fp32 300 x 12288 x 4096 (32 tiles on 74 pairs) 166 and 96 us (73 us
+// with 160-token tiles, cut), fp32 512 x 2560 x 9728 (2 tiles left of 76) 77 and 58 us; fp16 512 x 2560 x 9728 31 and
+// 35 us, fp16 2048 x 4096 x 12288 (14 left of 384) 143 and 144 us: those two stay uncut.
 struct W4Plan {
     int tok, npairs, rounds, tail_tiles, tail_parts;
 };
