@@ -375,7 +375,7 @@ SBQ_API size_t sbq_w4_packed_bytes(int64_t n, int64_t k);
 SBQ_API size_t sbq_w4_scale_bytes(int64_t n, int64_t k, int group);
 
 /* s = bf16(max(max|w|, 1e-8) / 7) per row and group, q = clamp(rint(w / s), -7, 7), packed.  w is [n, k]
- * with row stride ldw, SBQ_F32, SBQ_F16 or SBQ_BF16. */
+ * with row stride ldw, SBQ_F32, SBQ_F16 or SBQ_BF16.  A group with an infinity or a NaN gets the scale NaN. */
 SBQ_API int sbq_w4_quantize_pack(const void* w, int w_dtype, int64_t n, int64_t k, int64_t ldw, int group,
                                  void* packed, void* scales, float* rowmul, void* stream);
 

@@ -6,6 +6,7 @@
 // The scale is rounded before q is taken, so q fits the scale that is stored: |w| / s is at most
 // 7 (1 + 2^-8), which rounds to 7.  A bf16 scale is enough (its rounding is 2^-8 of a step that is
 // itself 1/14 of the group's range) and makes q * s exact in fp16 up to a power of two (w4.cuh).
+// A group that holds an infinity or a NaN has no scale: it gets NaN, and so do the results of its row.
 #include "w4.cuh"
 
 namespace sbq {
@@ -20,6 +21,13 @@ template <>
 __device__ __forceinline__ float w4_f32<__nv_bfloat16>(__nv_bfloat16 v) { return __bfloat162float(v); }
 
 constexpr int kPackThreads = 128;
+
+// The larger of two values, NaN if either is (fmaxf would drop it).
+__device__ __forceinline__ float w4_max_nan(float a, float b) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+    return r;
+}
 
 // The power of two that brings m (the row's largest |scale|) into [2^10, 2^11).
 __device__ __forceinline__ float w4_rowmul(float m) {
@@ -59,11 +67,12 @@ __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const T* __re
         for (int i = 0; i < 8; ++i) {
             const int64_t c = c8 * 8 + i;
             v[i] = (r < n && c < k) ? w4_f32(w[r * ldw + c]) : 0.0f;
-            amax = fmaxf(amax, fabsf(v[i]));
+            amax = w4_max_nan(amax, fabsf(v[i]));
         }
-        for (int o = lanes >> 1; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        for (int o = lanes >> 1; o > 0; o >>= 1) amax = w4_max_nan(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        if (isinf(amax)) amax = __int_as_float(0x7FC00000);
         const bool real = r < n && c8 / lanes * group < k;  // the group has columns of the weight
-        const __nv_bfloat16 sb = __float2bfloat16_rn(real ? __fdiv_rn(fmaxf(amax, 1e-8f), 7.0f) : 0.0f);
+        const __nv_bfloat16 sb = __float2bfloat16_rn(real ? __fdiv_rn(w4_max_nan(amax, 1e-8f), 7.0f) : 0.0f);
         const float s = __bfloat162float(sb);
         smax = fmaxf(smax, s);
         uint32_t word = 0;

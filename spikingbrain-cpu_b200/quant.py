@@ -340,8 +340,8 @@ def _int4_buffers(n: int, k: int, group: int, dev: torch.device):
 def pack_weight_int4(weight: torch.Tensor, group: int = 128, device=None):
     """Quantise an [n, k] float weight per output channel and group of ``group`` inputs on the device, packed.
 
-    ``s = bf16(max(max|w|, 1e-8) / 7)``, ``q = clamp(rint(w / s), -7, 7)``.  Returns ``(packed, scales,
-    rowmul)``, the three device buffers the 4-bit kernels read.
+    ``s = bf16(max(max|w|, 1e-8) / 7)``, ``q = clamp(rint(w / s), -7, 7)``; a group with an infinity or a NaN
+    gets the scale NaN.  Returns ``(packed, scales, rowmul)``, the three device buffers the 4-bit kernels read.
     """
     dev = _device(device)
     group = _check_group(group)

@@ -157,6 +157,23 @@ def test_quantiser(sbq, group, shape, dtype):
     assert torch.equal(s, s_ref) and torch.equal(q, q_ref)
 
 
+@pytest.mark.parametrize("m", [2, 30, 200])
+def test_weights_that_are_not_finite(sbq, m):
+    """An infinity or a NaN in a group makes its channel's results NaN, and no other's."""
+    w = acts(40, 256, F32, seed=50) * 0.02
+    clean = sbq.Int4Linear(w, None, group=64)
+    w[3, 70], w[17, 255], w[39, 0] = float("nan"), float("inf"), -float("inf")
+    lin = sbq.Int4Linear(w, None, group=64)
+    nan = torch.isnan(lin.scale)
+    assert nan.nonzero().tolist() == [[3, 1], [17, 3], [39, 0]]
+    x = acts(m, 256, F16, seed=51)
+    y, want = lin(x), clean(x)
+    bad = [3, 17, 39]
+    assert torch.isnan(y[:, bad]).all()
+    keep = [i for i in range(40) if i not in bad]
+    assert torch.equal(y[:, keep], want[:, keep])
+
+
 def test_pack_unpack_round_trip(sbq):
     for n, k, group in ((1, 1, 32), (31, 200, 64), (130, 1025, 128)):
         q, s = weight(n, k, group, seed=12)
