@@ -396,7 +396,8 @@ SBQ_API size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k, in
 /* y[m, n] = sum_k x[m, k] * q[n, k] * s[n, k / group] (+ bias[n]); x and y SBQ_F32, SBQ_F16 or SBQ_BF16.
  * q * s enters the product exactly, 16-bit x too, fp32 x with 22 bits; sums are fp32.  Up to 16 rows: the
  * decode product; above: the tensor-memory product.  x rows 16-byte aligned when k is a multiple of 16 (any row stride
- * otherwise), workspace 256-byte aligned (NULL when its size is 0). */
+ * otherwise), workspace 256-byte aligned (NULL when its size is 0).  y and x must not overlap (columns of one
+ * buffer do not). */
 SBQ_API int sbq_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* packed, const void* scales,
                           const float* rowmul, int group, const float* bias, int64_t m, int64_t n, int64_t k, void* y,
                           int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream);
@@ -415,9 +416,9 @@ SBQ_API int sbq_mlp_gateup_w4(const void* x, int x_dtype, int64_t ldx, const voi
  *   out = r' * rsqrt(mean(r'^2) + eps) * pre_weight                         (from r' before it is rounded)
  *
  * over rows of d elements (RMSNorm, model.py:30-39; the additions of Block.forward, model.py:388-392).
- * branch may be NULL (r' = residual_scale * residual), residual_out may be NULL, or the residual itself; out
- * and pre_weight are both set or both NULL; out may be the branch (same type and stride).  Other overlaps
- * are not allowed.  branch, residual (and residual_out, of its type), gate and out: SBQ_F32, SBQ_F16 or
+ * branch may be NULL (r' = residual_scale * residual), residual_out may be NULL; out and pre_weight are both
+ * set or both NULL.  Each output may be one of residual, branch and a full gate (same address, element size and
+ * row stride); other overlaps with these three, and of the outputs, are refused.  branch, residual (and residual_out, of its type), gate and out: SBQ_F32, SBQ_F16 or
  * SBQ_BF16, any row stride; weights fp32 [d].  gate: [d] (SBQ_GATE_PER_COLUMN), one per row at stride ld_gate
  * (SBQ_GATE_PER_ROW) or [m, d] (SBQ_GATE_FULL). */
 #define SBQ_GATE_NONE 0

@@ -199,8 +199,14 @@ static int check_w4_call(const void* x, int x_dtype, int64_t ldx, const W4Call& 
     if (reinterpret_cast<uintptr_t>(x) % xs) return set_error(SBQ_ERR_ALIGNMENT, "activation must be aligned to its element size");
     if (reinterpret_cast<uintptr_t>(c.y) % w4_elem(c.y_dtype))
         return set_error(SBQ_ERR_ALIGNMENT, "output must be aligned to its element size");
+    for (int i = 0; i < nmat; ++i)
+        if (reinterpret_cast<uintptr_t>(c.w[i].rowmul) % 4) return set_error(SBQ_ERR_ALIGNMENT, "rowmul must be 4-byte aligned");
+    if (reinterpret_cast<uintptr_t>(c.bias) % 4) return set_error(SBQ_ERR_ALIGNMENT, "bias must be 4-byte aligned");
     if (c.n > (int64_t(1) << 31) - 256 || c.k >= (int64_t(1) << 30) || c.m > (int64_t(1) << 31) - 256)
         return set_error(SBQ_ERR_UNSUPPORTED, "shape too large");
+    const int ys = w4_elem(c.y_dtype);  // one CTA may store its part of y while another still reads x
+    if (w4_overlap({x, ldx * xs, c.k * xs}, {c.y, c.ldy * ys, c.n * ys}, c.m))
+        return set_error(SBQ_ERR_INVALID_ARGUMENT, "output and activation must not overlap");
     return SBQ_OK;
 }
 

@@ -463,6 +463,13 @@ static int check_operand(const void* p, int dtype, int64_t ld, int64_t width, in
     return SBQ_OK;
 }
 
+// Each element of a row is read by the thread that writes it, before it does: an output may take the place of an
+// operand with the same rows, and share no byte with another.
+static bool norm_in_the_way(const W4Rows& out, const W4Rows& in, int64_t m) {
+    if (!out.p || !in.p || !w4_overlap(out, in, m)) return false;
+    return out.p != in.p || (m > 1 && out.ld != in.ld) || out.width != in.width;
+}
+
 }  // namespace sbq
 
 using namespace sbq;
@@ -500,6 +507,15 @@ extern "C" int sbq_residual_norm(const sbq_residual_norm_args* a, void* stream) 
     if (!st && a->pre_weight) st = check_operand(a->pre_weight, SBQ_F32, d, d, 1, "pre_weight", &l, false);
     if (!st && a->post_weight) st = check_operand(a->post_weight, SBQ_F32, d, d, 1, "post_weight", &l, false);
     if (st) return st;
+    const auto rows = [&](const void* q, int dtype, int64_t ld) { return W4Rows{q, ld * w4_elem(dtype), d * w4_elem(dtype)}; };
+    const W4Rows r = rows(a->residual, a->residual_dtype, a->ld_residual), y = rows(a->branch, a->branch_dtype, a->ld_branch),
+                 g = rows(a->gate_mode == SBQ_GATE_FULL ? a->gate : nullptr, a->gate_dtype, a->ld_gate),
+                 ro = rows(a->residual_out, a->residual_dtype, a->ld_residual_out), x = rows(a->out, a->out_dtype, a->ld_out);
+    for (const W4Rows* in : {&r, &y, &g})
+        if (norm_in_the_way(ro, *in, m) || norm_in_the_way(x, *in, m))
+            return set_error(SBQ_ERR_INVALID_ARGUMENT, "an output overlaps an operand with other rows");
+    if (a->residual_out && a->out && w4_overlap(ro, x, m))
+        return set_error(SBQ_ERR_INVALID_ARGUMENT, "the outputs overlap");
     const int mode = l.aligned ? kAligned : l.shifted ? kShifted : kStrided;
     p.y = a->branch, p.r = a->residual, p.gate = a->gate, p.w_post = a->post_weight, p.w_pre = a->pre_weight;
     p.r_out = a->residual_out, p.x = a->out;

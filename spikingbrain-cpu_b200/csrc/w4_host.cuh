@@ -21,7 +21,7 @@ struct W4Call {
 
 // The activation as the kernels read it: 16-bit parts [m, k] with row stride ld.  fp16 and bf16 inputs
 // are read in place; the parts of an fp32 input (and of a bf16 input above 16 rows) are fp16 made by
-// w4_prepare_acts, each row multiplied by a power of two whose inverse is inv[row].
+// w4_acts_kernel, each row multiplied by a power of two whose inverse is inv[row].
 struct W4Acts {
     const void* part[2];
     int64_t ld;
@@ -36,6 +36,22 @@ size_t gemm_w4_workspace(int64_t m, int64_t n, int64_t k, bool split, int nmat);
 int w4_sm_count();
 
 inline int w4_elem(int dtype) { return dtype == SBQ_F32 ? 4 : 2; }
+
+// m rows of `width` bytes, `ld` bytes apart.
+struct W4Rows {
+    const void* p;
+    int64_t ld, width;
+};
+
+// Whether rows of a and b share a byte.  Columns of one buffer (same ld) do not, however their ranges interleave; with
+// different strides, ranges that meet count as shared.
+inline bool w4_overlap(const W4Rows& a, const W4Rows& b, int64_t m) {
+    const intptr_t pa = reinterpret_cast<intptr_t>(a.p), pb = reinterpret_cast<intptr_t>(b.p);
+    if (pa + (m - 1) * a.ld + a.width <= pb || pb + (m - 1) * b.ld + b.width <= pa) return false;
+    if (m == 1 || a.ld != b.ld || a.ld <= 0) return true;
+    const int64_t off = ((pb - pa) % a.ld + a.ld) % a.ld;
+    return off < a.width || off + b.width > a.ld;
+}
 
 // Lets a kernel use `bytes` of dynamic shared memory on the current device: once per kernel and device (`done`, the
 // kernel's own), since the call costs as much host time as a tenth of a launch.

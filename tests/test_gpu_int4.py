@@ -388,6 +388,24 @@ def test_formats_loader_and_groups(sbq):
     assert block.mlp(x).shape == (2, 96)
 
 
+@pytest.mark.parametrize("m", [3, 20, 150])
+def test_output_beside_the_activation(sbq, m):
+    """Columns of one buffer as activation and output; shared bytes are refused."""
+    q, s = weight(64, 128, 64, seed=52)
+    lin = sbq.Int4Linear.from_quantized(q, s, None, group=64)
+    lin.out_dtype = F16
+    both = acts(m, 192, F16, seed=53)
+    x = both[:, :128].clone()
+    lin.forward_into(both[:, :128], both[:, 128:])
+    assert torch.equal(both[:, 128:], lin(x)) and torch.equal(both[:, :128], x)
+    for out in (both[:, :64], both[:, 127:191], both.view(-1)[1:m * 64 + 1].view(m, 64)):
+        with pytest.raises(ValueError, match="overlap"):
+            lin.forward_into(both[:, :128], out)
+    mlp = sbq.FusedGatedMLP(lin, lin, sbq.Int4Linear.from_quantized(*weight(128, 64, 64, seed=54), None, group=64))
+    with pytest.raises(ValueError, match="overlap"):
+        mlp.gateup_into(both[:, :128], both[:, 100:164])
+
+
 def test_refusals(sbq):
     L = sbq._lib
     q, s = weight(32, 64, 32, seed=36)

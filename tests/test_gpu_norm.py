@@ -195,6 +195,32 @@ def test_refusals(sbq):
         sbq.residual_norm(y, r, w)
 
 
+def test_outputs_over_operands(sbq):
+    """An output may lie on an operand with the same rows or beside it in one buffer; anything else is refused."""
+    for d in (96, 333, 20000):
+        m = 5
+        y, r, w = rand(m, d, seed=50), rand(m, d, seed=51), rand(d, seed=52)
+        g = rand(m, d, seed=53)
+        want = sbq.residual_norm(y, r, w, post_weight=w, gate=g, gate_act="silu")
+        for i in range(3):
+            ops = [y.clone(), r.clone(), g.clone()]
+            got = sbq.residual_norm(ops[0], ops[1], w, post_weight=w, gate=ops[2], gate_act="silu", residual_out=ops[i])
+            assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+        both = torch.empty(m, 2 * d, device="cuda")
+        both[:, :d], both[:, d:] = y, r
+        plain = sbq.residual_norm(y, r, w)
+        sbq.residual_norm(both[:, :d], both[:, d:], w, residual_out=both[:, d:])
+        assert torch.equal(both[:, d:], plain[0]) and torch.equal(both[:, :d], y)
+        stack = rand(m + 1, d, seed=54)
+        wide = rand(m, 2 * d, seed=55)
+        for branch, res, out in ((y, stack[1:], stack[:-1]), (stack[1:], r, stack[:-1]), (y, wide[:, :d], wide[:, 1:d + 1]),
+                                 (wide[:, :d], r, wide[:, d - 1:2 * d - 1]), (y, stack[:-1], stack.view(-1)[1:m * d + 1].view(m, d))):
+            with pytest.raises(ValueError, match="overlaps"):
+                sbq.residual_norm(branch, res, w, residual_out=out)
+        with pytest.raises(ValueError, match="overlaps"):  # the same address, elements of another size
+            sbq.residual_norm(stack[:-1].view(F16).view(m, 2 * d)[:, :d], r[:, :], w, residual_out=stack[:-1])
+
+
 @pytest.mark.parametrize("m", [1, 300])
 def test_streams_and_graphs(sbq, m):
     step = sbq.ResidualNorm(rand(768, seed=40), rand(768, seed=41), "sigmoid", 0.5, 2.0).cuda()
