@@ -72,7 +72,9 @@ def residual_norm(branch: torch.Tensor | None, residual: torch.Tensor, pre_weigh
                                  residual_scale=residual_scale, branch_scale=branch_scale, eps=eps, out_dtype=out_dtype,
                                  residual_out=residual_out)
     if torch.is_grad_enabled() and (residual.requires_grad or (branch is not None and branch.requires_grad) or
-                                    (gate is not None and gate.requires_grad)):
+                                    (gate is not None and gate.requires_grad) or
+                                    (pre_weight is not None and pre_weight.requires_grad) or
+                                    (post_weight is not None and post_weight.requires_grad)):
         raise ValueError("residual_norm has no gradient: call it under torch.no_grad() or detach its inputs")
     act = L.GATE_ACTS.get(gate_act)
     if act is None:

@@ -408,7 +408,7 @@ def _raw_stream(device: torch.device) -> int:
 
 def _in_place(x: torch.Tensor, k: int, device: torch.device) -> bool:
     """Whether the library takes x [..., k] where it is, as a decode loop passes it."""
-    return x.dtype in _DTYPE_CODE and x.shape[-1] == k and x.device == device and x.is_contiguous() \
+    return x.dtype in _DTYPE_CODE and x.shape[-1:] == (k,) and x.device == device and x.is_contiguous() \
         and (x.data_ptr() % 16 == 0 or k % 16 != 0)
 
 

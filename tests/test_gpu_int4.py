@@ -424,6 +424,8 @@ def test_refusals(sbq):
     lin = sbq.Int4Linear.from_quantized(q, s, None, group=32)
     with pytest.raises(ValueError, match="feature size"):
         lin(torch.zeros(2, 48, device="cuda"))
+    with pytest.raises(ValueError, match="feature size"):
+        lin(torch.zeros((), device="cuda"))
     with pytest.raises(ValueError, match="output must be"):
         lin.forward_into(torch.zeros(2, 64, device="cuda"), torch.zeros(2, 31, device="cuda"))
     with pytest.raises(ValueError, match="input must be"):

@@ -191,6 +191,13 @@ def test_refusals(sbq):
         sbq.residual_norm(y, r, w[:16])
     with pytest.raises(ValueError, match="no gradient"):
         sbq.residual_norm(y, r.requires_grad_(), w)
+    r.requires_grad_(False)
+    for kw in ({"pre_weight": w}, {"post_weight": w}, {"gate": w}):
+        kw = {name: torch.nn.Parameter(t.clone()) for name, t in kw.items()}
+        with pytest.raises(ValueError, match="no gradient"):
+            sbq.residual_norm(y, r, **kw)
+        with torch.no_grad():
+            sbq.residual_norm(y, r, **kw)
     with torch.no_grad():
         sbq.residual_norm(y, r, w)
 
