@@ -388,6 +388,43 @@ def test_formats_loader_and_groups(sbq):
     assert block.mlp(x).shape == (2, 96)
 
 
+@pytest.mark.parametrize("m,ld", [(3, 1 << 30), (40, 1 << 26), (140, 1 << 24)])
+def test_offsets_past_32_bits(sbq, m, ld):
+    """Rows so far apart that element offsets pass 2^31: the activation's and the result's."""
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    q, s = weight(72, 192, 64, seed=56)
+    lin = sbq.Int4Linear.from_quantized(q, s, None, group=64)
+    far = torch.empty((m - 1) * ld + 512, dtype=F16, device="cuda")
+    x, y = (far[o:].as_strided((m, c), (ld, 1)) for o, c in ((0, 192), (256, 72)))
+    x.copy_(acts(m, 192, F16, seed=57))
+    lin.forward_into(x, y)
+    check(y, x.contiguous(), q, s, 64)
+
+
+@pytest.mark.parametrize("m", [4, 20, 200])
+def test_gateup_of_far_gates(sbq, m):
+    """Gates far out on both sides: silu is 0 or the gate itself, and nothing overflows on the way."""
+    k = 64
+    q = torch.zeros(32, k, dtype=torch.int8, device="cuda")
+    q[:, 0] = 7
+    s = torch.full((32, 1), 0.5, dtype=BF16, device="cuda")
+    up_q = torch.zeros_like(q)
+    up_q[:, 1] = 2
+    gate, up = (sbq.Int4Linear.from_quantized(t, s, None, group=64) for t in (q, up_q))
+    down = sbq.Int4Linear.from_quantized(*weight(k, 32, 32, seed=58), None, group=32)
+    x = torch.zeros(m, k, device="cuda", dtype=F16)
+    x[:, 0] = torch.tensor([-10000.0, -30.0, -24.5, 8.0], device="cuda").repeat(m // 4)  # gates -35000, -105, -86, 28
+    x[:, 1] = 1.0                                                                       # up 1
+    g = x[:, :1].double() * 3.5
+    ref = (g * g.sigmoid()).expand(m, 32)
+    for h_dtype in (F32, F16, BF16):
+        h = sbq.FusedGatedMLP(gate, up, down, h_dtype=h_dtype).gateup(x)
+        # as in test_gateup, with exact gates; silu below 2^-120 may be 0
+        tol = ref.abs() * (8 * 2.0 ** -23 + torch.finfo(h_dtype).eps / 2) + 2.0 ** -118 + (2.0 ** -25 if h_dtype == F16 else 0.0)
+        assert ((h.double() - ref).abs() <= tol).all(), h_dtype
+
+
 @pytest.mark.parametrize("m", [3, 20, 150])
 def test_output_beside_the_activation(sbq, m):
     """Columns of one buffer as activation and output; shared bytes are refused."""

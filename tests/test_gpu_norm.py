@@ -202,6 +202,21 @@ def test_refusals(sbq):
         sbq.residual_norm(y, r, w)
 
 
+@pytest.mark.parametrize("d", [96, 333, 20000])
+def test_offsets_past_32_bits(sbq, d):
+    """Rows so far apart that element offsets pass 2^31, in place."""
+    m, ld = 4, 1 << 30
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    far = torch.empty((m - 1) * ld + d, dtype=BF16, device="cuda").as_strided((m, d), (ld, 1))
+    y, r, w = rand(m, d, seed=56, dtype=BF16), rand(m, d, seed=57, dtype=BF16), rand(d, seed=58)
+    far.copy_(r)
+    x = sbq.residual_norm(y, far, w, residual_out=far)[1]
+    wr, wx, er, ex = reference(y, r, w, None, None, "none", 1.0, 1.0, 1e-6)
+    check(far, wr, er)
+    check(x, wx, ex)
+
+
 def test_outputs_over_operands(sbq):
     """An output may lie on an operand with the same rows or beside it in one buffer; anything else is refused."""
     for d in (96, 333, 20000):
