@@ -49,6 +49,10 @@ __device__ __forceinline__ void w4_store_rowmul(float smax, float* rowmul) {
     }
 }
 
+// Last statement of a packing kernel.  A product queued right after it reads the weight before it waits for its
+// predecessor and may start as soon as this grid's CTAs have ended: every store must be visible to the device by then.
+__device__ __forceinline__ void w4_settle() { __threadfence(); }
+
 // One CTA per packed row (rows past n are written as zeros), one thread per 8 columns; the threads of a
 // group are neighbouring lanes.
 template <typename T>
@@ -88,6 +92,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const T* __re
         }
     }
     w4_store_rowmul(smax, rowmul + r);
+    w4_settle();
 }
 
 // Given codes and scales (row strides ldq, lds) -> packed.  Codes outside [-8, 7] are clamped to it.
@@ -119,6 +124,7 @@ __global__ void __launch_bounds__(kPackThreads) w4_pack_kernel(const int8_t* __r
         }
     }
     w4_store_rowmul(smax, rowmul + r);
+    w4_settle();
 }
 
 // Packed -> codes [n, k] and scales [n, ceil(k / group)] (either may be null).

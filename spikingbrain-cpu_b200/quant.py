@@ -453,6 +453,9 @@ class Int4Linear(nn.Module):
         mod = cls.__new__(cls)
         nn.Module.__init__(mod)
         mod._adopt((packed, scales, rowmul), (out_features, in_features), bias, group)
+        # the products read the weight before they wait for the kernel before them: this one stands between them and a
+        # kernel that has just written the buffers
+        torch.zeros(1, device=packed.device)
         return mod
 
     @classmethod
