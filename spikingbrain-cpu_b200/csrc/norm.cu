@@ -11,7 +11,7 @@
 //
 // The bytes bound it.  Measured on B200: 8192 x 4096, fp32 in and fp16 out, without a post norm 69.5 us (6.8 TB/s, 1.03 of
 // the measured copy rate), with it 75 us; 1 x 4096 2.9 us (a launch); 16-bit rows with a gate per element, which have
-// half the bytes per element and twice the arithmetic, 3001 x 2560 22 us (3.5 TB/s) and 3001 x 2559 36 us.
+// half the bytes per element and twice the arithmetic, 3001 x 2560 19.7 us (3.9 TB/s) and 3001 x 2559 29 us.
 #include "w4_host.cuh"
 
 namespace sbq {
@@ -38,14 +38,7 @@ __device__ __forceinline__ float ld1(const void* p, int dtype, int64_t i) {
     return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
 }
 
-__device__ __forceinline__ void ld8(const void* p, int dtype, int64_t i, float (&v)[8]) {
-    if (dtype == SBQ_F32) {
-        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
-        const float4 a = q[0], b = q[1];
-        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        return;
-    }
-    const uint4 a = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i);
+__device__ __forceinline__ void unpack8(const uint4& a, int dtype, float (&v)[8]) {
     const uint32_t u[4] = {a.x, a.y, a.z, a.w};
     if (dtype == SBQ_F16) {
 #pragma unroll
@@ -57,6 +50,16 @@ __device__ __forceinline__ void ld8(const void* p, int dtype, int64_t i, float (
 #pragma unroll
         for (int j = 0; j < 4; ++j) v[2 * j] = __uint_as_float(u[j] << 16), v[2 * j + 1] = __uint_as_float(u[j] & 0xFFFF0000u);
     }
+}
+
+__device__ __forceinline__ void ld8(const void* p, int dtype, int64_t i, float (&v)[8]) {
+    if (dtype == SBQ_F32) {
+        const float4* q = reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        const float4 a = q[0], b = q[1];
+        v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
+        return;
+    }
+    unpack8(*reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(p) + i), dtype, v);
 }
 
 __device__ __forceinline__ void st8(void* p, int dtype, int64_t i, const float (&v)[8]) {
@@ -310,9 +313,17 @@ __device__ __forceinline__ float square8(const float (&r)[8], float ss) {
     return ss;
 }
 
+// CTAs per SM that the register kernel is compiled for (above 512 threads: two of them as long as that spills little).
+__host__ __device__ constexpr int norm_ctas(int threads, int chunks, int mode) {
+    return threads == 512                 ? (mode == kAligned ? 4 : 3)
+           : chunks == 1 && threads == 768  ? (mode == kShifted ? 1 : 2)
+           : chunks == 1 && threads == 1024 ? (mode == kAligned ? 2 : 1)
+                                            : 1;
+}
+
 // V chunks of 8 elements per thread, everything a row needs from memory (but the weights) requested at the start.
 template <int TPR, int V, int MAXT, int MODE, bool GATE>
-__global__ void __launch_bounds__(MAXT, MAXT == 512 ? (MODE == kAligned ? 4 : 3) : 1) norm_kernel(const NormParams p) {
+__global__ void __launch_bounds__(MAXT, norm_ctas(MAXT, V, MODE)) norm_kernel(const NormParams p) {
     __shared__ float part[2][32];
     const int n = row_threads<TPR>(), tid = (int)threadIdx.x % n;
     const int64_t first = TPR ? (int64_t)blockIdx.x * (MAXT / (TPR ? TPR : 1)) + threadIdx.x / n : (int64_t)blockIdx.x;
@@ -352,6 +363,135 @@ __global__ void __launch_bounds__(MAXT, MAXT == 512 ? (MODE == kAligned ? 4 : 3)
 #pragma unroll
         for (int i = 0; i < 8; ++i) r[v][i] = r[v][i] * inv * w[i];
         if (live) norm_store<TPR, MODE>(p.x, p.x_dtype, row * p.ldx, v, tid, p.d, phase, r[v]);
+    }
+}
+
+// The same with the row in shared memory: each thread copies the chunks that it will read itself (so that nobody waits for
+// another's copies) into 16-byte planes [warp][chunk][plane][lane], and goes over them in rolled loops.  Registers no longer
+// grow with the chunks of a thread, so a thread can take several, which share what a row costs besides its elements (sums
+// over the CTA, square roots, addresses).
+template <bool L1>
+__device__ __forceinline__ void stage16(uint4* dst, const void* src) {
+    const uint32_t to = (uint32_t)__cvta_generic_to_shared(dst);
+    if (L1)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+    else
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(src) : "memory");
+}
+
+// Requests one chunk of an operand; what lies outside the row is dropped by stage_read.  A chunk of fp32 is a whole
+// sector that is copied in two halves: through L1, or it would be fetched twice (8192 x 4096: 119 and 103 us).
+template <int MODE>
+__device__ __forceinline__ void stage_row(const void* p, int dtype, int64_t row, int64_t ld, int c0, const NormParams& q, uint4* dst) {
+    const int64_t at = row * ld + c0;
+    if (c0 >= q.d) return;
+    bool whole = true;
+    if (MODE != kAligned) whole = (c0 >= 0 && c0 + 8 <= q.d) || (at >= 0 && at + 8 <= (q.m - 1) * ld + q.d);
+    if (whole) {
+        if (dtype == SBQ_F32) {
+            stage16<true>(dst, static_cast<const float*>(p) + at);
+            stage16<true>(dst + 32, static_cast<const float*>(p) + at + 4);
+        } else {
+            stage16<false>(dst, static_cast<const uint16_t*>(p) + at);
+        }
+    } else {
+        for (int i = 0; i < 8; ++i) {
+            if ((unsigned)(c0 + i) >= (unsigned)q.d) continue;
+            if (dtype == SBQ_F32)
+                reinterpret_cast<float*>(dst + (i >> 2) * 32)[i & 3] = static_cast<const float*>(p)[at + i];
+            else
+                reinterpret_cast<uint16_t*>(dst)[i] = static_cast<const uint16_t*>(p)[at + i];
+        }
+    }
+}
+
+template <int MODE>
+__device__ __forceinline__ void stage_read(const uint4* src, int dtype, int c0, int d, float (&v)[8]) {
+    const uint4 a = src[0];
+    if (dtype == SBQ_F32) {
+        const uint4 b = src[32];
+        const uint32_t u[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = __uint_as_float(u[i]);
+    } else {
+        unpack8(a, dtype, v);
+    }
+    if (MODE == kShifted && (c0 < 0 || c0 + 8 > d)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if ((unsigned)(c0 + i) >= (unsigned)d) v[i] = 0.0f;
+    }
+}
+
+constexpr int kStagedThreads = 512;
+constexpr int kStagedBytes = 220 * 1024, kStagedHalf = 110 * 1024;  // one and two CTAs per SM
+template <int MODE, bool GATE>
+__global__ void __launch_bounds__(kStagedThreads, 3) norm_staged_kernel(const NormParams p, int chunks, int y_planes, int planes) {
+    extern __shared__ uint4 stage[];
+    __shared__ float part[2][32];
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    const int tid = threadIdx.x, d = p.d, hop = (int)blockDim.x * 8, step = planes * 32;
+    const int64_t row = blockIdx.x;
+    const int phase = norm_phase<MODE>(p, row), first = tid * 8 - phase;
+    uint4* const mine = stage + (tid >> 5) * chunks * step + (tid & 31);
+    const int at_r = y_planes * 32, at_g = at_r + (p.r_dtype == SBQ_F32 ? 64 : 32);
+    const bool staged_gate = GATE && p.gcol && p.ldg;
+    uint4* s = mine;
+    if (p.y)
+        for (int v = 0, c = first; v < chunks; ++v, c += hop, s += step) stage_row<MODE>(p.y, p.y_dtype, row, p.ldy, c, p, s);
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    s = mine;
+    for (int v = 0, c = first; v < chunks; ++v, c += hop, s += step) {
+        stage_row<MODE>(p.r, p.r_dtype, row, p.ldr, c, p, s + at_r);
+        if (staged_gate) stage_row<MODE>(p.gate, p.g_dtype, row, p.ldg, c, p, s + at_g);
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    float inv = 1.0f, ss = 0.0f;
+    if (p.y && p.w_post) {
+        asm volatile("cp.async.wait_group 1;" ::: "memory");
+        s = mine;
+        for (int v = 0, c = first; v < chunks; ++v, c += hop, s += step) {
+            if (c >= d) continue;
+            float y[8];
+            stage_read<MODE>(s, p.y_dtype, c, d, y);
+            ss += square8(y, 0.0f);
+        }
+        inv = rsqrtf(row_sum<0>(ss, part[0]) / (float)d + p.eps);
+        ss = 0.0f;
+    }
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    s = mine;
+    for (int v = 0, c = first; v < chunks; ++v, c += hop, s += step) {
+        if (c >= d) continue;
+        float y[8], r[8], g[8];
+        if (p.y) stage_read<MODE>(s, p.y_dtype, c, d, y);
+        stage_read<MODE>(s + at_r, p.r_dtype, c, d, r);
+        if (GATE) {
+            if (staged_gate)
+                stage_read<MODE>(s + at_g, p.g_dtype, c, d, g);
+            else
+                norm_gate<0, MODE>(p, row, v, tid, phase, g);
+        }
+        norm_combine<0, MODE, GATE>(p, v, tid, phase, inv, y, g, r);
+        ss += square8(r, 0.0f);
+        if (p.r_out) norm_store<0, MODE>(p.r_out, p.r_dtype, row * p.ldro, v, tid, d, phase, r);
+        if (p.x) {  // r' in fp32 takes the place of the chunk's operands
+            s[0] = make_uint4(__float_as_uint(r[0]), __float_as_uint(r[1]), __float_as_uint(r[2]), __float_as_uint(r[3]));
+            s[32] = make_uint4(__float_as_uint(r[4]), __float_as_uint(r[5]), __float_as_uint(r[6]), __float_as_uint(r[7]));
+        }
+    }
+    if (!p.x) return;
+    inv = rsqrtf(row_sum<0>(ss, part[1]) / (float)d + p.eps);
+    s = mine;
+    for (int v = 0, c = first; v < chunks; ++v, c += hop, s += step) {
+        if (c >= d) continue;
+        float r[8], w[8];
+        stage_read<kAligned>(s, SBQ_F32, c, d, r);
+        norm_load_vec<0, MODE>(p.w_pre, SBQ_F32, v, tid, d, phase, w);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) r[i] = r[i] * inv * w[i];
+        norm_store<0, MODE>(p.x, p.x_dtype, row * p.ldx, v, tid, d, phase, r);
     }
 }
 
@@ -413,24 +553,68 @@ static cudaError_t launch_norm(const NormParams& p, int mode, int threads, cudaS
     return launch_norm_m<TPR, V, MAXT, kStrided>(p, threads, s);
 }
 
+template <int MODE, bool GATE>
+static cudaError_t launch_norm_staged_g(const NormParams& p, int threads, int chunks, int planes, cudaStream_t s) {
+    static std::atomic<uint64_t> allowed{0};
+    const cudaError_t e = w4_allow_smem(norm_staged_kernel<MODE, GATE>, kStagedBytes, allowed);
+    if (e != cudaSuccess) return e;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3((unsigned)p.m);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = (size_t)threads * chunks * planes * 16;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, norm_staged_kernel<MODE, GATE>, p, chunks, p.y ? (p.y_dtype == SBQ_F32 ? 2 : 1) : 0, planes);
+}
+
+template <int MODE>
+static cudaError_t launch_norm_staged(const NormParams& p, int threads, int chunks, int planes, cudaStream_t s) {
+    return p.gate ? launch_norm_staged_g<MODE, true>(p, threads, chunks, planes, s)
+                  : launch_norm_staged_g<MODE, false>(p, threads, chunks, planes, s);
+}
+
 template <int MODE>
 static cudaError_t launch_norm_long(const NormParams& p, cudaStream_t s) {
     return p.gate ? w4_launch(norm_long_kernel<MODE, true>, (unsigned)p.m, kLongThreads, 0, s, p)
                   : w4_launch(norm_long_kernel<MODE, false>, (unsigned)p.m, kLongThreads, 0, s, p);
 }
 
-// One chunk per thread up to 8192 columns (1024 threads), on as many warps as the row fills.  Measured on B200, one and
-// two chunks: 8192 x 4096 with both norms 75 and 78 us, gated 3001 x 2560 26 and 31 us, 3001 x 2559 38 and 53 us.
-// What hides a row's chain of loads and sums is other rows on the SM: 32 registers per thread (40 for the
-// shifted accesses, which spill at 32) took the gated cases to 22 and 36 us; weights requested early, or
-// persistent CTAs that request their next row early, cost registers and were slower.
+// In registers, one chunk per thread up to 8192 columns (1024 threads), on as many warps as the row fills: two chunks
+// hold twice the registers (8192 x 4096 fp32 with both norms 75 and 78 us).  What hides a row's chain of loads and sums is
+// other rows on the SM, so registers are held down to what norm_ctas needs (8192 x 8192 fp32: one CTA per SM 219, two 160 us).
+// Measured on B200, in registers and staged, two norms and a full gate in bf16: 3001 x 2560 22.2 and 19.7 us, 3001 x 2559
+// 35.6 and 29.1, 3001 x 6144 58.8 and 44.5, 3001 x 8191 174 and 77, 3001 x 20480 241 and 184; one wave of rows or less is
+// faster in registers (592 x 4096 7.7 and 9.8 us: a thread's chunks come one after the other), and so are fp32 rows (3001 x
+// 4096 31.9 and 40.4 us).  Weights requested early, persistent CTAs that request their next row early, and one warp
+// per row were slower.
 static cudaError_t launch_norm_any(const NormParams& p, int mode, cudaStream_t s) {
     const int span = p.d + (mode == kShifted ? 7 : 0);
+    // More elements than one wave of full SMs takes at 8 per thread, in rows that are worth several chunks per thread: the
+    // staged kernel for 16-bit rows, and for others where the registers leave one CTA per SM.  Two CTAs of it must fit on
+    // an SM if the registers do better than one (aligned rows up to 16384 columns).
+    if (mode != kStrided && span > 1024 && p.m * p.d > (int64_t)16384 * w4_sm_count()) {
+        const bool full_gate = p.gate && p.gcol && p.ldg, y32 = p.y && p.y_dtype == SBQ_F32, r32 = p.r_dtype == SBQ_F32,
+                   g32 = full_gate && p.g_dtype == SBQ_F32;
+        int planes = 1 + r32 + (p.y != nullptr) + y32 + full_gate + g32;
+        planes = planes < 2 ? 2 : planes;  // r' in fp32
+        const int pieces = (span + 7) / 8, most = (int)ceil_div(pieces, kStagedThreads), chunks = most < 2 ? 2 : most;
+        const int threads = (int)ceil_div(ceil_div(pieces, chunks), 32) * 32;
+        const bool wide = y32 || r32 || g32, crowded = span > (mode == kShifted ? 4096 : 8192);
+        const int room = mode == kShifted || span > 16384 ? kStagedBytes : kStagedHalf;
+        if ((!wide || crowded) && (int64_t)threads * chunks * planes * 16 <= room)
+            return mode == kAligned ? launch_norm_staged<kAligned>(p, threads, chunks, planes, s)
+                                    : launch_norm_staged<kShifted>(p, threads, chunks, planes, s);
+    }
     if (span <= 64) return launch_norm<8, 1, 256>(p, mode, 256, s);
     if (span <= 128) return launch_norm<16, 1, 256>(p, mode, 256, s);
     if (span <= 256) return launch_norm<32, 1, 256>(p, mode, 256, s);
     const int one = (span + 255) / 256 * 32, two = (span + 511) / 512 * 32;  // threads for one or two chunks each
     if (one <= 512) return launch_norm<0, 1, 512>(p, mode, one, s);
+    if (one <= 768) return launch_norm<0, 1, 768>(p, mode, one, s);
     if (one <= 1024) return launch_norm<0, 1, 1024>(p, mode, one, s);
     if (two <= 1024) return launch_norm<0, 2, 1024>(p, mode, two, s);
     if (mode == kAligned) return launch_norm_long<kAligned>(p, s);

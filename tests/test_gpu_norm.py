@@ -202,6 +202,33 @@ def test_refusals(sbq):
         sbq.residual_norm(y, r, w)
 
 
+@pytest.mark.parametrize("m,d", [(2400, 1032), (2400, 1029), (1000, 2559), (1000, 2560), (700, 4095), (420, 6143), (310, 8192), (310, 8191),
+                                 (210, 12287), (160, 16384), (160, 16383), (130, 20480), (130, 20479), (90, 30001)])
+@pytest.mark.parametrize("gate", ["none", "vector", "token", "full"])
+def test_many_rows(sbq, m, d, gate):
+    """More rows than the SMs hold at once, every type, a row of NaN and rows at their ends."""
+    for i, (yt, rt, xt) in enumerate(((BF16, BF16, BF16), (F16, F32, F16), (F32, F32, F32), (BF16, F16, F32))):
+        y, r = rand(m, d, seed=60 + i, dtype=yt), rand(m, d, seed=70 + i, dtype=rt)
+        w, wp = 1 + rand(d, seed=80, scale=0.1), 1 + rand(d, seed=81, scale=0.1)
+        g = {"none": None, "vector": rand(d, seed=82), "token": rand(m, 1, seed=83, dtype=yt), "full": rand(m, d, seed=84, dtype=yt)}[gate]
+        y[m // 2, d - 1] = float("nan")
+        post = wp if i != 3 else None
+        mine = r.clone()
+        got_r, got_x = sbq.residual_norm(y, mine, w, post_weight=post, gate=g, gate_act="sigmoid", out_dtype=xt, residual_out=mine)
+        assert torch.isnan(got_x[m // 2]).all() and (torch.isnan(got_r[m // 2]).all() if post is not None else True)
+        keep = [k for k in range(m) if k != m // 2]
+        wr, wx, er, ex = reference(y[keep], r[keep], w, post, g if g is None or g.dim() == 1 else g[keep], "sigmoid", 1.0, 1.0, 1e-6)
+        check(got_r[keep], wr, er)
+        check(got_x[keep], wx, ex)
+        # without the branch, and without the norm
+        nr, nx = sbq.residual_norm(None, r, w, residual_scale=0.5)
+        wr, wx, er, ex = reference(None, r, w, None, None, "none", 0.5, 1.0, 1e-6)
+        check(nr, wr, er)
+        check(nx, wx, ex)
+        only = sbq.residual_norm(y[keep], r[keep], None, branch_scale=2.0)[0]
+        check(only, *[v for k, v in enumerate(reference(y[keep], r[keep], None, None, None, "none", 1.0, 2.0, 1e-6)) if k in (0, 2)])
+
+
 @pytest.mark.parametrize("d", [96, 333, 20000])
 def test_offsets_past_32_bits(sbq, d):
     """Rows so far apart that element offsets pass 2^31, in place."""
