@@ -389,7 +389,7 @@ SBQ_API int sbq_w4_unpack(const void* packed, const void* scales, int64_t n, int
                           int64_t ldq, void* scale, int64_t lds, void* stream);
 
 /* Workspace of sbq_linear_w4 (matrices = 1) / sbq_mlp_gateup_w4 (2) on the current device: the activation where it
- * is not read in place (fp32 x, bf16 x above 16 rows, k not a multiple of 16) and, above 128 rows, the partial
+ * is not read in place (fp32 x, bf16 x above 16 rows, k not a multiple of 16) and, above 64 rows, the partial
  * sums of tiles that are cut along k.  Its contents need not be kept between calls. */
 SBQ_API size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_dtype, int matrices);
 

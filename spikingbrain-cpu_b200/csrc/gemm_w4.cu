@@ -149,7 +149,7 @@ __device__ __forceinline__ int w4_channel(int n0, int row) { return n0 + (NMAT =
 __device__ __forceinline__ void group_sync(int grp) { asm volatile("bar.sync %0, 128;" ::"r"(1 + grp) : "memory"); }
 
 // ---------------------------------------------------------------------------------------------
-// More than 128 rows: CTA pairs (cta_group::2), persistent.  A pair computes tiles of 256 channels x TOK tokens one
+// Many rows: CTA pairs (cta_group::2), persistent.  A pair computes tiles of 256 channels x TOK tokens one
 // after the other; blocks of 128 k run through the rings without a break between tiles.  Each CTA converts its
 // own 128 channels and loads half of the tokens.  With two matrices a CTA's lanes 0..63 are gate channels and
 // lanes 64..127 the same channels of the up projection (128 channels per pair).
@@ -583,7 +583,7 @@ __global__ void __launch_bounds__(2 * kW4Rows) w4_reduce_kernel(const GemmW4Para
 }
 
 // ---------------------------------------------------------------------------------------------
-// 17..128 rows: 128 channels x 64 tokens per CTA, two CTAs per SM, k split over the CTAs of a cluster when
+// Few rows: 128 channels x 64 tokens per CTA, two CTAs per SM, k split over the CTAs of a cluster when
 // the tiles alone are too few: each pushes its fp32 sums into the shared memory of the CTA that owns the
 // channel, which adds them in part order.  The two converter warpgroups take alternate blocks (each warp on half of
 // every block, as in the pair kernel, was 15 % slower: with two CTAs on an SM the waits of a block count) and both
@@ -877,9 +877,9 @@ static cudaError_t launch_maps(dim3 grid, int threads, int smem, int parts, cuda
 }
 
 template <int PARTS, int NMAT, int GPT>
-static cudaError_t launch_gemm_w4(int tok, int npairs, const W4Maps& m, GemmW4Params p, cudaStream_t s) {
+static cudaError_t launch_gemm_w4(bool small, int npairs, const W4Maps& m, GemmW4Params p, cudaStream_t s) {
     p.seg_blocks = p.y_dtype == SBQ_F32 ? kSegSteps / (8 * PARTS) : p.kt;
-    if (tok == kSTok4)
+    if (small)
         return launch_maps<gemm_w4_small_kernel<PARTS, NMAT, GPT>>(
                            dim3((unsigned)ceil_div(p.n, kW4Rows / NMAT), (unsigned)ceil_div(p.m, kSTok4), (unsigned)p.parts),
                            kW4Threads, W4Small<PARTS>::kBytes, p.parts, s, m, p);
@@ -888,54 +888,70 @@ static cudaError_t launch_gemm_w4(int tok, int npairs, const W4Maps& m, GemmW4Pa
 }
 
 template <int PARTS, int NMAT>
-static cudaError_t launch_gemm_w4_g(int gpt, int tok, int npairs, const W4Maps& m, const GemmW4Params& p, cudaStream_t s) {
-    if (gpt == 1) return launch_gemm_w4<PARTS, NMAT, 1>(tok, npairs, m, p, s);
-    if (gpt == 2) return launch_gemm_w4<PARTS, NMAT, 2>(tok, npairs, m, p, s);
-    return launch_gemm_w4<PARTS, NMAT, 4>(tok, npairs, m, p, s);
+static cudaError_t launch_gemm_w4_g(int gpt, bool small, int npairs, const W4Maps& m, const GemmW4Params& p, cudaStream_t s) {
+    if (gpt == 1) return launch_gemm_w4<PARTS, NMAT, 1>(small, npairs, m, p, s);
+    if (gpt == 2) return launch_gemm_w4<PARTS, NMAT, 2>(small, npairs, m, p, s);
+    return launch_gemm_w4<PARTS, NMAT, 4>(small, npairs, m, p, s);
 }
 
-constexpr int64_t kW4SmallRows = 128;
-
-// The pair kernel's schedule: tokens per tile, whole rounds of tiles over the pairs, and the tiles left over cut into
-// parts along k.  It takes the shortest time by a model of a block of 128 k: eight MMAs (two parts of x: sixteen) of
-// 50 + 0.39 N cycles, or the conversion's 0.33 us, whichever is longer.  Cutting costs about 13 us (storing the sums,
-// a second launch, reading them) and 50 ns for every part's 256 KiB.
-// Measured on B200 at 256 tokens per tile, uncut and cut: fp32 300 x 12288 x 4096 (32 tiles on 74 pairs) 166 and 96 us (73 us
-// with 160-token tiles, cut), fp32 512 x 2560 x 9728 (2 tiles left of 76) 77 and 58 us; fp16 512 x 2560 x 9728 31 and
-// 35 us, fp16 2048 x 4096 x 12288 (14 left of 384) 143 and 144 us: those two stay uncut.
+// Which kernel, and its schedule, by a model of the time (us) fitted to measurements on B200 (k 2560 to 12288, n 1024 to
+// 12288, 130 to 1024 rows; mostly within 10 %).  It counts blocks of 128 k on the longest path.
+//   Pair kernel: eight MMAs per block (two parts of x: sixteen, and two more for the pauses in which the accumulator is
+//   read) of 50 + 0.39 N cycles, or what it takes to bring and convert the operands, whichever is longer; tiles in rounds over the pairs, the
+//   last round's cut along k or not.  Cutting costs 3 us (a second launch) and 80 ns for every part's 256 KiB of sums,
+//   and the cut tiles end no earlier than the stores of the round before.
+//   Small kernel: 64 tokens per tile, two CTAs per SM; with k split a CTA shares its SM all the time.
+// Fp16 rows: 200 x 4096 x 4096 18.6 us (16 tiles in four parts; 64 narrow tiles uncut 23.0), 300 x 9728 x 2560 27.1 (20 in three;
+// uncut 46.8), 512 x 4096 x 4096 23.9 (64 uncut), 300 x 4096 x 1024 11.7 with the small kernel (cut tiles 14.8, uncut 21.0).
 struct W4Plan {
+    int small_parts;  // small kernel: CTAs of a cluster along k; 0: pair kernel
     int tok, npairs, rounds, tail_tiles, tail_parts;
 };
 
 static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, bool split, int nmat) {
-    const int64_t cols = ceil_div(n, 2 * kW4Rows / nmat), pairs = w4_sm_count() / 2, kt = w4_tiles_k(k);
+    const int64_t sms = w4_sm_count(), pairs = sms / 2, kt = w4_tiles_k(k);
     W4Plan best{};
-    double best_t = 1e30;
+    // k parts per tile (the cluster size): the largest power of two up to 8 that keeps the grid within 7/8 of the
+    // CTA slots (two per SM) and gives every part at least two blocks.  A cluster needs all of its CTAs in one
+    // GPC at once: 64 x 4096 x 12288 (96 tiles) takes 20.1 us with 2 parts, 28.2 us with 3 (288 of 296 slots)
+    const int64_t small_tiles = ceil_div(n, kW4Rows / nmat) * ceil_div(m, kSTok4);
+    int64_t parts = 1;
+    while (parts < 8 && small_tiles * (2 * parts) * 8 <= 2 * sms * 7 && kt / (2 * parts) >= 2) parts *= 2;
+    best.small_parts = (int)parts;
+    if (m <= kSTok4) return best;  // a pair's tile would be no fuller
+    const int64_t waves = ceil_div(small_tiles * parts, 2 * sms);
+    const double small_block = parts > 1 ? (split ? 1.4 : 0.84) : waves > 1 ? (split ? 1.25 : 0.68) : (split ? 1.15 : 0.57);
+    double best_t = (split ? 7.5 : 6.5) + (double)(waves * ceil_div(kt, parts)) * small_block;
     // with two matrices a taker warpgroup finishes whole sets of 32 tokens
-    for (int tok = kTok; tok >= 32 * nmat; tok -= 32 * nmat) {
-        const int64_t tiles = cols * ceil_div(m, tok), rounds = tiles / pairs, tail = tiles % pairs;
-        const double mma = (split ? 16 : 8) * (50 + 0.39 * tok) / 1850, block = mma > 0.33 ? mma : 0.33;
-        W4Plan pl{tok, 0, (int)rounds, (int)tail, 1};
-        double least = (double)((rounds + (tail > 0)) * kt) * block;
-        for (int64_t parts = 2; parts <= 16 && tail > 0 && parts * tail <= pairs && 2 * parts <= kt; ++parts) {
-            const double t = (double)(rounds * kt + ceil_div(kt, parts)) * block + 13.0 + 0.05 * (double)(parts * tail);
-            if (t < least) least = t, pl.tail_parts = (int)parts;
+    const int set = 32 * nmat, widest = m < kTok ? (int)ceil_div(m, set) * set : kTok;
+    for (int tok = widest; tok >= set; tok -= set) {
+        const int64_t tiles = ceil_div(n, 2 * kW4Rows / nmat) * ceil_div(m, tok), rounds = tiles / pairs, tail = tiles % pairs;
+        const double mma = (split ? 18 : 8) * (50 + 0.39 * tok) / 1850, least = split ? 0.92 : 0.53,
+                     block = mma > least ? mma : least, fixed = (split ? 10 : 8) + (double)(rounds * kt) * block;
+        for (int64_t cut = 1; cut == 1 || (cut <= 16 && cut * tail <= pairs && 2 * cut <= kt); ++cut) {
+            double end = tail > 0 ? (double)ceil_div(kt, cut) * block : 0.0;
+            if (cut > 1) {
+                if (rounds > 0 && end < 8.0) end = 8.0;
+                end += 3.0 + 0.08 * (double)(cut * tail) * tok / kTok;
+            }
+            // a schedule with more tiles or parts must gain 3 %: it reads more than the model knows
+            if (fixed + end < 0.97 * best_t) {
+                best_t = fixed + end;
+                best = W4Plan{0, tok, (int)(rounds > 0 ? pairs : tail * cut), (int)rounds, (int)tail, (int)cut};
+            }
+            if (tail == 0) break;
         }
-        pl.npairs = rounds > 0 ? (int)pairs : pl.tail_tiles * pl.tail_parts;
-        // a narrower tile must gain 3 %: it reads the weight more often than the model knows
-        if (least < 0.97 * best_t) best_t = least, best = pl;
     }
     return best;
 }
 
 size_t gemm_w4_workspace(int64_t m, int64_t n, int64_t k, bool split, int nmat) {
-    if (m <= kW4SmallRows) return 0;
     const W4Plan pl = w4_plan(m, n, k, split, nmat);
-    return pl.tail_parts > 1 ? (size_t)pl.tail_tiles * pl.tail_parts * kTok * 2 * kW4Rows * 4 : 0;
+    return !pl.small_parts && pl.tail_parts > 1 ? (size_t)pl.tail_tiles * pl.tail_parts * kTok * 2 * kW4Rows * 4 : 0;
 }
 
 int gemm_w4_run(const W4Call& c, const W4Acts& x) {
-    const int nmat = c.w[1].packed ? 2 : 1, ch = kW4Rows / nmat, sms = w4_sm_count();
+    const int nmat = c.w[1].packed ? 2 : 1, ch = kW4Rows / nmat;
     GemmW4Params p{};
     p.m = (int)c.m;
     p.n = (int)c.n;
@@ -948,16 +964,11 @@ int gemm_w4_run(const W4Call& c, const W4Acts& x) {
     p.y = c.y;
     p.ldy = c.ldy;
     p.y_dtype = c.y_dtype;
-    const int tok = c.m <= kW4SmallRows ? kSTok4 : kTok;
-    W4Plan pl{};
-    if (tok == kSTok4) {
-        // k parts per tile (the cluster size): the largest power of two up to 8 that keeps the grid within 7/8 of the
-        // CTA slots (two per SM) and gives every part at least two blocks.  A cluster needs all of its CTAs in one
-        // GPC at once: 64 x 4096 x 12288 (96 tiles) takes 20.1 us with 2 parts, 28.2 us with 3 (288 of 296 slots)
-        const int64_t tiles = ceil_div(c.n, ch) * ceil_div(c.m, kSTok4);
-        while (p.parts < 8 && tiles * (2 * p.parts) * 8 <= (int64_t)2 * sms * 7 && p.kt / (2 * p.parts) >= 2) p.parts *= 2;
+    const W4Plan pl = w4_plan(c.m, c.n, c.k, x.part[1] != nullptr, nmat);
+    const bool small = pl.small_parts > 0;
+    if (small) {
+        p.parts = pl.small_parts;
     } else {
-        pl = w4_plan(c.m, c.n, c.k, x.part[1] != nullptr, nmat);
         p.rounds = pl.rounds;
         p.tail_tiles = pl.tail_tiles;
         p.tail_parts = pl.tail_parts;
@@ -965,12 +976,12 @@ int gemm_w4_run(const W4Call& c, const W4Acts& x) {
         p.partial = static_cast<float*>(x.scratch);
     }
     W4Maps maps;
-    const int st = tok == kSTok4 ? make_maps(maps, c, x, kSTok4, ch) : make_maps(maps, c, x, p.tok / 2, ch);
+    const int st = make_maps(maps, c, x, small ? kSTok4 : p.tok / 2, ch);
     if (st) return st;
-    cudaError_t e = x.part[1] ? (nmat == 2 ? launch_gemm_w4_g<2, 2>(c.gpt, tok, pl.npairs, maps, p, c.stream)
-                                           : launch_gemm_w4_g<2, 1>(c.gpt, tok, pl.npairs, maps, p, c.stream))
-                              : (nmat == 2 ? launch_gemm_w4_g<1, 2>(c.gpt, tok, pl.npairs, maps, p, c.stream)
-                                           : launch_gemm_w4_g<1, 1>(c.gpt, tok, pl.npairs, maps, p, c.stream));
+    cudaError_t e = x.part[1] ? (nmat == 2 ? launch_gemm_w4_g<2, 2>(c.gpt, small, pl.npairs, maps, p, c.stream)
+                                           : launch_gemm_w4_g<2, 1>(c.gpt, small, pl.npairs, maps, p, c.stream))
+                              : (nmat == 2 ? launch_gemm_w4_g<1, 2>(c.gpt, small, pl.npairs, maps, p, c.stream)
+                                           : launch_gemm_w4_g<1, 1>(c.gpt, small, pl.npairs, maps, p, c.stream));
     if (e == cudaSuccess && p.tail_parts > 1) {
         cudaLaunchConfig_t cfg{};
         cfg.gridDim = dim3((unsigned)(kTok / (4 * nmat)), (unsigned)pl.tail_tiles);

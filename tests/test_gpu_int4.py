@@ -206,6 +206,44 @@ def test_gateup(sbq, m, x_dtype, n, k, group):
         assert torch.equal(mlp(x), down(h))
 
 
+# tiles of 96 to 256 tokens, less and more than one for every pair of SMs, whole and cut along k
+MANY = [(2100, 2001, 640), (1300, 5003, 515), (200, 12100, 900), (512, 9500, 2600), (300, 4100, 4100), (90, 900, 9000), (4000, 2500, 700),
+        (77, 40000, 300), (333, 700, 4001), (2500, 2100, 130)]
+
+
+@pytest.mark.parametrize("m,n,k", MANY)
+@pytest.mark.parametrize("x_dtype", [F16, BF16, F32])
+def test_many_rows(sbq, m, n, k, x_dtype):
+    q, s = weight(n, k, 64, seed=60)
+    lin = sbq.Int4Linear.from_quantized(q, s, acts(1, n, F32, seed=61)[0], group=64)
+    x = acts(m, k, x_dtype, seed=62)
+    for y_dtype in (F32, F16):
+        lin.out_dtype = y_dtype
+        y = lin(x)
+        check(y, x, q, s, 64, bias=lin.bias)
+        assert torch.equal(y, lin(x))
+
+
+@pytest.mark.parametrize("m,n,k", MANY)
+@pytest.mark.parametrize("x_dtype", [BF16, F32])
+def test_gateup_many_rows(sbq, m, n, k, x_dtype):
+    qg, sg = weight(n, k, 128, seed=63)
+    qu, su = weight(n, k, 128, seed=64)
+    gate, up = (sbq.Int4Linear.from_quantized(q, s, None, group=128) for q, s in ((qg, sg), (qu, su)))
+    down = sbq.Int4Linear.from_quantized(*weight(16, n, 128, seed=65), None, group=128)
+    x = acts(m, k, x_dtype, seed=66)
+    wg, wu = dense(qg, sg, 128), dense(qu, su, 128)
+    g, u = x.double() @ wg.t(), x.double() @ wu.t()
+    ref = g * g.sigmoid() * u
+    tg, tu = tolerance(x, wg, F32, g), tolerance(x, wu, F32, u)
+    err = 1.1 * tg * u.abs() + (g * g.sigmoid()).abs() * tu + 1.1 * tg * tu + 8 * 2.0 ** -23 * ref.abs()  # as in test_gateup
+    for h_dtype in (F32, F16):
+        h = sbq.FusedGatedMLP(gate, up, down, h_dtype=h_dtype).gateup(x)
+        tol = err + ref.abs() * torch.finfo(h_dtype).eps / 2 + (2.0 ** -25 if h_dtype == F16 else 0.0)
+        bad = ((h.double() - ref).abs() - tol).max().item()
+        assert bad <= 0, bad
+
+
 @pytest.mark.parametrize("m", [3, 16, 24, 150])
 def test_strided_rows_and_untouched_surroundings(sbq, m):
     q, s = weight(40, 96, 32, seed=17)
