@@ -23,9 +23,9 @@
 // 6e-7 (fp32 x) at any k from 512 to 12288, with 64 steps 1.2e-6.  16-bit results,
 // whose own rounding (2^-12 and up) is far above it, are summed in one piece.
 //
-// Measured on B200, groups of 128: 4096 x 4096 x 12288 fp16 270 us (1.52 PFLOP/s, 0.92 of cuBLAS's measured bf16 rate),
-// 2048 x 4096 x 12288 fp16 143 us, with fp32 results 171 us (a segment ends in the wait for the accumulator to be read); gate/up 2048 x 4096 x 12288 295 us with bf16 x.  Long
-// products are bound by the tensor cores; one tile per pair (512 x 4096 x 4096, 24 us) by about 8 us of set-up, first
+// Measured on B200, groups of 128: 4096 x 4096 x 12288 fp16 267 us (1.54 PFLOP/s, 0.93 of cuBLAS's measured bf16 rate),
+// 2048 x 4096 x 12288 fp16 143 us, with fp32 results 167 us (a segment ends in the wait for the accumulator to be read);
+// gate/up 2048 x 4096 x 12288 291 us with bf16 x.  Long products are bound by the tensor cores; one tile per pair (512 x 4096 x 4096, 24 us) by about 8 us of set-up, first
 // loads and stores and 0.5 us per block of 128 k; 64 x 4096 x 12288 (20 us) by x, read again for every 128 channels.
 #include "tc.cuh"
 #include "w4_host.cuh"
