@@ -63,7 +63,7 @@ class FusedGatedMLP(nn.Module):
         gate = self.gate_proj
         k, n, dev = gate.in_features, gate.out_features, gate.packed.device
         if self.int4 and _in_place(x, k, dev):
-            h = x.new_empty((*x.shape[:-1], n), dtype=self.h_dtype)
+            h = torch.empty(*x.shape[:-1], n, dtype=self.h_dtype, device=dev)
             self._run_int4(x, x.numel() // k, k, k, h, n, dev)
             return h
         x2, on_host = self._rows(x, dev)

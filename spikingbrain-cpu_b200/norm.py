@@ -118,7 +118,7 @@ def residual_norm(branch: torch.Tensor | None, residual: torch.Tensor, pre_weigh
     x = None
     if pre_weight is not None:
         w = _weight(pre_weight, d, "pre_weight", dev)
-        x = residual.new_empty(shape, dtype=out_dtype)
+        x = torch.empty(*shape, dtype=out_dtype, device=dev)
         a.pre_weight, a.out, a.ld_out = w.data_ptr(), x.data_ptr(), d
     if residual_out is not None:
         if residual_out.shape != shape or residual_out.dtype != residual.dtype or residual_out.device != dev:
