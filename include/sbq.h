@@ -418,7 +418,7 @@ SBQ_API int sbq_mlp_gateup_w4(const void* x, int x_dtype, int64_t ldx, const voi
  * over rows of d elements (RMSNorm, model.py:30-39; the additions of Block.forward, model.py:388-392).
  * branch may be NULL (r' = residual_scale * residual), residual_out may be NULL; out and pre_weight are both
  * set or both NULL.  Each output may be one of residual, branch and a full gate (same address, element size and
- * row stride); other overlaps with these three, and of the outputs, are refused.  branch, residual (and residual_out, of its type), gate and out: SBQ_F32, SBQ_F16 or
+ * row stride); other overlaps with these three, with a weight or another gate, and of the outputs, are refused.  branch, residual (and residual_out, of its type), gate and out: SBQ_F32, SBQ_F16 or
  * SBQ_BF16, any row stride; weights fp32 [d].  gate: [d] (SBQ_GATE_PER_COLUMN), one per row at stride ld_gate
  * (SBQ_GATE_PER_ROW) or [m, d] (SBQ_GATE_FULL). */
 #define SBQ_GATE_NONE 0

@@ -648,7 +648,8 @@ static int check_operand(const void* p, int dtype, int64_t ld, int64_t width, in
 }
 
 // Each element of a row is read by the thread that writes it, before it does: an output may take the place of an
-// operand with the same rows, and share no byte with another.
+// operand with the same rows, and share no byte with another.  What every thread of a row reads (a gate per row) or every
+// row (weights, a gate per column) lies under no output at all: nothing orders those reads before another thread's stores.
 static bool norm_in_the_way(const W4Rows& out, const W4Rows& in, int64_t m) {
     if (!out.p || !in.p || !w4_overlap(out, in, m)) return false;
     return out.p != in.p || (m > 1 && out.ld != in.ld) || out.width != in.width;
@@ -693,11 +694,25 @@ extern "C" int sbq_residual_norm(const sbq_residual_norm_args* a, void* stream) 
     if (st) return st;
     const auto rows = [&](const void* q, int dtype, int64_t ld) { return W4Rows{q, ld * w4_elem(dtype), d * w4_elem(dtype)}; };
     const W4Rows r = rows(a->residual, a->residual_dtype, a->ld_residual), y = rows(a->branch, a->branch_dtype, a->ld_branch),
-                 g = rows(a->gate_mode == SBQ_GATE_FULL ? a->gate : nullptr, a->gate_dtype, a->ld_gate),
+                 // one row: a gate per column is a full one
+                 g = rows(a->gate_mode == SBQ_GATE_FULL || (a->gate_mode == SBQ_GATE_PER_COLUMN && m == 1) ? a->gate : nullptr,
+                          a->gate_dtype, a->ld_gate),
                  ro = rows(a->residual_out, a->residual_dtype, a->ld_residual_out), x = rows(a->out, a->out_dtype, a->ld_out);
     for (const W4Rows* in : {&r, &y, &g})
         if (norm_in_the_way(ro, *in, m) || norm_in_the_way(x, *in, m))
             return set_error(SBQ_ERR_INVALID_ARGUMENT, "an output overlaps an operand with other rows");
+    // a gate per row as rows of one element, from the lowest address on; neighbours in memory as one range
+    const int64_t gs = w4_elem(a->gate_dtype), gld = m > 1 ? a->ld_gate * gs : gs;
+    const W4Rows gate{static_cast<const char*>(a->gate) + (gld < 0 ? (m - 1) * gld : 0), gld < 0 ? -gld : gld, gs};
+    for (const W4Rows* out : {&ro, &x}) {
+        if (!out->p) continue;
+        bool meet = (a->pre_weight && w4_overlap(*out, a->pre_weight, 4 * d, m)) ||
+                    (a->post_weight && w4_overlap(*out, a->post_weight, 4 * d, m));
+        if (a->gate && a->gate_mode == SBQ_GATE_PER_ROW)
+            meet = meet || (gate.ld > gs ? w4_overlap(*out, gate, m) : w4_overlap(*out, gate.p, gate.ld == gs ? m * gs : gs, m));
+        if (a->gate && a->gate_mode == SBQ_GATE_PER_COLUMN && m > 1) meet = meet || w4_overlap(*out, a->gate, d * gs, m);
+        if (meet) return set_error(SBQ_ERR_INVALID_ARGUMENT, "an output overlaps a weight or a gate");
+    }
     if (a->residual_out && a->out && w4_overlap(ro, x, m))
         return set_error(SBQ_ERR_INVALID_ARGUMENT, "the outputs overlap");
     const int mode = l.aligned ? kAligned : l.shifted ? kShifted : kStrided;

@@ -53,6 +53,15 @@ inline bool w4_overlap(const W4Rows& a, const W4Rows& b, int64_t m) {
     return off < a.width || off + b.width > a.ld;
 }
 
+// Whether one of m rows shares a byte with the `bytes` bytes at q.
+inline bool w4_overlap(const W4Rows& a, const void* q, int64_t bytes, int64_t m) {
+    const int64_t off = reinterpret_cast<intptr_t>(q) - reinterpret_cast<intptr_t>(a.p);
+    if (off + bytes <= 0 || off >= (m - 1) * a.ld + a.width) return false;
+    if (off < 0 || m == 1 || a.ld <= 0) return true;
+    const int64_t at = off % a.ld;  // behind the start of the row before it, and then before the start of the next one
+    return at < a.width || at + bytes > a.ld;
+}
+
 // Lets a kernel use `bytes` of dynamic shared memory on the current device: once per kernel and device (`done`, the
 // kernel's own), since the call costs as much host time as a tenth of a launch.
 template <class K>

@@ -58,7 +58,7 @@ def residual_norm(branch: torch.Tensor | None, residual: torch.Tensor, pre_weigh
     rounded.  ``gate``: [d], [..., 1] or [..., d]; ``gate_act``: none, sigmoid, silu or tanh.  Statistics are
     fp32.  Without ``pre_weight`` there is no x (None is returned for it).  ``residual_out`` receives r' ([..., d] in
     the residual's type; it may be the residual itself, other overlaps with it, the branch or a full gate are
-    refused unless they are the same elements); with no branch, a residual_scale of 1 and no
+    refused unless they are the same elements, and so is every overlap with a weight or another gate); with no branch, a residual_scale of 1 and no
     ``residual_out`` the residual is returned as it is.
     """
     dev, shape = residual.device, residual.shape

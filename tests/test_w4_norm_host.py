@@ -1,0 +1,89 @@
+"""Argument checks of the 4-bit entry points and of sbq_residual_norm, before any launch (no GPU needed).
+
+The calls below carry made-up addresses: each of them has to be refused on the host.  Where a call next to a
+refused one is to be let through, the host's answer is looked at only for the refusal's words.
+"""
+
+import ctypes
+
+import pytest
+import torch
+
+BASE = 1 << 20  # an address no test reads
+
+
+def norm_status(sbq, m, d, **fields):
+    """(status, message) of sbq_residual_norm on fp32 rows: a branch, a residual and both outputs in buffers of
+    their own, 16 MiB apart, with `fields` on top."""
+    L = sbq._lib
+    a = L.ResidualNormArgs()
+    step = 1 << 24
+    a.branch, a.residual, a.residual_out, a.out = (BASE + i * step for i in range(4))
+    a.pre_weight = BASE + 4 * step
+    a.ld_branch = a.ld_residual = a.ld_residual_out = a.ld_out = d
+    a.m, a.d = m, d
+    a.residual_scale = a.branch_scale = 1.0
+    a.eps = 1e-6
+    for name, value in fields.items():
+        setattr(a, name, value)
+    status = L.load().sbq_residual_norm(ctypes.byref(a), None)
+    return status, L.load().sbq_last_error().decode()
+
+
+def refused(sbq, m, d, **fields):
+    status, message = norm_status(sbq, m, d, **fields)
+    return status == sbq._lib.ERR_INVALID_ARGUMENT and "overlaps" in message
+
+
+RES, FREE = BASE + (1 << 24), BASE + 6 * (1 << 24)
+OUTPUTS = {"residual_out": BASE + 2 * (1 << 24), "out": BASE + 3 * (1 << 24)}
+
+
+@pytest.fixture
+def no_device():
+    if torch.cuda.is_available():
+        pytest.skip("made-up addresses, some of which pass the checks: only where nothing can be launched")
+
+
+@pytest.mark.parametrize("m,d", [(1, 8), (5, 96), (300, 333)])
+def test_norm_outputs_over_a_vector(sbq, no_device, m, d):
+    """No output may lie on a weight or a gate per column: every row reads them, whenever another row is stored."""
+    L = sbq._lib
+    last = (m - 1) * d * 4
+    for name in ("pre_weight", "post_weight", "gate"):
+        mode = {"gate_mode": L.GATE_PER_COLUMN} if name == "gate" else {}
+        for out, at in OUTPUTS.items():
+            for off in (0, last, last + 4 * (d - 1), -4 * (d - 1)):
+                if name == "gate" and m == 1 and off == 0:
+                    continue  # one row: the gate's elements are those of a full gate
+                assert refused(sbq, m, d, **{name: at + off}, **mode), (name, out, off)
+            for off in (last + 4 * d, -4 * d):
+                assert not refused(sbq, m, d, **{name: at + off}, **mode), (name, out, off)
+
+
+def test_norm_outputs_around_a_vector(sbq, no_device):
+    """A vector that lies between the rows of an output shares nothing with it; one that reaches a row does."""
+    L = sbq._lib
+    m, d, ld = 7, 40, 128
+    for name, mode in (("pre_weight", {}), ("post_weight", {}), ("gate", {"gate_mode": L.GATE_PER_COLUMN})):
+        for out, at in OUTPUTS.items():
+            wide = {"ld_" + out: ld}
+            for col, bad in ((40, False), (88, False), (39, True), (89, True), (0, True)):
+                assert refused(sbq, m, d, **{name: at + 4 * (3 * ld + col)}, **mode, **wide) == bad, (name, out, col)
+
+
+@pytest.mark.parametrize("m,d", [(1, 300), (4, 96), (4, 600)])
+def test_norm_outputs_over_a_gate_per_row(sbq, no_device, m, d):
+    """A gate per row that is a column of an output is refused, in place or not; a column beside it is not."""
+    L = sbq._lib
+    ld = d + 16
+    for out, at in OUTPUTS.items():
+        wide = {"ld_" + out: ld, "gate_mode": L.GATE_PER_ROW, "ld_gate": ld}
+        for col, bad in ((0, True), (d - 1, True), (d, False), (d + 15, False)):
+            assert refused(sbq, m, d, gate=at + 4 * col, **wide) == bad, (out, col)
+        # gates next to each other, inside a row of the output and outside of all of them
+        wide["ld_gate"] = 1
+        assert refused(sbq, m, d, gate=at, **wide)
+        assert not refused(sbq, m, d, gate=FREE, **wide)
+    assert refused(sbq, m, d, gate=RES, gate_mode=L.GATE_PER_ROW, ld_gate=d, residual_out=RES)
+    assert not refused(sbq, m, d, gate=RES, gate_mode=L.GATE_PER_ROW, ld_gate=d)
