@@ -368,12 +368,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     const bool fresh = left == 0;
                     if (fresh) {
                         left = p.seg_blocks < w.kb1 - kb ? p.seg_blocks : w.kb1 - kb;
-                        if (seg > 0 && !tc::mbar_wait(taken, (seg - 1) & 1)) {
+                        if (seg > 0 && !tc::mbar_wait_cluster(taken, (seg - 1) & 1)) {
                             ok = false;
                             break;
                         }
                     }
-                    if (!tc::mbar_wait(&ready[s], ph)) {
+                    if (!tc::mbar_wait_cluster(&ready[s], ph)) {
                         ok = false;
                         break;
                     }
