@@ -116,4 +116,10 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 int set_error(int status, const char* fmt, ...);
 int check_launch(const char* what);
 
+// Ends an entry point that wrote a packed weight.  A product reads its weight before it waits for the kernel before it
+// (griddepcontrol.wait), as early as when that kernel's CTAs have ended, and by TMA: neither is ordered behind the stores of a
+// packing kernel.  So an empty kernel follows, launched in plain stream order: it begins when the packing kernel is complete
+// and its stores are visible to every reader, and a product can at most overtake the empty one.
+int packed_launch(const char* what, cudaStream_t s);
+
 }  // namespace sbq

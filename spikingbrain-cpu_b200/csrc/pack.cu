@@ -90,6 +90,16 @@ __global__ void __launch_bounds__(256) unpack_int8_kernel(const int8_t* __restri
     for (int64_t c = lane; c < k; c += 32) q[r * ldq + c] = packed[packed_offset(r, c, kt_total)];
 }
 
+// Does nothing: see packed_launch.
+__global__ void packed_kernel() {}
+
+int packed_launch(const char* what, cudaStream_t s) {
+    const int st = check_launch(what);
+    if (st) return st;
+    packed_kernel<<<1, 32, 0, s>>>();
+    return check_launch(what);
+}
+
 static int check_pack_args(const void* a, const void* packed, int64_t n, int64_t k, int64_t ld) {
     if (!a || !packed) return set_error(SBQ_ERR_INVALID_ARGUMENT, "null pointer");
     if (n <= 0 || k <= 0) return set_error(SBQ_ERR_INVALID_ARGUMENT, "n and k must be positive (n=%lld k=%lld)",

@@ -49,10 +49,6 @@ __device__ __forceinline__ void w4_store_rowmul(float smax, float* rowmul) {
     }
 }
 
-// Last statement of a packing kernel.  A product queued right after it reads the weight before it waits for its
-// predecessor and may start as soon as this grid's CTAs have ended: every store must be visible to the device by then.
-__device__ __forceinline__ void w4_settle() { __threadfence(); }
-
 // One CTA per packed row (rows past n are written as zeros), one thread per 8 columns; the threads of a
 // group are neighbouring lanes.
 template <typename T>
@@ -92,7 +88,6 @@ __global__ void __launch_bounds__(kPackThreads) w4_quantize_kernel(const T* __re
         }
     }
     w4_store_rowmul(smax, rowmul + r);
-    w4_settle();
 }
 
 // Given codes and scales (row strides ldq, lds) -> packed.  Codes outside [-8, 7] are clamped to it.
@@ -124,7 +119,6 @@ __global__ void __launch_bounds__(kPackThreads) w4_pack_kernel(const int8_t* __r
         }
     }
     w4_store_rowmul(smax, rowmul + r);
-    w4_settle();
 }
 
 // Packed -> codes [n, k] and scales [n, ceil(k / group)] (either may be null).
@@ -200,7 +194,7 @@ extern "C" int sbq_w4_quantize_pack(const void* w, int w_dtype, int64_t n, int64
         default:
             return set_error(SBQ_ERR_UNSUPPORTED, "weight dtype %d not supported (f32, f16, bf16)", w_dtype);
     }
-    return check_launch("w4_quantize_pack");
+    return packed_launch("w4_quantize_pack", s);
 }
 
 extern "C" int sbq_w4_pack(const int8_t* q, int64_t ldq, const void* scale, int64_t lds, int64_t n, int64_t k,
@@ -209,10 +203,11 @@ extern "C" int sbq_w4_pack(const int8_t* q, int64_t ldq, const void* scale, int6
     if (st) return st;
     if (!scale || !rowmul) return set_error(SBQ_ERR_INVALID_ARGUMENT, "null pointer");
     if (lds < ceil_div(k, group)) return set_error(SBQ_ERR_INVALID_ARGUMENT, "scale row stride smaller than the row");
-    w4_pack_kernel<<<(unsigned)(ceil_div(n, kTileRows) * kTileRows), kPackThreads, 0, static_cast<cudaStream_t>(stream)>>>(
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    w4_pack_kernel<<<(unsigned)(ceil_div(n, kTileRows) * kTileRows), kPackThreads, 0, s>>>(
         q, ldq, static_cast<const __nv_bfloat16*>(scale), lds, n, k, group, static_cast<uint8_t*>(packed),
         static_cast<__nv_bfloat16*>(scales), rowmul);
-    return check_launch("w4_pack");
+    return packed_launch("w4_pack", s);
 }
 
 extern "C" int sbq_w4_unpack(const void* packed, const void* scales, int64_t n, int64_t k, int group, int8_t* q,

@@ -36,3 +36,45 @@ def test_gates_and_weights_in_one_buffer(sbq, m, d):
     got = sbq.residual_norm(y, r, gate_act="tanh", residual_out=r, **own)
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
     assert torch.equal(buf[m:], kept[m:]) and torch.equal(buf[:, :4], kept[:, :4]) and torch.equal(buf[:, 4 + d:], kept[:, 4 + d:])
+
+
+@pytest.mark.parametrize("m,n,k", [(1, 512, 2048), (20, 512, 2048), (300, 4096, 4096)])
+@pytest.mark.parametrize("x_dtype", [F16, F32])
+def test_product_right_behind_the_packing(sbq, m, n, k, x_dtype):
+    """Products read their weight before they wait for the kernel before them: one that follows the packing of its
+    weight at once finds it complete, eager and in a graph, also where the buffers held another weight before."""
+    L = sbq._lib
+    ws = [rand(n, k, seed=10 + i, scale=0.02) for i in range(3)]
+    x = rand(m, k, seed=20, dtype=x_dtype)
+    lin = sbq.Int4Linear(ws[0], None, group=64)
+    quantised = [sbq.quantize_per_group(w, 64) for w in ws]
+    wants = []
+    for q, s in quantised:
+        other = sbq.Int4Linear.from_quantized(q, s, None, group=64)
+        torch.cuda.synchronize()
+        wants.append(other(x))
+
+    def pack(i, kind):
+        w, (q, s) = ws[i], quantised[i]
+        bufs = (lin.packed.data_ptr(), lin.scales.data_ptr(), lin.rowmul.data_ptr(), torch.cuda.current_stream().cuda_stream)
+        if kind:
+            L.call("sbq_w4_pack", q.data_ptr(), k, s.data_ptr(), s.shape[1], n, k, 64, *bufs)
+        else:
+            L.call("sbq_w4_quantize_pack", w.data_ptr(), L.F32, n, k, k, 64, *bufs)
+
+    torch.cuda.synchronize()
+    got = []
+    for i in range(60):
+        pack(i % 3, i & 1)
+        got.append((lin(x), wants[i % 3]))
+    assert all(torch.equal(a, b) for a, b in got)
+    graph, outs = torch.cuda.CUDAGraph(), []
+    with torch.cuda.graph(graph):
+        for i in range(6):
+            pack(i % 3, i & 1)
+            outs.append(lin(x))
+    for _ in range(3):
+        graph.replay()
+        assert all(torch.equal(o, wants[i % 3]) for i, o in enumerate(outs))
+    fresh = sbq.Int4Linear(ws[1], None, group=64)(x)  # as a user writes it
+    assert torch.equal(fresh, wants[1])
