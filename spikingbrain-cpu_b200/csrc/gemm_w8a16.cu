@@ -774,8 +774,9 @@ static int gemm_small(const CUtensorMap& mx, const CUtensorMap& mx2, const CUten
 // Both GEMMs launch as programmatic dependents of the previous kernel on the stream: they set up,
 // request their first weight tiles and convert them before griddepcontrol.wait, and touch
 // activations and outputs only after it.  Only kernels that call griddepcontrol.launch_dependents
-// let a dependent start early, and in this library those write activations only (never packed
-// weights, scales or biases); any other predecessor completes first, as in plain stream order.
+// let a dependent start before they end, and in this library those write activations only (never packed
+// weights, scales or biases); the packing entry points end with an empty kernel, which starts when the
+// packing is complete (packed_launch).
 template <bool OUT_F16, bool GATED, int AK, int TOK>
 static cudaError_t launch_pair(dim3 grid, cudaStream_t s, const CUtensorMap& mx, const CUtensorMap& mx2,
                                const CUtensorMap& mw, const GemmW16Params& p) {

@@ -144,7 +144,7 @@ extern "C" int sbq_quantize_pack(const void* w, int w_dtype, int64_t n, int64_t 
         default:
             return set_error(SBQ_ERR_UNSUPPORTED, "weight dtype %d not supported (f32, f16, bf16)", w_dtype);
     }
-    return check_launch("quantize_pack");
+    return packed_launch("quantize_pack", s);
 }
 
 extern "C" int sbq_pack_int8(const int8_t* q, int64_t n, int64_t k, int64_t ldq, void* packed, int32_t* rowsum,
@@ -154,7 +154,7 @@ extern "C" int sbq_pack_int8(const int8_t* q, int64_t n, int64_t k, int64_t ldq,
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (cudaMemsetAsync(packed, 0, sbq_packed_bytes(n, k), s) != cudaSuccess) return check_launch("memset packed");
     pack_int8_kernel<<<(unsigned)ceil_div(n, 8), 256, 0, s>>>(q, n, k, ldq, static_cast<int8_t*>(packed), rowsum);
-    return check_launch("pack_int8");
+    return packed_launch("pack_int8", s);
 }
 
 extern "C" int sbq_unpack_int8(const void* packed, int64_t n, int64_t k, int8_t* q, int64_t ldq, void* stream) {

@@ -78,3 +78,16 @@ def test_product_right_behind_the_packing(sbq, m, n, k, x_dtype):
         assert all(torch.equal(o, wants[i % 3]) for i, o in enumerate(outs))
     fresh = sbq.Int4Linear(ws[1], None, group=64)(x)  # as a user writes it
     assert torch.equal(fresh, wants[1])
+
+
+@pytest.mark.parametrize("m", [1, 40, 300])
+def test_int8_product_right_behind_the_packing(sbq, m):
+    """The same for the int8 formats, whose products read their weight as early."""
+    n, k = 1024, 2048
+    ws, x = [rand(n, k, seed=30 + i, scale=0.02) for i in range(2)], rand(m, k, seed=33, dtype=F16)
+    for kind in (sbq.Int8Linear, sbq.DynamicInt8Linear):
+        lins = [kind(w, None) for w in ws]
+        torch.cuda.synchronize()
+        wants = [lin(x) for lin in lins]
+        got = [(kind(ws[i & 1], None)(x), wants[i & 1]) for i in range(40)]
+        assert all(torch.equal(a, b) for a, b in got)
