@@ -393,6 +393,11 @@ SBQ_API int sbq_w4_unpack(const void* packed, const void* scales, int64_t n, int
  * sums of tiles that are cut along k.  Its contents need not be kept between calls. */
 SBQ_API size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k, int x_dtype, int matrices);
 
+/* Host only: how a call of these sizes runs on the current device (148 SMs are assumed where there is none).  plan[4]:
+ * kernel (0 decode product, 1 tensor-memory product of a CTA, 2 of CTA pairs), tokens per tile, parts along k (1: CTAs of
+ * a cluster; 2: parts of each tile of the last round), rounds of whole tiles (2). */
+SBQ_API int sbq_linear_w4_plan(int64_t m, int64_t n, int64_t k, int x_dtype, int matrices, int* plan);
+
 /* y[m, n] = sum_k x[m, k] * q[n, k] * s[n, k / group] (+ bias[n]); x and y SBQ_F32, SBQ_F16 or SBQ_BF16.
  * q * s enters the product exactly, 16-bit x too, fp32 x with 22 bits; sums are fp32.  Up to 16 rows: the
  * decode product; above: the tensor-memory product.  x rows 16-byte aligned when k is a multiple of 16 (any row stride

@@ -117,6 +117,7 @@ SIGNATURES = {
     "sbq_w4_pack": (_c_int, [_vp, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_int, _vp, _vp, _vp, _vp]),
     "sbq_w4_unpack": (_c_int, [_vp, _vp, _c_i64, _c_i64, _c_int, _vp, _c_i64, _vp, _c_i64, _vp]),
     "sbq_linear_w4_workspace_bytes": (_sz, [_c_i64, _c_i64, _c_i64, _c_int, _c_int]),
+    "sbq_linear_w4_plan": (_c_int, [_c_i64, _c_i64, _c_i64, _c_int, _c_int, ctypes.POINTER(_c_int)]),
     "sbq_linear_w4": (_c_int, [_vp, _c_int, _c_i64, _vp, _vp, _vp, _c_int, _vp, _c_i64, _c_i64, _c_i64, _vp, _c_int,
                                _c_i64, _vp, _sz, _vp]),
     "sbq_mlp_gateup_w4": (_c_int, [_vp, _c_int, _c_i64, _vp, _vp, _vp, _vp, _vp, _vp, _c_int, _c_i64, _c_i64, _c_i64, _vp,

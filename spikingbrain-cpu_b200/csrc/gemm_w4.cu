@@ -921,7 +921,8 @@ static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, bool split, int nmat) {
     if (m <= kSTok4) return best;  // a pair's tile would be no fuller
     const int64_t waves = ceil_div(small_tiles * parts, 2 * sms);
     const double small_block = parts > 1 ? (split ? 1.4 : 0.84) : waves > 1 ? (split ? 1.25 : 0.68) : (split ? 1.15 : 0.57);
-    double best_t = (split ? 7.5 : 6.5) + (double)(waves * ceil_div(kt, parts)) * small_block;
+    // its token tiles are the grid's y dimension: above 65535 of them the pair kernel takes the call
+    double best_t = ceil_div(m, kSTok4) > 65535 ? 1e30 : (split ? 7.5 : 6.5) + (double)(waves * ceil_div(kt, parts)) * small_block;
     // with two matrices a taker warpgroup finishes whole sets of 32 tokens
     const int set = 32 * nmat, widest = m < kTok ? (int)ceil_div(m, set) * set : kTok;
     for (int tok = widest; tok >= set; tok -= set) {
@@ -948,6 +949,14 @@ static W4Plan w4_plan(int64_t m, int64_t n, int64_t k, bool split, int nmat) {
 size_t gemm_w4_workspace(int64_t m, int64_t n, int64_t k, bool split, int nmat) {
     const W4Plan pl = w4_plan(m, n, k, split, nmat);
     return !pl.small_parts && pl.tail_parts > 1 ? (size_t)pl.tail_tiles * pl.tail_parts * kTok * 2 * kW4Rows * 4 : 0;
+}
+
+void gemm_w4_plan(int64_t m, int64_t n, int64_t k, bool split, int nmat, int* plan) {
+    const W4Plan pl = w4_plan(m, n, k, split, nmat);
+    plan[0] = pl.small_parts ? 1 : 2;
+    plan[1] = pl.small_parts ? kSTok4 : pl.tok;
+    plan[2] = pl.small_parts ? pl.small_parts : pl.tail_parts;
+    plan[3] = pl.small_parts ? 0 : pl.rounds;
 }
 
 int gemm_w4_run(const W4Call& c, const W4Acts& x) {

@@ -263,6 +263,18 @@ extern "C" size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k,
     return act_bytes(m, k, x_dtype) + (m > kW4GemvRows ? gemm_w4_workspace(m, n, round16(k), x_dtype == SBQ_F32, matrices == 2 ? 2 : 1) : 0);
 }
 
+extern "C" int sbq_linear_w4_plan(int64_t m, int64_t n, int64_t k, int x_dtype, int matrices, int* plan) {
+    if (!plan) return set_error(SBQ_ERR_INVALID_ARGUMENT, "null pointer");
+    if (m <= 0 || n <= 0 || k <= 0) return set_error(SBQ_ERR_INVALID_ARGUMENT, "m, n, k must be positive");
+    plan[0] = plan[2] = plan[3] = 0;
+    plan[1] = 8;
+    if (m > kW4GemvRows)
+        gemm_w4_plan(m, n, round16(k), x_dtype == SBQ_F32, matrices == 2 ? 2 : 1, plan);
+    else if (m > 8)
+        plan[1] = 16;
+    return SBQ_OK;
+}
+
 extern "C" int sbq_linear_w4(const void* x, int x_dtype, int64_t ldx, const void* packed, const void* scales,
                              const float* rowmul, int group, const float* bias, int64_t m, int64_t n, int64_t k, void* y,
                              int y_dtype, int64_t ldy, void* workspace, size_t workspace_bytes, void* stream) {

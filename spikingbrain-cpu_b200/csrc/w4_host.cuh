@@ -33,6 +33,7 @@ struct W4Acts {
 int gemv_w4_run(const W4Call& c, const W4Acts& x);  // up to 16 rows
 int gemm_w4_run(const W4Call& c, const W4Acts& x);  // fp16 parts only
 size_t gemm_w4_workspace(int64_t m, int64_t n, int64_t k, bool split, int nmat);
+void gemm_w4_plan(int64_t m, int64_t n, int64_t k, bool split, int nmat, int* plan);
 int w4_sm_count();
 
 inline int w4_elem(int dtype) { return dtype == SBQ_F32 ? 4 : 2; }

@@ -91,3 +91,23 @@ def test_int8_product_right_behind_the_packing(sbq, m):
         wants = [lin(x) for lin in lins]
         got = [(kind(ws[i & 1], None)(x), wants[i & 1]) for i in range(40)]
         assert all(torch.equal(a, b) for a, b in got)
+
+
+@pytest.mark.parametrize("m", [65535 * 64, 65535 * 64 + 1])
+def test_more_rows_than_a_grid_dimension(sbq, m):
+    """64-row tiles beyond 65535, which is what a grid has in y: the linear and the gate/up form."""
+    n, k = 16, 32
+    q, s = torch.randint(-8, 8, (n, k), device="cuda", dtype=torch.int8), rand(n, 1, seed=40).abs().add(0.5).to(BF16)
+    lin = sbq.Int4Linear.from_quantized(q, s, None, group=32)
+    x = rand(m, k, seed=41)
+    w = q.double() * s.double()
+    ref, mags = x.double() @ w.t(), x.double().abs() @ w.abs().t()
+    # fp32 x has 22 bits (2^-23 of each element); 4 tensor-core steps, the factor and the rounding of the result
+    tol = mags * (2.0 ** -23 + 8 * 2.0 ** -22)
+    assert ((lin(x).double() - ref).abs() <= tol).all()
+    del mags
+    down = sbq.Int4Linear.from_quantized(q.t().contiguous(), torch.ones(k, 1, dtype=BF16, device="cuda"), None, group=32)
+    mlp = sbq.FusedGatedMLP(lin, lin, down, h_dtype=F32)
+    h = ref * ref.sigmoid() * ref
+    # d (silu(g) u) with g = u: at most 2.1 |g| of the product's error, and a few roundings
+    assert ((mlp.gateup(x).double() - h).abs() <= 2.2 * tol * (ref.abs() + tol) + 8 * 2.0 ** -23 * h.abs()).all()

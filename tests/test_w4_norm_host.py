@@ -87,3 +87,32 @@ def test_norm_outputs_over_a_gate_per_row(sbq, no_device, m, d):
         assert not refused(sbq, m, d, gate=FREE, **wide)
     assert refused(sbq, m, d, gate=RES, gate_mode=L.GATE_PER_ROW, ld_gate=d, residual_out=RES)
     assert not refused(sbq, m, d, gate=RES, gate_mode=L.GATE_PER_ROW, ld_gate=d)
+
+
+def plan(sbq, m, n, k, x_dtype="F32", matrices=1):
+    L = sbq._lib
+    out = (ctypes.c_int * 4)()
+    L.call("sbq_linear_w4_plan", m, n, k, getattr(L, x_dtype), matrices, out)
+    return list(out)
+
+
+def test_plan_of_a_call(sbq):
+    L = sbq._lib
+    assert plan(sbq, 1, 4096, 4096) == [0, 8, 0, 0] and plan(sbq, 16, 4096, 4096)[:2] == [0, 16]
+    assert plan(sbq, 17, 4096, 4096, "F16")[:2] == [1, 64]
+    assert plan(sbq, 4096, 12288, 4096, "F16")[:2] == [2, 256]
+    for m, n, k in ((0, 16, 16), (16, -1, 16), (16, 16, 0)):
+        assert L.load().sbq_linear_w4_plan(m, n, k, L.F16, 1, (ctypes.c_int * 4)()) == L.ERR_INVALID_ARGUMENT
+    assert L.load().sbq_linear_w4_plan(16, 16, 16, L.F16, 1, None) == L.ERR_INVALID_ARGUMENT
+
+
+@pytest.mark.parametrize("matrices", [1, 2])
+@pytest.mark.parametrize("x_dtype", ["F16", "BF16", "F32"])
+def test_every_row_count_fits_its_launch(sbq, x_dtype, matrices):
+    """The CTA kernel's 64-row tiles are the y dimension of its grid, which ends at 65535."""
+    for m in (65535 * 64, 65535 * 64 + 1, 1 << 23, 1 << 27, (1 << 31) - 257):
+        for n in (1, 16, 64, 128, 129, 1024):
+            for k in (16, 100, 512, 2560):
+                kernel, tokens, parts, _ = plan(sbq, m, n, k, x_dtype, matrices)
+                assert kernel == 2 or -(-m // tokens) <= 65535, (m, n, k)
+                assert kernel == 1 or tokens == 256 and parts >= 1
