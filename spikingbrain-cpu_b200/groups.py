@@ -9,7 +9,8 @@ streams them all with a single read of x and one launch.  ``fuse_shared_inputs``
 ``GroupMember`` modules in the members' places: the first member called with a given x runs the
 whole group, the others return their slice of that result, so the reference's model code runs
 unchanged.  A result is handed out once per computation; a member called again (or with another
-x) recomputes.  Members' outputs are column views of the group's [m, padded N] result.
+x) recomputes.  The result and x are held until every member has been called.  Members' outputs are
+column views of the group's [m, padded N] result.
 
 The int8 formats and the int4 ones are supported (all members of one group share the format, and the
 group size of an int4 one).  int8-dyn members
@@ -51,8 +52,7 @@ class SharedInputGroup(nn.Module):
         self.n_pad = off
         self.mode = getattr(members[0], "mode", None)
         self.out_dtype = torch.float32
-        self._result = None
-        self._key = None
+        self._result = self._key = None
         self._handed = set()
         if kind is Int4Linear:
             self._join_int4(members)
@@ -118,13 +118,17 @@ class SharedInputGroup(nn.Module):
         return [out[..., o:o + n] for o, n in zip(self.offsets, self.sizes)]
 
     def member_output(self, index: int, x: torch.Tensor) -> torch.Tensor:
-        key = (id(x), x.data_ptr(), x._version, tuple(x.shape), x.dtype, x.device)
-        if self._result is None or self._key != key or index in self._handed:
+        # x itself is kept while its result is: a tensor that has been freed may come back with the same id, address and
+        # version as another input
+        key = (x.data_ptr(), x._version, tuple(x.shape), x.dtype, x.device)
+        if self._result is None or self._key[0] is not x or self._key[1:] != key or index in self._handed:
             self._result = self.forward_all(x)
-            self._key = key
-            self._handed = set()
+            self._key, self._handed = (x, *key), set()
+        out = self._result[index]
         self._handed.add(index)
-        return self._result[index]
+        if len(self._handed) == len(self.sizes):
+            self._result = self._key = None
+        return out
 
 
 class GroupMember(nn.Module):

@@ -111,3 +111,20 @@ def test_more_rows_than_a_grid_dimension(sbq, m):
     h = ref * ref.sigmoid() * ref
     # d (silu(g) u) with g = u: at most 2.1 |g| of the product's error, and a few roundings
     assert ((mlp.gateup(x).double() - h).abs() <= 2.2 * tol * (ref.abs() + tol) + 8 * 2.0 ** -23 * h.abs()).all()
+
+
+@pytest.mark.parametrize("fmt", ["int4-g64", "int8"])
+def test_group_members_called_with_different_inputs(sbq, fmt):
+    """A step that calls some members of a group only, and the next one that begins with another member."""
+    parent = torch.nn.Module()
+    names = ["q_proj", "k_proj"]
+    lins = [sbq.make_linear(fmt, rand(48, 128, seed=50 + i)) for i in range(2)]
+    for name, lin in zip(names, lins):
+        setattr(parent, name, lin)
+    sbq.groups.fuse_shared_inputs(parent, names)
+    for i in range(10):
+        for name, lin in (("q_proj", lins[0]), ("k_proj", lins[1])):
+            x = rand(3, 128, seed=60 + 2 * i + (name == "k_proj"), dtype=F16)
+            got, want = parent.get_submodule(name)(x), lin(x)
+            assert (got - want).norm() <= 2.0 ** -18 * want.norm()
+            del x
