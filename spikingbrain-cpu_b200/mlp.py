@@ -14,7 +14,7 @@ import torch.nn as nn
 
 from . import _lib as L
 from .quant import (_DTYPE_CODE, Int4Linear, Int8Linear, _in_place, _int4_rows, _int4_workspace, _prepare_x, _ptr, _raw_stream, _stream,
-                    _workspace)
+                    _workspace, _written)
 
 
 class FusedGatedMLP(nn.Module):
@@ -96,8 +96,7 @@ class FusedGatedMLP(nn.Module):
                    _ptr(self.gate_proj.packed), _ptr(self.gate_proj.scale), _ptr(self.up_proj.packed),
                    _ptr(self.up_proj.scale), m, n, x2.shape[1], _ptr(h), L.F16 if h.dtype == torch.float16 else L.F32,
                    h.stride(0), _ptr(ws), ws_bytes, _stream(h.device))
-        return h
-
+        return _written(h)
 
     def _gateup_int4(self, x2: torch.Tensor, h: torch.Tensor) -> torch.Tensor:
         m, n, k = x2.shape[0], self.gate_proj.out_features, self.gate_proj.in_features
@@ -107,7 +106,7 @@ class FusedGatedMLP(nn.Module):
         if x2.shape[1] != k or (x2.stride(1) != 1 and k > 1) or x2.dtype not in _DTYPE_CODE or x2.device != dev:
             raise ValueError("input must be an fp32/fp16/bf16 [m, %d] view with unit column stride" % k)
         self._run_int4(x2, m, k, x2.stride(0) if m > 1 else k, h, h.stride(0) if m > 1 else n, dev)
-        return h
+        return _written(h)
 
     def _run_int4(self, x: torch.Tensor, m: int, k: int, ldx: int, h: torch.Tensor, ldh: int, dev: torch.device) -> None:
         if m == 0:

@@ -16,7 +16,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .quant import _DTYPE_CODE, _raw_stream
+from .quant import _DTYPE_CODE, _raw_stream, _written
 
 
 def _rows(t: torch.Tensor, d: int, what: str, dev: torch.device) -> tuple[torch.Tensor, int]:
@@ -138,6 +138,8 @@ def residual_norm(branch: torch.Tensor | None, residual: torch.Tensor, pre_weigh
         status = L.load().sbq_residual_norm(ctypes.byref(a), _raw_stream(dev))
         if status:
             L.check(status, "sbq_residual_norm")
+        if residual_out is not None:
+            _written(residual_out)
     return new, x
 
 

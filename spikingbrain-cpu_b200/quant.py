@@ -47,6 +47,13 @@ def _stream(device: torch.device) -> ctypes.c_void_p:
     return ctypes.c_void_p(torch.cuda.current_stream(device).cuda_stream)
 
 
+def _written(t: torch.Tensor) -> torch.Tensor:
+    """t, after a kernel wrote to its address: counted as a change in place, as torch's own operations count theirs (a kept
+    SharedInputGroup result, or a tensor saved for a gradient, goes by that count)."""
+    torch._C._increment_version((t,))
+    return t
+
+
 def _ptr(t: torch.Tensor | None):
     return None if t is None else ctypes.c_void_p(t.data_ptr())
 
@@ -224,7 +231,7 @@ class Int8Linear(_PackedLinear):
                    _ptr(self.scale), _ptr(self.bias), m, n, x2.shape[1], _ptr(out),
                    L.F32 if out.dtype == torch.float32 else L.F16, out.stride(0), _ptr(ws), ws_bytes,
                    _stream(out.device))
-        return out
+        return _written(out)
 
     def gemv_job(self, x2: torch.Tensor, out: torch.Tensor) -> L.GemvJob:
         """This projection as one job of a grouped decode launch (see ``gemv_group``)."""
@@ -518,7 +525,7 @@ class Int4Linear(nn.Module):
         if x2.device != dev or out.device != dev:
             raise ValueError("input and output must be on the weight's device %s" % dev)
         self._run(x2, m, k, x2.stride(0) if m > 1 else k, out, out.stride(0) if m > 1 else n, dev)
-        return out
+        return _written(out)
 
     def _run(self, x: torch.Tensor, m: int, k: int, ldx: int, out: torch.Tensor, ldy: int, dev: torch.device) -> None:
         if m == 0:

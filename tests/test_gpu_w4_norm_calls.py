@@ -128,3 +128,28 @@ def test_group_members_called_with_different_inputs(sbq, fmt):
             got, want = parent.get_submodule(name)(x), lin(x)
             assert (got - want).norm() <= 2.0 ** -18 * want.norm()
             del x
+
+
+@pytest.mark.parametrize("writer", ["int4", "int8", "gateup int4", "gateup int8", "residual_norm"])
+def test_calls_that_write_into_a_tensor_count_as_changes_of_it(sbq, writer):
+    """The kernels write through addresses; the tensor's version moves all the same, and a group whose x was refilled
+    this way computes anew."""
+    parent = torch.nn.Module()
+    parent.q_proj, parent.k_proj = lins = [sbq.make_linear("int4-g64", rand(48, 128, seed=70 + i)) for i in range(2)]
+    sbq.groups.fuse_shared_inputs(parent, ["q_proj", "k_proj"])
+    fmt = "int8" if writer.endswith("int8") else "int4-g64"
+    step = sbq.make_linear(fmt, rand(128, 128, seed=72))
+    mlp = sbq.FusedGatedMLP(*(sbq.make_linear(fmt, rand(128, 128, seed=73 + i)) for i in range(3)))
+    src, x = rand(3, 128, seed=76, dtype=F16), rand(3, 128, seed=77, dtype=F16)
+    write = {"int4": lambda: step.forward_into(src, x), "int8": lambda: step.forward_into(src, x),
+             "gateup int4": lambda: mlp.gateup_into(src, x), "gateup int8": lambda: mlp.gateup_into(src, x),
+             "residual_norm": lambda: sbq.residual_norm(src, x, residual_out=x)}[writer]
+    parent.q_proj(x)
+    version, before = x._version, x.clone()
+    write()
+    assert x._version > version and not torch.equal(x, before)
+    got, want = parent.k_proj(x), lins[1](x)
+    assert (got - want).norm() <= 2.0 ** -18 * want.norm()
+    with torch.inference_mode():  # tensors without a version
+        x = x.clone()
+        write()
