@@ -32,6 +32,7 @@ class FusedGatedMLP(nn.Module):
             raise ValueError("the fused gate/up epilogue has no bias term")
         if gate.out_features != up.out_features or gate.in_features != up.in_features:
             raise ValueError("gate and up projections must have the same shape")
+        self._check_devices(gate, up)
         if down.in_features != gate.out_features * shards:
             raise ValueError("down projection input must match the gate/up output")
         self.shards = shards
@@ -50,6 +51,11 @@ class FusedGatedMLP(nn.Module):
         h = self.gateup_into(x2, torch.empty(m, n, dtype=self.h_dtype, device=dev))
         y = self.down_proj(h).reshape(*shape[:-1], self.down_proj.out_features)
         return y.to("cpu") if on_host else y
+
+    @staticmethod
+    def _check_devices(gate: nn.Module, up: nn.Module) -> None:
+        if gate._buffers["packed"].device != up._buffers["packed"].device:
+            raise ValueError("gate and up projections must be on the same device: one launch reads both")
 
     def _rows(self, x: torch.Tensor, dev: torch.device):
         """(rows of x as the kernels take them, whether x came from the host)."""
@@ -75,6 +81,7 @@ class FusedGatedMLP(nn.Module):
         if self.int4:
             raise ValueError("grouped decode launches take int8 weights")
         g, u = self.gate_proj, self.up_proj
+        self._check_devices(g, u)
         return L.GemvJob(x2.data_ptr(), x2.stride(0), g.packed.data_ptr(), g.scale.data_ptr(), u.packed.data_ptr(),
                          u.scale.data_ptr(), None, g.out_features, x2.shape[1], h.data_ptr(),
                          L.F32 if h.dtype == torch.float32 else L.F16, h.stride(0))
@@ -90,6 +97,7 @@ class FusedGatedMLP(nn.Module):
         m, n = x2.shape[0], self.gate_proj.out_features
         if self.int4:
             return self._gateup_int4(x2, h)
+        self._check_devices(self.gate_proj, self.up_proj)
         if m > 0:
             ws, ws_bytes = _workspace(m, x2.shape[1], x2.dtype, h.device)
             L.call("sbq_mlp_gateup_w8_ws", _ptr(x2), _DTYPE_CODE[x2.dtype], x2.stride(0),
@@ -109,6 +117,7 @@ class FusedGatedMLP(nn.Module):
         return _written(h)
 
     def _run_int4(self, x: torch.Tensor, m: int, k: int, ldx: int, h: torch.Tensor, ldh: int, dev: torch.device) -> None:
+        self._check_devices(self.gate_proj, self.up_proj)
         if m == 0:
             return
         if dev.index != torch._C._cuda_getDevice():  # the library launches on the current device

@@ -116,3 +116,33 @@ def test_every_row_count_fits_its_launch(sbq, x_dtype, matrices):
                 kernel, tokens, parts, _ = plan(sbq, m, n, k, x_dtype, matrices)
                 assert kernel == 2 or -(-m // tokens) <= 65535, (m, n, k)
                 assert kernel == 1 or tokens == 256 and parts >= 1
+
+
+def int4(sbq, n, k, device, group=64):
+    """An Int4Linear around buffers of the right sizes on any device, which cannot be run."""
+    lib = sbq._lib.load()
+    mod = sbq.Int4Linear.__new__(sbq.Int4Linear)
+    torch.nn.Module.__init__(mod)
+    mod._adopt((torch.zeros(lib.sbq_w4_packed_bytes(n, k), dtype=torch.uint8, device=device),
+                torch.zeros(lib.sbq_w4_scale_bytes(n, k, group), dtype=torch.uint8, device=device),
+                torch.zeros((n + 15) // 16 * 16, dtype=torch.int32, device=device)), (n, k), None, group)
+    return mod
+
+
+def int8(sbq, n, k, device):
+    return sbq.Int8Linear.from_packed(torch.zeros(sbq._lib.packed_bytes(n, k), dtype=torch.int8, device=device),
+                                      torch.zeros(n, device=device), None, n, k)
+
+
+@pytest.mark.parametrize("make", [int4, int8])
+def test_gate_and_up_on_different_devices(sbq, make):
+    """One launch reads both weights: both have to be on its device, also when a module was moved later."""
+    down = make(sbq, 64, 128, "cpu")
+    with pytest.raises(ValueError, match="same device"):
+        sbq.FusedGatedMLP(make(sbq, 128, 64, "cpu"), make(sbq, 128, 64, "meta"), down)
+    mlp = sbq.FusedGatedMLP(make(sbq, 128, 64, "cpu"), make(sbq, 128, 64, "cpu"), down)
+    mlp.up_proj.to("meta")
+    x = torch.zeros(2, 64)
+    for call in (mlp, mlp.gateup, lambda t: mlp.gateup_into(t, torch.zeros(2, 128))):
+        with pytest.raises(ValueError, match="same device"):
+            call(x)
