@@ -344,6 +344,20 @@ def _int4_buffers(n: int, k: int, group: int, dev: torch.device):
             torch.empty((n + 15) // 16 * 16, dtype=torch.int32, device=dev))
 
 
+def _check_int4_buffers(n: int, k: int, group: int, packed: torch.Tensor, scales: torch.Tensor,
+                        rowmul: torch.Tensor | None = None) -> int:
+    """The group size, if the buffers are those of an [n, k] weight on one CUDA device: the kernels read by n, k and group."""
+    lib, group = L.load(), _check_group(group)
+    bufs = [(packed, int(lib.sbq_w4_packed_bytes(n, k)), torch.uint8), (scales, int(lib.sbq_w4_scale_bytes(n, k, group)), torch.uint8)]
+    if rowmul is not None:
+        bufs.append((rowmul, (n + 15) // 16 * 16, torch.int32))
+    if any(size == 0 or t.numel() != size or t.dtype != dtype or not t.is_contiguous() for t, size, dtype in bufs):
+        raise ValueError("packed buffers do not match a [%d, %d] weight in groups of %d" % (n, k, group))
+    if any(not t.is_cuda or t.device != packed.device for t, _, _ in bufs):
+        raise ValueError("packed buffers must be on one CUDA device")
+    return group
+
+
 def pack_weight_int4(weight: torch.Tensor, group: int = 128, device=None):
     """Quantise an [n, k] float weight per output channel and group of ``group`` inputs on the device, packed.
 
@@ -394,6 +408,7 @@ def pack_int4(q: torch.Tensor, scale: torch.Tensor, group: int = 128, device=Non
 
 def unpack_int4(packed: torch.Tensor, scales: torch.Tensor, n: int, k: int, group: int):
     """Packed buffers -> ``(q int8 [n, k], scale bf16 [n, ceil(k / group)])`` on the same device."""
+    group = _check_int4_buffers(n, k, group, packed, scales)
     dev = packed.device
     q = torch.empty(n, k, dtype=torch.int8, device=dev)
     scale = torch.empty(n, -(-k // group), dtype=torch.bfloat16, device=dev)
@@ -449,14 +464,7 @@ class Int4Linear(nn.Module):
     def from_packed(cls, packed: torch.Tensor, scales: torch.Tensor, rowmul: torch.Tensor, out_features: int,
                     in_features: int, bias: torch.Tensor | None = None, group: int = 128):
         """A module around buffers of ``pack_weight_int4`` / ``pack_int4``; they are adopted, not copied."""
-        lib = L.load()
-        group = _check_group(group)
-        sizes = (int(lib.sbq_w4_packed_bytes(out_features, in_features)),
-                 int(lib.sbq_w4_scale_bytes(out_features, in_features, group)), (out_features + 15) // 16 * 16)
-        for t, size, dtype in zip((packed, scales, rowmul), sizes, (torch.uint8, torch.uint8, torch.int32)):
-            if t.numel() == size and t.dtype == dtype and t.is_contiguous() and t.is_cuda and t.device == packed.device:
-                continue
-            raise ValueError("packed buffers do not match a [%d, %d] weight in groups of %d" % (out_features, in_features, group))
+        group = _check_int4_buffers(out_features, in_features, group, packed, scales, rowmul)
         mod = cls.__new__(cls)
         nn.Module.__init__(mod)
         mod._adopt((packed, scales, rowmul), (out_features, in_features), bias, group)

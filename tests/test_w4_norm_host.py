@@ -146,3 +146,29 @@ def test_gate_and_up_on_different_devices(sbq, make):
     for call in (mlp, mlp.gateup, lambda t: mlp.gateup_into(t, torch.zeros(2, 128))):
         with pytest.raises(ValueError, match="same device"):
             call(x)
+
+
+def test_buffers_of_another_size_are_not_unpacked(sbq):
+    """unpack_int4 reads what n, k and group say: the buffers have to be those of such a weight, on one CUDA device."""
+    n, k, group = 40, 200, 64
+    lin = int4(sbq, n, k, "cpu", group)
+    bad = [(lin.packed, lin.scales, 56, k, group), (lin.packed, lin.scales, n, 300, group), (lin.packed, lin.scales, n, k, 32),
+           (lin.packed[:-1024], lin.scales, n, k, group), (lin.packed, lin.scales[1:], n, k, group),
+           (lin.packed.view(torch.int8), lin.scales, n, k, group), (lin.packed, lin.scales.view(torch.bfloat16), n, k, group),
+           (torch.zeros(2 * lin.packed.numel(), dtype=torch.uint8)[::2], lin.scales, n, k, group),
+           (lin.packed[:0], lin.scales[:0], 0, k, group), (lin.packed[:0], lin.scales[:0], n, 0, group)]
+    for args in bad:
+        with pytest.raises(ValueError, match="do not match"):
+            sbq.unpack_int4(*args)
+    with pytest.raises(ValueError, match="group size"):
+        sbq.unpack_int4(lin.packed, lin.scales, n, k, 48)
+    with pytest.raises(ValueError, match="one CUDA device"):
+        sbq.unpack_int4(lin.packed, lin.scales, n, k, group)
+    for args in bad:
+        args = (*args[:2], lin.rowmul, *args[2:4], None, args[4])
+        with pytest.raises(ValueError, match="do not match"):
+            sbq.Int4Linear.from_packed(*args)
+    with pytest.raises(ValueError, match="do not match"):
+        sbq.Int4Linear.from_packed(lin.packed, lin.scales, lin.rowmul[:-1], n, k, None, group)
+    with pytest.raises(ValueError, match="one CUDA device"):
+        sbq.Int4Linear.from_packed(lin.packed, lin.scales, lin.rowmul, n, k, None, group)
