@@ -144,6 +144,8 @@ __global__ void __launch_bounds__(kPackThreads) w4_unpack_kernel(const uint8_t* 
     }
 }
 
+static bool off_element(const void* p, size_t size) { return reinterpret_cast<uintptr_t>(p) % size != 0; }
+
 static int check_w4_pack(const void* a, const void* packed, const void* scales, int64_t n, int64_t k, int64_t ld,
                          int group) {
     if (!a || !packed || !scales) return set_error(SBQ_ERR_INVALID_ARGUMENT, "null pointer");
@@ -176,6 +178,8 @@ extern "C" int sbq_w4_quantize_pack(const void* w, int w_dtype, int64_t n, int64
     int st = check_w4_pack(w, packed, scales, n, k, ldw, group);
     if (st) return st;
     if (!rowmul) return set_error(SBQ_ERR_INVALID_ARGUMENT, "null rowmul pointer");
+    if (off_element(w, w_dtype == SBQ_F32 ? 4 : 2) || off_element(rowmul, 4))
+        return set_error(SBQ_ERR_ALIGNMENT, "weight and rowmul must be aligned to their element size");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const unsigned grid = (unsigned)(ceil_div(n, kTileRows) * kTileRows);
     uint8_t* out = static_cast<uint8_t*>(packed);
@@ -202,6 +206,8 @@ extern "C" int sbq_w4_pack(const int8_t* q, int64_t ldq, const void* scale, int6
     int st = check_w4_pack(q, packed, scales, n, k, ldq, group);
     if (st) return st;
     if (!scale || !rowmul) return set_error(SBQ_ERR_INVALID_ARGUMENT, "null pointer");
+    if (off_element(scale, 2) || off_element(rowmul, 4))
+        return set_error(SBQ_ERR_ALIGNMENT, "scale and rowmul must be aligned to their element size");
     if (lds < ceil_div(k, group)) return set_error(SBQ_ERR_INVALID_ARGUMENT, "scale row stride smaller than the row");
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     w4_pack_kernel<<<(unsigned)(ceil_div(n, kTileRows) * kTileRows), kPackThreads, 0, s>>>(
@@ -215,6 +221,7 @@ extern "C" int sbq_w4_unpack(const void* packed, const void* scales, int64_t n, 
     int st = check_w4_pack(packed, packed, scales, n, k, q ? ldq : k, group);
     if (st) return st;
     if (scale && lds < ceil_div(k, group)) return set_error(SBQ_ERR_INVALID_ARGUMENT, "scale row stride smaller than the row");
+    if (off_element(scale, 2)) return set_error(SBQ_ERR_ALIGNMENT, "scale must be aligned to its element size");
     if (!q && !scale) return SBQ_OK;
     w4_unpack_kernel<<<(unsigned)n, kPackThreads, 0, static_cast<cudaStream_t>(stream)>>>(
         static_cast<const uint8_t*>(packed), static_cast<const __nv_bfloat16*>(scales), n, k, group, q, ldq,

@@ -172,3 +172,22 @@ def test_buffers_of_another_size_are_not_unpacked(sbq):
         sbq.Int4Linear.from_packed(lin.packed, lin.scales, lin.rowmul[:-1], n, k, None, group)
     with pytest.raises(ValueError, match="one CUDA device"):
         sbq.Int4Linear.from_packed(lin.packed, lin.scales, lin.rowmul, n, k, None, group)
+
+
+def test_packing_of_misaligned_operands(sbq, no_device):
+    """Addresses that are not multiples of the element size are refused, as the products refuse them."""
+    L, at = sbq._lib, BASE
+    bufs = (at, at + 4096, at + 8192)  # packed, scales, rowmul
+
+    def refused(name, *args):
+        status, message = getattr(L.load(), name)(*args, None), L.load().sbq_last_error().decode()
+        return status == L.ERR_ALIGNMENT and "aligned" in message
+
+    w = at + 65536
+    for dtype, off, bad in ((L.F32, 2, True), (L.F32, 4, False), (L.F16, 1, True), (L.BF16, 3, True), (L.BF16, 2, False)):
+        assert refused("sbq_w4_quantize_pack", w + off, dtype, 16, 32, 32, 32, *bufs) == bad
+    assert refused("sbq_w4_quantize_pack", w, L.F32, 16, 32, 32, 32, *bufs[:2], bufs[2] + 2)
+    for scale, row, bad in ((1, 0, True), (2, 0, False), (0, 2, True), (0, 4, False)):
+        assert refused("sbq_w4_pack", w + 1, 32, w + 4096 + scale, 1, 16, 32, 32, *bufs[:2], bufs[2] + row) == bad
+    assert refused("sbq_w4_unpack", *bufs[:2], 16, 32, 32, w + 1, 32, w + 4097, 1)
+    assert not refused("sbq_w4_unpack", *bufs[:2], 16, 32, 32, w + 1, 32, w + 4098, 1)
