@@ -14,6 +14,7 @@ import ctypes
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 
 from . import _lib as L
 from .quant import _DTYPE_CODE, _raw_stream, _written
@@ -61,6 +62,9 @@ def residual_norm(branch: torch.Tensor | None, residual: torch.Tensor, pre_weigh
     refused unless they are the same elements, and so is every overlap with a weight or another gate); with no branch, a residual_scale of 1 and no
     ``residual_out`` the residual is returned as it is.
     """
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None
+                                              for t in (branch, residual, gate, pre_weight, post_weight)):
+        raise ValueError("residual_norm has no gradient: its inputs must not carry forward-mode tangents")
     dev, shape = residual.device, residual.shape
     if dev.type != "cuda":
         raise ValueError("residual_norm runs on a CUDA device, got " + str(dev))

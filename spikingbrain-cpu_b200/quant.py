@@ -440,7 +440,7 @@ class Int4Linear(nn.Module):
 
     x may be fp32, fp16 or bf16 (fp32 enters the product with 22 bits, the others exactly), products are
     summed in fp32, and ``out_dtype`` (fp32 as in the other formats, or fp16 / bf16) is the type of the
-    result.  Frozen like every format here: no gradient flows through it.  State dicts hold ``qweight``
+    result.  Frozen like every format here: no gradient and no forward-mode tangent flows through it.  State dicts hold ``qweight``
     (int8 codes [n, k]) and ``scale`` (bf16 [n, ceil(k / group)]); both are copies of the packed weight, so
     writing into them does not change it (load a state dict, or pack anew).
     """

@@ -191,3 +191,18 @@ def test_packing_of_misaligned_operands(sbq, no_device):
         assert refused("sbq_w4_pack", w + 1, 32, w + 4096 + scale, 1, 16, 32, 32, *bufs[:2], bufs[2] + row) == bad
     assert refused("sbq_w4_unpack", *bufs[:2], 16, 32, 32, w + 1, 32, w + 4097, 1)
     assert not refused("sbq_w4_unpack", *bufs[:2], 16, 32, 32, w + 1, 32, w + 4098, 1)
+
+
+def test_norm_refuses_forward_mode_tangents(sbq):
+    """residual_norm has no gradient in either mode: a dual tensor is refused, whichever operand it is."""
+    import torch.autograd.forward_ad as fwd
+
+    with fwd.dual_level():
+        rows, vec = torch.randn(3, 8), torch.randn(8)
+        dual = fwd.make_dual(rows, torch.ones(3, 8)), fwd.make_dual(vec, torch.ones(8))
+        for branch, residual, kw in ((dual[0], rows, {}), (rows, dual[0], {}), (rows, rows, {"gate": dual[0]}),
+                                     (rows, rows, {"pre_weight": dual[1]}), (rows, rows, {"post_weight": dual[1]})):
+            with pytest.raises(ValueError, match="no gradient"):
+                sbq.residual_norm(branch, residual, **kw)
+        with pytest.raises(ValueError, match="CUDA device"):  # plain tensors within a dual level
+            sbq.residual_norm(rows, rows, vec)
