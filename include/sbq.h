@@ -399,7 +399,9 @@ SBQ_API size_t sbq_linear_w4_workspace_bytes(int64_t m, int64_t n, int64_t k, in
 SBQ_API int sbq_linear_w4_plan(int64_t m, int64_t n, int64_t k, int x_dtype, int matrices, int* plan);
 
 /* y[m, n] = sum_k x[m, k] * q[n, k] * s[n, k / group] (+ bias[n]); x and y SBQ_F32, SBQ_F16 or SBQ_BF16.
- * q * s enters the product exactly, 16-bit x too, fp32 x with 22 bits; sums are fp32.  Up to 16 rows: the
+ * q * s enters the product exactly (above 16 rows: scales down to 2^-27 of the largest of their row), 16-bit x too, fp32 x
+ * with 22 bits; sums are fp32.  fp32 x, and bf16 x above 16 rows, are read as fp16 parts of the scaled row: elements that lie
+ * more than 2^17 (bf16: 2^31) below their row's largest are off by up to 2^-39 of it instead.  Up to 16 rows: the
  * decode product; above: the tensor-memory product.  x rows 16-byte aligned when k is a multiple of 16 (any row stride
  * otherwise), workspace 256-byte aligned (NULL when its size is 0).  y and x must not overlap (columns of one
  * buffer do not). */

@@ -4,7 +4,8 @@
 //   y[t, n] = xinv[t] / rowmul[n] * sum_k xh[t, k] * (q[n, k] s[n, k / group] rowmul[n])  (+ bias[n])
 //
 // xh is x in fp16 (x itself, or its power-of-two-scaled parts, linear_w4.cu), and q * s * rowmul is exact in
-// fp16 (w4.cuh), so the products are those of the definition and the sums are fp32 in tensor memory.
+// fp16 (w4.cuh, down to scales of 2^-27 of the row's largest), so the products are those of the definition and the
+// sums are fp32 in tensor memory.
 //
 // Channels are the MMA's M, tokens its N.  Per 128 columns of k (one packed tile):
 //   * warp 0 (one thread) loads the tokens' x (TMA, 128-byte swizzle), the codes (64 bytes per channel, 64-byte
@@ -20,8 +21,9 @@
 // Tensor-core accumulation truncates: measured on B200, the relative error of a sum grows by about 1.3e-8 per
 // k16 step (1.2e-5 at k = 12288).  Where the result is kept in fp32 the sum is therefore cut into segments
 // of kSegSteps = 32 steps, and each finished segment is added to fp32 registers (round to nearest): 3e-7 (bf16 x) to
-// 6e-7 (fp32 x) at any k from 512 to 12288, with 64 steps 1.2e-6.  16-bit results,
-// whose own rounding (2^-12 and up) is far above it, are summed in one piece.
+// 6e-7 (fp32 x) at any k from 512 to 12288, with 64 steps 1.2e-6.  16-bit results are summed in one piece: that error is
+// relative to the largest partial sum, so it lies far below the result's own rounding (2^-12 or 2^-9 of its value) unless
+// the sum cancels to a few hundredths of its parts or k passes about 100,000.
 //
 // Measured on B200, groups of 128: 4096 x 4096 x 12288 fp16 267 us (1.54 PFLOP/s, 0.93 of cuBLAS's measured bf16 rate),
 // 2048 x 4096 x 12288 fp16 143 us, with fp32 results 167 us (a segment ends in the wait for the accumulator to be read);
@@ -515,8 +517,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
                     float res[16];
 #pragma unroll
                     for (int j = 0; j < 16; ++j) res[j] = buf[j * kW4Rows + (row ^ 64)];
-                    // a 16-bit result: the approximate exponential and division (a few 2^-22) are far below its
-                    // rounding
+                    // a 16-bit result: the approximate exponential (documented to 2 + 1.2 |g| units of 2^-23) and
+                    // division are off by 2^-16 of silu at most, at gates near -87, and by 2^-19 above -10, under its rounding
+                    // of 2^-12 or 2^-9.  The reduction of cut tiles and the few-row kernel, with fewer results to a
+                    // thread, take expf and an exact division
                     if (p.y_dtype == SBQ_F32) {
 #pragma unroll
                         for (int j = 0; j < 16; ++j)

@@ -24,7 +24,8 @@ int w4_sm_count() {
 // fp16 x, and bf16 x up to 16 rows, are read in place when k is a multiple of 16.  Otherwise one launch writes x into
 // the workspace, its rows filled with zeros up to a multiple of 16 columns:
 //   fp32 x               row r times 2^(14 - e), 2^e <= max |x[r]| < 2^(e + 1) over its finite values, as two fp16 parts
-//                        hi + lo (22 bits, the difference x - hi is exact), inv[r] = 2^(e - 14);
+//                        hi + lo (22 bits, the difference x - hi is exact; below 2^-17 of the row's largest 2^-39 of it),
+//                        inv[r] = 2^(e - 14);
 //   bf16 x, over 16 rows the same in one fp16 part (exact unless an element is below 2^-31 of the row's largest);
 //   16-bit x             as it is.
 // Infinities and NaN stay what they are.

@@ -148,8 +148,10 @@ __device__ __forceinline__ float rcp_approx(float v) {
     return r;
 }
 
-// 1 / (1 + 2^(-g log2 e)) from the hardware's power of two and reciprocal: relative error a few 2^-22 where the
-// gate is not 0 or 1 to fp32.  (expf and an exact division made the gated step instruction-bound.)
+// 1 / (1 + 2^(-g log2 e)) from the hardware's power of two and reciprocal, for every type of result.  Relative error at
+// most (2 + 0.32 |g|) 2^-22 for g down to -87, 0 below: the rounding of the exponent (2^-24) and of log2 e (2^-26) count |g|
+// times, the power of two is good to 2^-22, the rest adds about as much.  So a gate of -20 is off by 2e-6 of itself, which
+// is 2e-9; 16-bit results round far above it.  (expf and an exact division made the gated step instruction-bound.)
 __device__ __forceinline__ float sigmoid_approx(float g) { return rcp_approx(1.0f + ex2_approx(-1.44269504f * g)); }
 
 __device__ __forceinline__ void gate_act8(float (&g)[8], int act) {

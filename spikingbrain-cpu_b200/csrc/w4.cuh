@@ -62,6 +62,9 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
     return d;
 }
 
+// The published way from small integers to floats without a conversion instruction: the integer goes into the mantissa
+// under an exponent that makes its last place one, and the implied leading one is subtracted with the offset.
+//
 // Eight codes -> four fp16 pairs of q (exact).  0x6400 | u is 1024 + u; with the code four bits higher
 // it is 1024 + 16 u, so two of the four pairs need no shift: (1024 + 16 u) / 16 - 72 = u - 8.
 __device__ __forceinline__ void w4_to_half(uint32_t w, uint32_t (&h)[4]) {

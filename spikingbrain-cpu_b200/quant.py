@@ -438,7 +438,8 @@ class Int4Linear(nn.Module):
     """Formats ``int4-g32`` / ``int4-g64`` / ``int4-g128``: 4-bit weight, one bf16 scale per output channel and
     group of input features; y = x (q * s)^T + b.
 
-    x may be fp32, fp16 or bf16 (fp32 enters the product with 22 bits, the others exactly), products are
+    x may be fp32, fp16 or bf16 (fp32 enters the product with 22 bits, the others exactly; elements of fp32 rows,
+    and of bf16 rows when there are more than 16, keep an absolute 2^-39 of their row's largest), products are
     summed in fp32, and ``out_dtype`` (fp32 as in the other formats, or fp16 / bf16) is the type of the
     result.  Frozen like every format here: no gradient and no forward-mode tangent flows through it.  State dicts hold ``qweight``
     (int8 codes [n, k]) and ``scale`` (bf16 [n, ceil(k / group)]); both are copies of the packed weight, so

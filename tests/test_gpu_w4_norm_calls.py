@@ -153,3 +153,42 @@ def test_calls_that_write_into_a_tensor_count_as_changes_of_it(sbq, writer):
     with torch.inference_mode():  # tensors without a version
         x = x.clone()
         write()
+
+
+@pytest.mark.parametrize("act", ["sigmoid", "silu"])
+@pytest.mark.parametrize("d", [680, 681, 5441])
+def test_gates_towards_zero(sbq, act, d):
+    """The gated term alone, fp32, for gates whose weight beside a residual would hide their error."""
+    m = 4
+    g = torch.linspace(-85.0, 0.0, m * d, device="cuda").view(m, d)
+    y = 1.0 + rand(m, d, seed=90).abs()
+    r, _ = sbq.residual_norm(y, torch.zeros_like(y), gate=g, gate_act=act, residual_scale=0.0)
+    gd = g.double()
+    ref = y.double() * torch.sigmoid(gd) * (gd if act == "silu" else 1.0)
+    # the exponent -g log2 e is rounded (2^-24) and so is log2 e (2^-26): |g| (2^-24 + 2^-26) = 0.3125 |g| 2^-22 of the power
+    # of two, which is good to 2^-22; the sum, the reciprocal and the products add at most 2^-22 together
+    tol = ref.abs() * (2.0 + 0.32 * gd.abs()) * 2.0 ** -22
+    assert ((r.double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(4, 64, 384), (40, 64, 384), (405, 5433, 272)])
+@pytest.mark.parametrize("x_dtype", [F16, BF16, F32])
+def test_elements_far_below_their_rows_largest(sbq, m, n, k, x_dtype):
+    """A row whose largest element meets zero weights only.  fp32 rows, and bf16 ones of more than 16, are read as fp16
+    parts of the scaled row: what lies far below the largest keeps an absolute 2^-39 of it, and no more."""
+    q = torch.randint(-8, 8, (n, k), device="cuda", dtype=torch.int8, generator=torch.Generator(device="cuda").manual_seed(91))
+    s = (rand(n, -(-k // 64), seed=92).abs() * 0.01 + 0.002).to(BF16)
+    q[:, 5] = 0
+    lin = sbq.Int4Linear.from_quantized(q, s, None, group=64)
+    w = q.double() * s.double().repeat_interleave(64, dim=1)[:, :k]
+    for far in (2.0 ** 10, 2.0 ** 15, 2.0 ** 20, 2.0 ** 30, 2.0 ** 45, 2.0 ** 90):
+        x = rand(m, k, seed=93)
+        x[:, 5] = far if x_dtype != F16 else min(far, 2.0 ** 15)
+        x = x.to(x_dtype)
+        ref = x.double() @ w.t()
+        mags = x.double().abs() @ w.abs().t()
+        steps = (2 if x_dtype == F32 else 1) * -(-k // 16) + -(-k // 128) + 16
+        tol = mags * steps * 2.0 ** -22 + ref.abs() * 2.0 ** -24
+        if x_dtype == F32 or (x_dtype == BF16 and m > 16):
+            tol = tol + mags * 2.0 ** -23 + 2.0 ** -39 * x[:, 5:6].double() * w.abs().sum(1)
+        assert ((lin(x).double() - ref).abs() <= tol).all(), far
