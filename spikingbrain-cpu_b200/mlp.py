@@ -146,7 +146,7 @@ def fuse_gated_mlp(model: nn.Module, h_dtype: torch.dtype = torch.float16) -> in
         parts = [getattr(mod, a, None) for a in ("gate_proj", "up_proj", "down_proj")]
         same = any(all(isinstance(p, kind) for p in parts) for kind in (Int8Linear, Int4Linear))
         if same and getattr(parts[0], "group", None) == getattr(parts[1], "group", None) and parts[0].bias is None \
-                and parts[1].bias is None:
+                and parts[1].bias is None and parts[0].packed.device == parts[1].packed.device:
             parent_name, _, child = name.rpartition(".")
             if not name:
                 raise ValueError("cannot replace the root module in place")

@@ -206,3 +206,15 @@ def test_norm_refuses_forward_mode_tangents(sbq):
                 sbq.residual_norm(branch, residual, **kw)
         with pytest.raises(ValueError, match="CUDA device"):  # plain tensors within a dual level
             sbq.residual_norm(rows, rows, vec)
+
+
+@pytest.mark.parametrize("make", [int4, int8])
+def test_fusing_leaves_a_block_spread_over_devices_alone(sbq, make):
+    model = torch.nn.Module()
+    for name, device in (("together", "cpu"), ("apart", "meta")):
+        block = torch.nn.Module()
+        block.gate_proj, block.up_proj, block.down_proj = make(sbq, 128, 64, "cpu"), make(sbq, 128, 64, device), make(sbq, 64, 128, "cpu")
+        setattr(model, name, block)
+    apart = model.apart
+    assert sbq.fuse_gated_mlp(model) == 1
+    assert isinstance(model.together, sbq.FusedGatedMLP) and model.apart is apart
