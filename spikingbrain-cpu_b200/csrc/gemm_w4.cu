@@ -25,10 +25,14 @@
 // relative to the largest partial sum, so it lies far below the result's own rounding (2^-12 or 2^-9 of its value) unless
 // the sum cancels to a few hundredths of its parts or k passes about 100,000.
 //
-// Measured on B200, groups of 128: 4096 x 4096 x 12288 fp16 267 us (1.54 PFLOP/s, 0.93 of cuBLAS's measured bf16 rate),
-// 2048 x 4096 x 12288 fp16 143 us, with fp32 results 167 us (a segment ends in the wait for the accumulator to be read);
-// gate/up 2048 x 4096 x 12288 291 us with bf16 x.  Long products are bound by the tensor cores; one tile per pair (512 x 4096 x 4096, 24 us) by about 8 us of set-up, first
-// loads and stores and 0.5 us per block of 128 k; 64 x 4096 x 12288 (20 us) by x, read again for every 128 channels.
+// Measured on B200, groups of 128, in bursts of a few ms (the power cap not yet reached): 4096 x 4096 x 12288 fp16 271 us (1.52
+// PFLOP/s, 0.92 of cuBLAS's measured bf16 burst rate), 2048 x 4096 x 12288 fp16 144 us, with fp32 results 170 us (a segment
+// ends in the wait for the accumulator to be read); gate/up 2048 x 4096 x 12288 293 us with bf16 x.  Call after call, under the
+// power cap, 310 to 316 us and 340 to 345 us.  Long products are bound by the tensor cores (active 72 to 75 % of the cycles at
+// the lowered clock); one tile per pair (512 x 4096 x 4096, 24.5 us) by about 8 us of set-up, first loads and stores and
+// 0.5 us per block of 128 k; 64 x 4096 x 12288 (20 us) by x, read again for every 128 channels (100 MB of L2 traffic for 27 of
+// weight).  The gate/up instances of the pair kernel spill up to 180 bytes a thread in the takers' exchange, once per tile
+// and beside the MMAs (0.7 % of all instructions).
 #include "tc.cuh"
 #include "w4_host.cuh"
 

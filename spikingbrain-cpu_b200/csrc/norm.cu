@@ -11,7 +11,8 @@
 //
 // The bytes bound it.  Measured on B200: 8192 x 4096, fp32 in and fp16 out, without a post norm 69.5 us (6.8 TB/s, 1.03 of
 // the measured copy rate), with it 75 us; 1 x 4096 2.9 us (a launch); 16-bit rows with a gate per element, which have
-// half the bytes per element and twice the arithmetic, 3001 x 2560 19.7 us (3.9 TB/s) and 3001 x 2559 29 us.
+// half the bytes per element and twice the arithmetic, 3001 x 2560 19.7 us (3.9 TB/s) and 3001 x 2559 29 us (up to 22 and
+// 34 on some boxes): there instruction issue bounds it (75 to 78 % of the slots, 64 and 102 instructions per 32 elements).
 #include "w4_host.cuh"
 
 namespace sbq {
@@ -587,7 +588,8 @@ static cudaError_t launch_norm_long(const NormParams& p, cudaStream_t s) {
 
 // In registers, one chunk per thread up to 8192 columns (1024 threads), on as many warps as the row fills: two chunks
 // hold twice the registers (8192 x 4096 fp32 with both norms 75 and 78 us).  What hides a row's chain of loads and sums is
-// other rows on the SM, so registers are held down to what norm_ctas needs (8192 x 8192 fp32: one CTA per SM 219, two 160 us).
+// other rows on the SM, so registers are held down to what norm_ctas needs (8192 x 8192 fp32: one CTA per SM 219, two 160 us;
+// the gated kernels then spill 24 to 104 bytes a thread, staged ones 32 to 84, which is 2 to 3 % of their instructions).
 // Measured on B200, in registers and staged, two norms and a full gate in bf16: 3001 x 2560 22.2 and 19.7 us, 3001 x 2559
 // 35.6 and 29.1, 3001 x 6144 58.8 and 44.5, 3001 x 8191 174 and 77, 3001 x 20480 241 and 184; one wave of rows or less is
 // faster in registers (592 x 4096 7.7 and 9.8 us: a thread's chunks come one after the other), and so are fp32 rows (3001 x
