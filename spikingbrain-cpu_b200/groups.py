@@ -9,7 +9,10 @@ streams them all with a single read of x and one launch.  ``fuse_shared_inputs``
 ``GroupMember`` modules in the members' places: the first member called with a given x runs the
 whole group, the others return their slice of that result, so the reference's model code runs
 unchanged.  A result is handed out once per computation; a member called again (or with another
-x) recomputes.  The result and x are held until every member has been called.  Members' outputs are
+x, an x changed in place, on another stream, or inside a graph capture after a call outside of it)
+recomputes.  The result and x are held until every member has been called: a graph should be captured
+around calls of all of them.  An x made under ``torch.inference_mode`` has no version to tell changes by
+and is refused by torch; ``torch.no_grad`` does not have this limit.  Members' outputs are
 column views of the group's [m, padded N] result.
 
 The int8 formats and the int4 ones are supported (all members of one group share the format, and the
@@ -24,7 +27,12 @@ import torch
 import torch.nn as nn
 
 from . import _lib as L
-from .quant import DynamicInt8Linear, Int4Linear, Int8Linear, _DTYPE_CODE, _prepare_x, _ptr, _stream, _workspace
+from .quant import DynamicInt8Linear, Int4Linear, Int8Linear, _DTYPE_CODE, _prepare_x, _ptr, _raw_stream, _stream, _workspace
+
+
+def _context(x: torch.Tensor) -> tuple:
+    """What a result computed now is ordered with: the current stream, and whether a graph is being captured on it."""
+    return (_raw_stream(x.device), torch.cuda.is_current_stream_capturing()) if x.is_cuda else ()
 
 
 class SharedInputGroup(nn.Module):
@@ -120,7 +128,7 @@ class SharedInputGroup(nn.Module):
     def member_output(self, index: int, x: torch.Tensor) -> torch.Tensor:
         # x itself is kept while its result is: a tensor that has been freed may come back with the same id, address and
         # version as another input
-        key = (x.data_ptr(), x._version, tuple(x.shape), x.dtype, x.device)
+        key = (x.data_ptr(), x._version, tuple(x.shape), x.dtype, x.device, *_context(x))
         if self._result is None or self._key[0] is not x or self._key[1:] != key or index in self._handed:
             self._result = self.forward_all(x)
             self._key, self._handed = (x, *key), set()

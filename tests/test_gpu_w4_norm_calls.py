@@ -192,3 +192,44 @@ def test_elements_far_below_their_rows_largest(sbq, m, n, k, x_dtype):
         if x_dtype == F32 or (x_dtype == BF16 and m > 16):
             tol = tol + mags * 2.0 ** -23 + 2.0 ** -39 * x[:, 5:6].double() * w.abs().sum(1)
         assert ((lin(x).double() - ref).abs() <= tol).all(), far
+
+
+@pytest.mark.parametrize("fmt", ["int4-g64", "int8"])
+def test_group_members_called_on_streams_and_in_graphs(sbq, fmt):
+    """A kept result belongs to the stream, and the graph or not, that it was computed in: elsewhere a member computes anew."""
+    parent, names = torch.nn.Module(), ["q_proj", "k_proj"]
+    lins = [sbq.make_linear(fmt, rand(48, 128, seed=80 + i)) for i in range(2)]
+    for name, lin in zip(names, lins):
+        setattr(parent, name, lin)
+    group = sbq.groups.fuse_shared_inputs(parent, names)
+    computed = []
+    forward_all = group.forward_all
+    group.forward_all = lambda x: computed.append(x) or forward_all(x)
+
+    def same(got, want):
+        return (got - want).norm() <= 2.0 ** -18 * want.norm()
+
+    x, side = rand(3, 128, seed=82, dtype=F16), torch.cuda.Stream()
+    parent.q_proj(x)
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = parent.k_proj(x)
+    torch.cuda.synchronize()
+    assert len(computed) == 2 and same(got, lins[1](x))
+    # one member before the capture, the other one in it: the graph holds the product, of x as it is at each replay
+    y = rand(3, 128, seed=83, dtype=F16)
+    graph = torch.cuda.CUDAGraph()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        parent.q_proj(y)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=side):
+        out = parent.k_proj(y)
+    with torch.cuda.stream(side):
+        after = parent.q_proj(y)  # and nothing of the graph's goes to an eager call
+    torch.cuda.synchronize()
+    assert same(after, lins[0](y))
+    for seed in (84, 85):
+        y.copy_(rand(3, 128, seed=seed, dtype=F16))
+        graph.replay()
+        assert same(out, lins[1](y))
