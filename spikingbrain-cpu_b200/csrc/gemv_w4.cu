@@ -16,7 +16,7 @@
 // registers leave one CTA per SM).
 //
 // Measured on B200, groups of 128: 1 x 2560 x 151936 42 us with fp16 x (4.8 TB/s of weight and scales, 0.73 of the copy
-// rate) and 47 us with bf16; gate/up 1 x 4096 x 12288 14.6 us (3.6 TB/s; up to 19 on some boxes); 1 x 4096 x 4096
+// rate) and 47 us with bf16; gate/up 1 x 4096 x 12288 14.6 us (3.6 TB/s; up to 19 on some machines); 1 x 4096 x 4096
 // 4.5 us, of which an empty launch is 2.6.  Long launches are bound by instruction issue: 141 instructions per 1 KiB tile
 // (bf16 157), 72 (88) of them the conversion, at 2.4 per cycle and SM (counted with ncu on the first two).
 #include "w4.cuh"

@@ -12,7 +12,7 @@
 // The bytes bound it.  Measured on B200: 8192 x 4096, fp32 in and fp16 out, without a post norm 69.5 us (6.8 TB/s, 1.03 of
 // the measured copy rate), with it 75 us; 1 x 4096 2.9 us (a launch); 16-bit rows with a gate per element, which have
 // half the bytes per element and twice the arithmetic, 3001 x 2560 19.7 us (3.9 TB/s) and 3001 x 2559 29 us (up to 22 and
-// 34 on some boxes): there instruction issue bounds it (75 to 78 % of the slots, 64 and 102 instructions per 32 elements).
+// 34 on some machines): there instruction issue bounds it (75 to 78 % of the slots, 64 and 102 instructions per 32 elements).
 #include "w4_host.cuh"
 
 namespace sbq {
